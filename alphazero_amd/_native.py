@@ -12,6 +12,8 @@ LIB_PATH = os.environ.get("AZAMD_LIB") or os.path.join(_HERE, "libazamd.so")
 AZ_OK, AZ_ERR_ARG, AZ_ERR_HIP, AZ_ERR_STATE, AZ_ERR_ILLEGAL, AZ_ERR_NOCHILD, AZ_ERR_CAPACITY = 0, -1, -2, -3, -4, -5, -6
 AZ_FEAT_F32_NCHW, AZ_FEAT_BF16_NHWC = 0, 1
 AZ_NET_BF16, AZ_NET_F32 = 0, 1
+AZ_DT_F32, AZ_DT_BF16, AZ_DT_F16, AZ_DT_I8 = 0, 1, 2, 3
+AZ_REDUCE_NONE, AZ_REDUCE_MEAN, AZ_REDUCE_SUM = 0, 1, 2
 
 
 class AzConfig(C.Structure):
@@ -39,6 +41,19 @@ class AzLaneResult(C.Structure):
     _fields_ = [("counters", C.c_int64 * 8), ("host_seconds_rng", C.c_double), ("n_over", C.c_int32), ("over_slot", C.c_void_p),
                 ("over_winner", C.c_void_p), ("bits", C.c_void_p), ("caps", C.c_void_p), ("pi32", C.c_void_p),
                 ("to_play", C.c_void_p), ("difficulty", C.c_void_p), ("actions", C.c_void_p), ("root_value", C.c_void_p)]
+
+
+class AzLinearCeArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64),
+                ("features", C.c_int64), ("classes", C.c_int64), ("x_pitch", C.c_int64), ("weight_pitch", C.c_int64),
+                ("target_pitch", C.c_int64), ("ignore_index", C.c_int64), ("dtype", C.c_int32), ("target_dense", C.c_int32),
+                ("reduction", C.c_int32), ("entropy_coeff", C.c_float)]
+
+
+class AzInt8Args(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("x_scale", C.c_void_p), ("weight_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("y", C.c_void_p), ("tokens", C.c_int64), ("features", C.c_int64), ("channels", C.c_int64), ("x_pitch", C.c_int64),
+                ("weight_pitch", C.c_int64), ("x_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("y_dtype", C.c_int32)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/azamd.h
@@ -104,6 +119,13 @@ SIGNATURES = {
     "az_rng_seed": (_I32, [_VP, _I32, C.c_uint32]),
     "az_rng_dirichlet": (_I32, [_VP, _VP, C.c_double, _VP, _I32, _I32]),
     "az_rng_random_sample": (_I32, [_VP, _VP, _VP]),
+    "az_linear_ce_workspace": (_I64, [C.POINTER(AzLinearCeArgs), _I32]),
+    "az_linear_ce_forward": (_I32, [C.POINTER(AzLinearCeArgs), _VP, _VP, _VP, _VP, _VP, _I64, _VP]),
+    "az_linear_ce_backward": (_I32, [C.POINTER(AzLinearCeArgs), _VP, _VP, _VP, _VP, _VP, _VP, _I64, _VP]),
+    "az_dropout": (_I32, [_VP, _VP, _VP, _I64, _I32, _I32, C.c_uint64, _VP, C.c_uint64, _VP]),
+    "az_quantize_rows": (_I32, [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
+    "az_int8_workspace": (_I64, [C.POINTER(AzInt8Args)]),
+    "az_int8_linear": (_I32, [C.POINTER(AzInt8Args), _VP, _I64, _VP]),
 }
 
 _lib = None

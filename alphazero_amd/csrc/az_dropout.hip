@@ -1,0 +1,131 @@
+// Dropout whose mask is a function of (seed, offset, position) and is never stored (az_dropout).
+//
+// Positions go in groups of 8 in row-major order. Group g's 128 bits are Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel
+// random numbers: as easy as 1, 2, 3; 2011) of the counter (g, offset) under the key seed; position i takes 16 of them, the low
+// half of word (i % 8) / 2 first. It is kept where they are at least t = round(65536 p), times 65536 / (65536 - t): the scale
+// belongs to the probability that is really used, so the expectation is exact. The backward pass makes the same bits again.
+//
+// Bound by memory: 2 to 3 arrays of the input's size. 16 bits per element instead of 32 halve the integer work (20 32 x 32 -> 64
+// bit products per group), which would otherwise cost more time than the memory.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/azamd.h"
+#include "az_types.cuh"
+
+namespace az {
+int fail(int code, const std::string& msg);
+
+namespace {
+
+__device__ __forceinline__ void philox(uint64_t group, uint64_t offset, uint64_t seed, uint32_t (&w)[4]) {
+    uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
+    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)b;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    w[0] = c0;
+    w[1] = c1;
+    w[2] = c2;
+    w[3] = c3;
+}
+
+struct DropArgs {
+    const void *x, *residual;   // residual may be null
+    void* y;
+    int64_t count;
+    const uint64_t* seed_dev;   // null: seed
+    uint64_t seed, offset;
+    uint32_t threshold;
+    float scale;
+};
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (DT == DT_F32) {
+        const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = *(const uint4*)((const uint16_t*)p + i);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[2 * e] = from_bits<DT>((uint16_t)u[e]), v[2 * e + 1] = from_bits<DT>((uint16_t)(u[e] >> 16));
+    }
+}
+
+template <int DT, bool RES, bool WIDE>
+__global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
+    const int64_t group = (int64_t)blockIdx.x * 256 + threadIdx.x, i = group * 8;
+    if (i >= a.count) return;
+    uint32_t w[4];
+    const bool whole = WIDE && i + 8 <= a.count;
+    float v[8], r[8];
+    if (whole) {
+        load8<DT>(a.x, i, v);
+        if constexpr (RES) load8<DT>(a.residual, i, r);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = i + e < a.count ? load_scalar<DT>(a.x, i + e) : 0.0f;
+            if constexpr (RES) r[e] = i + e < a.count ? load_scalar<DT>(a.residual, i + e) : 0.0f;
+        }
+    }
+    philox((uint64_t)group, a.offset, a.seed_dev ? *a.seed_dev : a.seed, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+        v[e] = bits >= a.threshold ? v[e] * a.scale : 0.0f;     // a select: what is dropped may be anything
+        if constexpr (RES) v[e] += r[e];
+    }
+    if (whole) {
+        store4<DT>(a.y, i, v[0], v[1], v[2], v[3]);
+        store4<DT>(a.y, i + 4, v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i + e < a.count) store_scalar<DT>(a.y, i + e, v[e]);
+    }
+}
+
+template <int DT>
+void launch(const DropArgs& a, hipStream_t st) {
+    const bool wide = (((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.residual) & 15) == 0;
+    const dim3 grid((unsigned)((a.count + 2047) / 2048)), block(256);
+    if (a.residual) {
+        if (wide) hipLaunchKernelGGL((k_dropout<DT, true, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_dropout<DT, true, false>), grid, block, 0, st, a);
+    } else {
+        if (wide) hipLaunchKernelGGL((k_dropout<DT, false, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_dropout<DT, false, false>), grid, block, 0, st, a);
+    }
+}
+
+}  // namespace
+}  // namespace az
+
+using namespace az;
+
+extern "C" int az_dropout(const void* x, const void* residual, void* y, int64_t count, int32_t dtype, int32_t threshold, uint64_t seed,
+                          const uint64_t* seed_dev, uint64_t offset, void* stream) {
+    if (dtype != AZ_DT_F32 && dtype != AZ_DT_BF16 && dtype != AZ_DT_F16) return fail(AZ_ERR_ARG, "dtype is float32, bfloat16 or float16");
+    if (threshold < 0 || threshold > 65536) return fail(AZ_ERR_ARG, "threshold is 0..65536");
+    if (count < 0 || count > (int64_t(1) << 40)) return fail(AZ_ERR_ARG, "count is 0..2^40");
+    if (count == 0) return AZ_OK;
+    if (!x || !y) return fail(AZ_ERR_ARG, "null argument");
+    const DropArgs a{x, residual, y, count, seed_dev, seed, offset, (uint32_t)threshold, threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == AZ_DT_F32) launch<DT_F32>(a, st);
+    else if (dtype == AZ_DT_BF16) launch<DT_BF16>(a, st);
+    else launch<DT_F16>(a, st);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string("k_dropout: ") + hipGetErrorString(e));
+}

@@ -1,0 +1,176 @@
+// Tile loop of the matrix products of the head operators (az_head.hip, az_int8.hip): C[p][q] = sum_k P[p][k] * Q[q][k], both
+// operands with k contiguous, 16-bit floats or 8-bit integers, accumulated in 32 bits.
+//
+// A workgroup owns BP x BQ results and walks k in steps of 128 bytes (64 16-bit or 128 8-bit values). A step's BP + BQ rows of
+// 128 bytes go from global memory to LDS without passing through registers (buffer_load_dwordx4 ... lds, 1 KB = 8 rows per wave
+// and instruction), two stages in LDS. The load writes a wave's 64 x 16 bytes contiguously, so the bank permutation is made on
+// the global side: the lane that writes 16-byte piece c of row r fetches piece c ^ (r & 7), and a fragment read (16 rows, one
+// piece each) then touches all banks evenly. Reads behind the last row or the last k of a matrix are turned into zeros by the
+// buffer descriptor's range check, so ragged sizes need no other code.
+//
+// P is the matrix instruction's row operand: lane l then holds results p = 4 * (l >> 4) + 0..3 of column q = l & 15 of each
+// 16 x 16 tile, i.e. four neighbouring p of one q. Callers put the axis that is contiguous in their output (classes, features)
+// on P, and a softmax over P is mostly inside a lane.
+//
+// float32 operands come as three 16-bit planes (az_split3): h + m + l with 8 significant bits each. Six of the nine products of
+// planes are summed (the other three are below 2^-25 of the result), smallest first, by walking k six times with other plane
+// pairs: 2.5 PFLOP/s / 6 against the 0.16 PFLOP/s of the float32 matrix instructions.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace az {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum { MM_BF16 = 0, MM_F16 = 1, MM_I8 = 2 };
+
+struct MmOperand {
+    const char* base;    // 16-byte aligned
+    int64_t pitch;       // bytes between rows, a multiple of 16, at most MM_MAX_PITCH
+    int64_t plane;       // bytes between the planes of a split float32 operand
+    int32_t rows;
+};
+constexpr int64_t MM_MAX_PITCH = (int64_t(1) << 31) / 256 - 16;   // 256 rows of a tile stay below 2^31 bytes
+
+template <int KIND> struct MmAcc { typedef f32x4 type; };
+template <> struct MmAcc<MM_I8> { typedef i32x4 type; };
+
+template <int KIND>
+__device__ __forceinline__ typename MmAcc<KIND>::type mm_mfma(i32x4 a, i32x4 b, typename MmAcc<KIND>::type c) {
+    if constexpr (KIND == MM_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else if constexpr (KIND == MM_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+template <int BP_, int BQ_, int WP_, int WQ_, int KIND_>
+struct MmTile {
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, KIND = KIND_;
+    static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
+    static constexpr int TP = BP / WP, TQ = BQ / WQ;          // a wave's share
+    static constexpr int FP = TP / 16, FQ = TQ / 16;
+    static constexpr int LP = BP / 8 / WAVES, LQ = BQ / 8 / WAVES;   // 1 KB loads of a wave per stage
+    static constexpr int STAGE = (BP + BQ) * 128;
+    static constexpr int LDS = 2 * STAGE;
+    static_assert(BP % (8 * WAVES) == 0 && BQ % (8 * WAVES) == 0 && TP % 16 == 0 && TQ % 16 == 0, "tile shape");
+    typedef typename MmAcc<KIND>::type acc_t;
+};
+
+// Planes of step s of 6 (P, Q), smallest product first: (l,h) (h,l) (m,m) (m,h) (h,m) (h,h).
+__device__ __forceinline__ int mm_plane_p(int s) { return (0x001102 >> (4 * s)) & 3; }
+__device__ __forceinline__ int mm_plane_q(int s) { return (0x010120 >> (4 * s)) & 3; }
+
+// One tile: acc[i][j] = results p = p0 + wp * TP + 16 i + 4 (lane >> 4) + 0..3, q = q0 + wq * TQ + 16 j + (lane & 15), where
+// wave = wp * WQ + wq. kbytes: bytes of k per row (a multiple of 16). k_first / k_last: the 128-byte steps [k_first, k_last) of
+// the walk over `segments` times ceil(kbytes / 128) steps that this workgroup takes. All lanes of the workgroup call it; on
+// return every wave has read its last fragment and passed a barrier, so the LDS may be used for something else.
+template <class T>
+__device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, int64_t p0, int64_t q0, int kbytes, int k_first, int k_last,
+                                        bool split, char* lds, typename T::acc_t (&acc)[T::FP][T::FQ]) {
+#ifdef __HIP_DEVICE_COMPILE__   // the buffer resource type exists on the device only
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave / T::WQ, wq = wave % T::WQ;
+    const int ksteps = (kbytes + 127) >> 7;
+    const int row8 = lane >> 3, piece = (lane & 7) ^ row8;
+    const int pp = (int)P.pitch, qp = (int)Q.pitch;
+    int offp[T::LP], offq[T::LQ];
+#pragma unroll
+    for (int i = 0; i < T::LP; ++i) offp[i] = ((wave + i * T::WAVES) * 8 + row8) * pp + piece * 16;
+#pragma unroll
+    for (int i = 0; i < T::LQ; ++i) offq[i] = ((wave + i * T::WAVES) * 8 + row8) * qp + piece * 16;
+    const char* const pbase = P.base + p0 * P.pitch;
+    const char* const qbase = Q.base + q0 * Q.pitch;
+    // bytes from the tile's first row to the end of the matrix' last row; below zero (an empty tile) reads nothing
+    const int64_t pext = ((int64_t)P.rows - p0 - 1) * P.pitch + kbytes, qext = ((int64_t)Q.rows - q0 - 1) * Q.pitch + kbytes;
+    int ks = split ? k_first / ksteps : 0;      // segment and step within it of the next stage to fetch
+    int kk = k_first - ks * ksteps;
+
+    auto fetch = [&](int stage) {
+        const int k = kk << 7;
+        const char* pb = pbase + k;
+        const char* qb = qbase + k;
+        if (split) {
+            pb += mm_plane_p(ks) * P.plane;
+            qb += mm_plane_q(ks) * Q.plane;
+        }
+        const int64_t pn = pext - k, qn = qext - k;
+        const int pr = pn < 0 ? 0 : (pn > 0x7fffffff ? 0x7fffffff : (int)pn), qr = qn < 0 ? 0 : (qn > 0x7fffffff ? 0x7fffffff : (int)qn);
+        const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)pb, 0, pr, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, qr, 0x00020000);
+        // pieces behind the row's end would read the next row: sent out of range instead
+        const int past = k + piece * 16 >= kbytes ? (int)0x80000000 : 0;
+        char* dst = lds + stage * T::STAGE + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < T::LP; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + i * T::WAVES * 1024), 16, offp[i] | past, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::LQ; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(dst + T::BP * 128 + i * T::WAVES * 1024), 16, offq[i] | past, 0, 0, 0);
+        if (++kk == ksteps) {
+            kk = 0;
+            ++ks;
+        }
+    };
+    // fragment reads: 16 rows x 16 bytes, half h of the step; piece h * 4 + (lane >> 4) of row r sits at piece ^ (r & 7)
+    const int frow = lane & 15, fq4 = lane >> 4;
+    const int sw0 = ((fq4 ^ (frow & 7)) * 16), sw1 = (((4 + fq4) ^ (frow & 7)) * 16);
+    const int rdp = (wp * T::TP + frow) * 128, rdq = T::BP * 128 + (wq * T::TQ + frow) * 128;
+    auto read = [&](int stage, int h, i32x4 (&a)[T::FP], i32x4 (&b)[T::FQ]) {
+        const char* s = lds + stage * T::STAGE + (h ? sw1 : sw0);
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) a[i] = *(const i32x4*)(s + rdp + i * 2048);
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) b[j] = *(const i32x4*)(s + rdq + j * 2048);
+    };
+    auto multiply = [&](const i32x4 (&a)[T::FP], const i32x4 (&b)[T::FQ]) {
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FQ; ++j) acc[i][j] = mm_mfma<T::KIND>(a[i], b[j], acc[i][j]);
+    };
+    // every load of this wave has landed and every fragment read has returned, for all waves
+    auto meet = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+#pragma unroll
+    for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) acc[i][j] = typename T::acc_t{};
+    const int n = k_last - k_first;
+    if (n <= 0) return;
+    i32x4 a0[T::FP], b0[T::FQ], a1[T::FP], b1[T::FQ];
+    fetch(0);
+    meet();
+    if (n > 1) fetch(1);
+    read(0, 0, a0, b0);
+    int s = 0;
+    for (int t = 0; t < n; ++t) {
+        read(s, 1, a1, b1);
+        multiply(a0, b0);
+        meet();                              // stage t + 1 is in LDS, stage t has been read by all
+        if (t + 2 < n) fetch(s);
+        s ^= 1;
+        if (t + 1 < n) read(s, 0, a0, b0);
+        multiply(a1, b1);
+    }
+    meet();
+#endif
+}
+
+// Workgroup id -> tile (p, q): consecutive ids go round the 8 XCDs, so each XCD gets a contiguous stretch of the walk, and the
+// walk goes through groups of 8 p tiles with q outermost inside a group: the 32 tiles that an XCD works on at a time are about
+// 8 x 4, which read 12 operand strips through its L2 instead of 33.
+__device__ __forceinline__ void mm_place(int id, int tiles_p, int tiles_q, int& tp, int& tq) {
+    const int total = tiles_p * tiles_q, per = total >> 3, rest = total & 7;
+    const int xcd = id & 7, at = id >> 3;
+    const int l = xcd * per + (xcd < rest ? xcd : rest) + at;
+    const int group = l / (8 * tiles_q), in = l - group * 8 * tiles_q;
+    const int width = tiles_p - group * 8 < 8 ? tiles_p - group * 8 : 8;
+    tp = group * 8 + in % width;
+    tq = in / width;
+}
+
+}  // namespace az

@@ -1,0 +1,977 @@
+// Loss of a linear layer over many classes, with its gradient, without ever holding the logits (az_linear_ce_*).
+//
+//   z = x W^T + b            [rows, classes]
+//   lse_i = log sum_j exp z_ij,  p_ij = exp(z_ij - lse_i),  H_i = lse_i - sum_j p_ij z_ij
+//   L_i = T_i lse_i - sum_j pi_ij z_ij - c H_i,   T_i = sum_j pi_ij   (an index target is pi = one at that class)
+//   G_ij = dL_i/dz_ij = T_i p_ij - pi_ij + c p_ij (log p_ij + H_i)
+//   dx = G W,  dW = G^T x,  db_j = sum_i G_ij
+//
+// Forward: one product whose tiles end in (max, sum of exp, sum of exp * (z - max), sum of pi z) per row, joined per row by a second
+// kernel. Backward: the classes in pieces; per piece the logits are made again, turned into G (16 bits, in both orientations), and
+// two products take it to dx and dW. Bound by the matrix instructions: 2 N V D forward, 6 N V D backward.
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/azamd.h"
+#include "az_gemm.cuh"
+#include "az_types.cuh"
+
+namespace az {
+int fail(int code, const std::string& msg);
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// ------------------------------------------------------------------------------------------------ operands
+// Copies a [rows, cols] matrix (any row stride, any alignment) into rows of `pitch` bytes, zeros behind the last column; float32
+// is split into three planes. One thread writes 16 bytes per plane. Bound by memory; only operands that the tile loop cannot read
+// in place come here (float32, rows that do not start at multiples of 16 bytes).
+struct PackJob {
+    const void* src;
+    int64_t src_pitch;    // elements
+    int32_t rows, cols;
+    char* dst;
+    int64_t pitch, plane;   // bytes
+    __host__ __device__ int64_t blocks() const { return (rows * (pitch >> 4) + 255) / 256; }
+};
+
+template <int DT>
+__device__ __forceinline__ void pack_block(const PackJob& j, int64_t block) {
+    const int pieces = (int)(j.pitch >> 4);
+    const int64_t at = block * 256 + threadIdx.x;
+    if (at >= (int64_t)j.rows * pieces) return;
+    const int64_t r = at / pieces;
+    const int c0 = (int)(at - r * pieces) * 8;
+    __align__(16) uint16_t h[3][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = c0 + e;
+        if constexpr (DT == DT_F32) {
+            const float v = c < j.cols ? ((const float*)j.src)[r * j.src_pitch + c] : 0.0f;
+            split3(v, h[0][e], h[1][e], h[2][e]);
+        } else {
+            h[0][e] = c < j.cols ? ((const uint16_t*)j.src)[r * j.src_pitch + c] : (uint16_t)0;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < (DT == DT_F32 ? 3 : 1); ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + c0 * 2) = *(const uint4*)h[p];
+}
+
+// The same, transposed: dst row c = column c of the source, rows behind the last one (up to the pitch, a multiple of 128 bytes) zero;
+// rows that do not count (target equal to ignore) become zeros too, so that whatever a padded row holds - NaN included - stays out of
+// dW. 64 x 64 elements per workgroup through LDS.
+struct TurnJob {
+    const void* src;
+    int64_t src_pitch;
+    int32_t rows, cols;
+    char* dst;
+    int64_t pitch, plane;
+    const int64_t* target;   // null: every row counts
+    int64_t ignore;
+    __host__ __device__ int64_t blocks() const { return (int64_t)((cols + 63) / 64) * (pitch / 128); }
+};
+
+template <int DT>
+__device__ __forceinline__ void turn_block(const TurnJob& j, int64_t block, uint16_t (*tile)[64][66]) {
+    constexpr int NP = DT == DT_F32 ? 3 : 1;
+    const int across = (j.cols + 63) / 64;
+    const int64_t r0 = block / across * 64;
+    const int c0 = (int)(block % across) * 64;
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = i >> 6, c = i & 63;
+        const bool in = r0 + r < j.rows && c0 + c < j.cols && !(j.target && j.target[r0 + r] == j.ignore);
+        if constexpr (DT == DT_F32) {
+            const float v = in ? ((const float*)j.src)[(r0 + r) * j.src_pitch + c0 + c] : 0.0f;
+            split3(v, tile[0][r][c], tile[1][r][c], tile[2][r][c]);
+        } else {
+            tile[0][r][c] = in ? ((const uint16_t*)j.src)[(r0 + r) * j.src_pitch + c0 + c] : (uint16_t)0;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int c = i >> 3, piece = i & 7;
+        if (c0 + c >= j.cols) continue;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            __align__(16) uint16_t h[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = tile[p][piece * 8 + e][c];
+            *(uint4*)(j.dst + p * j.plane + (int64_t)(c0 + c) * j.pitch + (r0 + piece * 8) * 2) = *(const uint4*)h;
+        }
+    }
+}
+
+// All copies that a piece needs in one launch: they are independent and mostly small.
+struct PackArgs {
+    PackJob w, x;
+    TurnJob wt, xt;
+    int64_t end_w, end_x, end_wt;     // workgroups up to each
+};
+
+template <int DT>
+__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
+    __shared__ __align__(16) uint16_t tile[DT == DT_F32 ? 3 : 1][64][66];
+    const int64_t id = blockIdx.x;
+    if (id < a.end_w) pack_block<DT>(a.w, id);
+    else if (id < a.end_x) pack_block<DT>(a.x, id - a.end_w);
+    else if (id < a.end_wt) turn_block<DT>(a.wt, id - a.end_x, tile);
+    else turn_block<DT>(a.xt, id - a.end_wt, tile);
+}
+
+// ------------------------------------------------------------------------------------------------ shared arguments
+// Adds a part (max, sum e, sum e (z - max), sum pi z) to one whose maximum o[0] is already the largest of all.
+__device__ __forceinline__ void join_part(f32x4& o, const f32x4& v) {
+    if (v[0] == -INFINITY) {
+        o[1] += v[1];       // nothing, or the NaN of a logit that is none
+    } else {
+        const float d = v[0] - o[0], e = __builtin_amdgcn_exp2f(d * LOG2E);
+        o[1] += v[1] * e;
+        o[2] += e == 0.0f ? 0.0f : (v[2] + v[1] * d) * e;
+    }
+    o[3] += v[3];
+}
+
+struct Rows {               // what a row's target says
+    const int64_t* index;   // [rows] or null
+    const float* dense;     // [rows, classes] with row stride dense_pitch, or null
+    int64_t dense_pitch;
+    int64_t ignore;
+    int32_t rows, classes;
+    float entropy;          // c
+};
+
+struct StatArgs {
+    MmOperand w, x;
+    Rows t;
+    const void* bias;
+    int32_t kbytes, segments;
+    int32_t v0;             // first class of the piece that w starts at
+    int32_t tile0, tiles;   // first tile of the piece, tiles of all classes
+    f32x4* part;            // [rows][tiles] (max, sum e, sum e (z - max), sum pi z)
+    float* tpart;           // dense: [rows][tiles][2] sum pi, sum |pi|
+    float* zt;              // index: [rows] logit of the target
+    int32_t tiles_p, tiles_q;
+};
+
+template <class T, int DT>
+__device__ __forceinline__ void add_bias(const void* bias, int64_t p0, int wp, int lane, int v0, int classes, typename T::acc_t (&acc)[T::FP][T::FQ]) {
+    if (bias) {
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) {
+            const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4 + v0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float b = m + r < classes ? load_scalar<DT>(bias, m + r) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < T::FQ; ++j) acc[i][j][r] += b;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <class T, int DT, bool DENSE, bool ENT>
+__global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
+    __shared__ __align__(16) char lds[T::LDS];
+    int tp, tq;
+    mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
+    const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
+    typename T::acc_t acc[T::FP][T::FQ];
+    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
+    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    add_bias<T, DT>(a.bias, p0, wp, lane, a.v0, a.t.classes, acc);
+    const int left = a.t.classes - a.v0 - (int)p0 - wp * T::TP - (lane >> 4) * 4;   // classes from this lane's first one on
+    f32x4* const joint = (f32x4*)lds;                       // [WP][BQ]
+    float* const jt = (float*)(lds + T::WP * T::BQ * 16);   // [WP][BQ][2]
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (i * 16 + r >= left) acc[i][j][r] = -INFINITY;
+                top = fmaxf(top, acc[i][j][r]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f, s = 0.0f, dot = 0.0f, pi_sum = 0.0f, pi_abs = 0.0f;
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float d = acc[i][j][r] - base;
+                const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+                l += e;
+                if constexpr (ENT) s += e == 0.0f ? 0.0f : e * d;   // 0 * -inf of a class that cannot be
+            }
+        if constexpr (DENSE) {
+            if (n < a.t.rows) {
+                const float* pi = a.t.dense + n * a.t.dense_pitch + a.v0 + p0 + wp * T::TP + (lane >> 4) * 4;
+#pragma unroll
+                for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i * 16 + r < left) {
+                            const float v = pi[i * 16 + r];
+                            pi_sum += v;
+                            pi_abs += fabsf(v);
+                            dot += v == 0.0f ? 0.0f : v * acc[i][j][r];
+                        }
+            }
+        } else if (n < a.t.rows) {
+            const int64_t at = a.t.index[n] - (a.v0 + p0 + wp * T::TP + (lane >> 4) * 4);
+            if (at >= 0 && at < T::TP && at < left) {
+#pragma unroll
+                for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at == i * 16 + r) a.zt[n] = acc[i][j][r];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o < 64; o *= 2) {
+            l += __shfl_xor(l, o);
+            if constexpr (ENT) s += __shfl_xor(s, o);
+            if constexpr (DENSE) {
+                dot += __shfl_xor(dot, o);
+                pi_sum += __shfl_xor(pi_sum, o);
+                pi_abs += __shfl_xor(pi_abs, o);
+            }
+        }
+        if (lane < 16) {
+            const int q = wp * T::BQ + wq * T::TQ + j * 16 + lane;
+            joint[q] = f32x4{top, l, s, dot};
+            if constexpr (DENSE) {
+                jt[2 * q] = pi_sum;
+                jt[2 * q + 1] = pi_abs;
+            }
+        }
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < T::BQ; q += T::THREADS) {
+        if (q0 + q >= a.t.rows) break;
+        f32x4 v[T::WP];
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < T::WP; ++w) {
+            v[w] = joint[w * T::BQ + q];
+            top = fmaxf(top, v[w][0]);
+        }
+        f32x4 o = {top, 0.0f, 0.0f, 0.0f};
+        float ts = 0.0f, ta = 0.0f;
+#pragma unroll
+        for (int w = 0; w < T::WP; ++w) {
+            join_part(o, v[w]);
+            if constexpr (DENSE) {
+                ts += jt[2 * (w * T::BQ + q)];
+                ta += jt[2 * (w * T::BQ + q) + 1];
+            }
+        }
+        const int64_t at = (q0 + q) * a.tiles + a.tile0 + tp;
+        a.part[at] = o;
+        if constexpr (DENSE) {
+            a.tpart[2 * at] = ts;
+            a.tpart[2 * at + 1] = ta;
+        }
+    }
+}
+
+struct JoinArgs {
+    Rows t;
+    const f32x4* part;
+    const float* tpart;
+    const float* zt;
+    int32_t tiles, reduction;
+    float *lse, *ent, *tsum, *scalars;       // kept for the backward pass
+    float *ce, *tabs;                        // per row
+    float *loss, *out_ce, *out_ent;          // results, per row or one; the last two may be null
+};
+
+// One wave per row over the row's tiles.
+__device__ __forceinline__ void join_row(const JoinArgs& a, int64_t n) {
+    const int lane = threadIdx.x & 63;
+    const f32x4* part = a.part + n * a.tiles;
+    float top = -INFINITY;
+    for (int i = lane; i < a.tiles; i += 64) top = fmaxf(top, part[i][0]);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+    f32x4 v = {top, 0.0f, 0.0f, 0.0f};
+    float ts = 0.0f, ta = 0.0f;
+    for (int i = lane; i < a.tiles; i += 64) {
+        join_part(v, part[i]);
+        if (a.t.dense) {
+            ts += a.tpart[2 * (n * a.tiles + i)];
+            ta += a.tpart[2 * (n * a.tiles + i) + 1];
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        v[1] += __shfl_xor(v[1], o);
+        v[2] += __shfl_xor(v[2], o);
+        v[3] += __shfl_xor(v[3], o);
+        ts += __shfl_xor(ts, o);
+        ta += __shfl_xor(ta, o);
+    }
+    if (lane) return;
+    // every logit of the row is -inf: no softmax exists
+    const float lse = top == -INFINITY ? NAN : top + logf(v[1]);
+    const float h = top == -INFINITY ? NAN : logf(v[1]) - v[2] / v[1];
+    float ce;
+    bool counts = true;
+    if (a.t.dense) {
+        ce = ts * lse - v[3];
+        a.tsum[n] = ts;
+        a.tabs[n] = ta;
+    } else {
+        const int64_t t = a.t.index[n];
+        counts = t != a.t.ignore;
+        ce = t >= 0 && t < a.t.classes ? lse - a.zt[n] : NAN;   // a class that does not exist: a loss that nobody overlooks
+    }
+    a.lse[n] = lse;
+    a.ent[n] = h;
+    a.ce[n] = ce;
+    if (a.reduction == AZ_REDUCE_NONE) {
+        a.loss[n] = counts ? (a.t.entropy != 0.0f ? ce - a.t.entropy * h : ce) : 0.0f;
+        if (a.out_ce) a.out_ce[n] = counts ? ce : 0.0f;
+        if (a.out_ent) a.out_ent[n] = counts ? h : 0.0f;
+    }
+}
+
+// Sums over the rows by one workgroup of 1024, in a fixed order and in 64 bits (a row is 4 to 20 bytes here).
+__device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
+    __shared__ double sums[2][16];
+    __shared__ float tops[16];
+    __shared__ int numbers[16];
+    double ce = 0.0, h = 0.0;
+    float top = 0.0f;
+    int count = 0;
+    for (int n = threadIdx.x; n < a.t.rows; n += 1024) {
+        if (a.t.index && a.t.index[n] == a.t.ignore) continue;
+        ++count;
+        ce += a.ce[n];
+        h += a.ent[n];
+        if (a.t.dense) top = fmaxf(top, a.tabs[n]);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        ce += __shfl_xor(ce, o);
+        h += __shfl_xor(h, o);
+        top = fmaxf(top, __shfl_xor(top, o));
+        count += __shfl_xor(count, o);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        const int w = threadIdx.x >> 6;
+        sums[0][w] = ce;
+        sums[1][w] = h;
+        tops[w] = top;
+        numbers[w] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) {
+        ce += sums[0][w];
+        h += sums[1][w];
+        top = fmaxf(top, tops[w]);
+        count += numbers[w];
+    }
+    a.scalars[0] = (float)count;
+    // |G| <= 2 sum |pi| + |c| (1/e + log classes)
+    a.scalars[1] = (a.t.dense ? 2.0f * top : 1.0f) + fabsf(a.t.entropy) * (0.4f + logf((float)a.t.classes));
+    if (a.reduction == AZ_REDUCE_NONE) return;
+    const double d = a.reduction == AZ_REDUCE_MEAN ? (double)count : 1.0;
+    a.loss[0] = (float)((ce - (a.t.entropy != 0.0f ? a.t.entropy * h : 0.0)) / d);
+    if (a.out_ce) a.out_ce[0] = (float)(ce / d);
+    if (a.out_ent) a.out_ent[0] = (float)(h / d);
+}
+
+__global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n < a.t.rows) join_row(a, n);
+}
+__global__ __launch_bounds__(1024) void k_ce_reduce(JoinArgs a) { reduce_rows(a); }
+// Few rows: both in one launch.
+__global__ __launch_bounds__(1024) void k_ce_join_reduce(JoinArgs a) {
+    for (int n = threadIdx.x >> 6; n < a.t.rows; n += 16) join_row(a, n);
+    __threadfence_block();
+    __syncthreads();
+    reduce_rows(a);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// How G is held in 16 bits. The factor of a row (the caller's gradient, over the number of rows in a mean) stays out of what is
+// rounded wherever it can: rounded with it, the -1 at every row's target would be off by the same relative amount in every row, and
+// that would not average out. With one factor for all rows it multiplies the products' results. With a factor for each row it does so
+// for dx, and for dW, whose sum runs over the rows, G^T holds factor / largest factor.
+// float16 has too few exponents for small p: there G is held times the power of two that takes its bound to at most 2^14, so that
+// values down to 2^-27 of the bound keep all their bits.
+__device__ __forceinline__ float hold_scale(const float* scalars) {
+    return ldexpf(1.0f, 14 - (ilogbf(fmaxf(scalars[1], 1e-30f)) + 1));
+}
+
+// Largest |gradient| of the rows, for one gradient per row.
+__global__ __launch_bounds__(1024) void k_ce_largest(const float* grad, int rows, float* out) {
+    __shared__ float tops[16];
+    float top = 0.0f;
+    auto see = [&](float g) { top = g > top || g != g ? g : top; };      // a NaN stays
+    for (int n = threadIdx.x; n < rows; n += 1024) see(fabsf(grad[n]));
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) see(__shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) see(tops[w]);
+    *out = top;
+}
+
+// The factors that the results of the products with G get.
+struct Factor {
+    const float *grad, *scalars, *largest;   // largest: one gradient per row
+    int32_t mean, half;                      // half: G is held times hold_scale
+};
+__device__ __forceinline__ float factor_all(const Factor& f) {            // dW, db, and dx with one factor
+    float v = f.largest ? *f.largest : f.grad[0];
+    if (f.mean) v = f.scalars[0] > 0.0f ? v / f.scalars[0] : 0.0f;     // no row counts: G is zero
+    return f.half ? v / hold_scale(f.scalars) : v;
+}
+__device__ __forceinline__ float factor_row(const Factor& f, int64_t n) {  // dx with one factor per row
+    return f.half ? f.grad[n] / hold_scale(f.scalars) : f.grad[n];
+}
+
+struct GradArgs {
+    MmOperand w, x;
+    Rows t;
+    const void* bias;
+    int32_t kbytes, segments, v0;
+    int32_t tiles_p, tiles_q;
+    const float *lse, *ent, *tsum;
+    Factor f;
+    char* g;               // [rows][g_pitch] per plane, or null (no dx wanted)
+    int64_t g_pitch, g_plane;
+    char* gt;              // [classes of the piece][gt_pitch] per plane, or null (no dW wanted)
+    int64_t gt_pitch, gt_plane;
+    float* db;             // [tiles_q][db_pitch] sums over a tile's rows, or null
+    int64_t db_pitch;
+};
+
+template <class T, int DT, bool DENSE, bool ENT>
+__global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
+    __shared__ __align__(16) char lds[T::LDS];
+    constexpr int NP = DT == DT_F32 ? 3 : 1;
+    int tp, tq;
+    mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
+    const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
+    typename T::acc_t acc[T::FP][T::FQ];
+    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
+    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    add_bias<T, DT>(a.bias, p0, wp, lane, a.v0, a.t.classes, acc);
+    const int ml = (int)p0 + wp * T::TP + (lane >> 4) * 4;        // class of the piece
+    const int left = a.t.classes - a.v0 - ml;
+    const float hold = a.f.half ? hold_scale(a.f.scalars) : 1.0f;
+    float share[T::FQ];        // of a row's factor in the largest
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+        const bool row = n < a.t.rows;
+        int64_t target = 0;
+        float lse = 0.0f, h = 0.0f, total = 1.0f, f = hold;
+        bool counts = false;
+        share[j] = 1.0f;
+        if (row) {
+            lse = a.lse[n];
+            if constexpr (ENT) h = a.ent[n];
+            if constexpr (DENSE) total = a.tsum[n];
+            else target = a.t.index[n];
+            counts = DENSE || target != a.t.ignore;
+            if (a.f.largest) share[j] = *a.f.largest > 0.0f || *a.f.largest != *a.f.largest ? a.f.grad[n] / *a.f.largest : 0.0f;
+            if (!DENSE && (target < 0 || target >= a.t.classes)) f = NAN;
+        }
+        const int64_t at = target - a.v0 - ml;
+        const float* pi = DENSE && row ? a.t.dense + n * a.t.dense_pitch + a.v0 + ml : nullptr;
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float lp = acc[i][j][r] - lse;
+                const float p = __builtin_amdgcn_exp2f(lp * LOG2E);
+                float g = p;
+                const bool in = i * 16 + r < left;
+                if constexpr (DENSE) g = total * p - (in && row ? pi[i * 16 + r] : 0.0f);
+                else g = at == i * 16 + r ? p - 1.0f : p;
+                if constexpr (ENT) g += p == 0.0f ? 0.0f : a.t.entropy * p * (lp + h);
+                acc[i][j][r] = in && counts ? g * f : 0.0f;
+            }
+    }
+    if (a.db) {
+        float* const joint = (float*)lds;      // [WQ][BP]
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < T::FQ; ++j) s += acc[i][j][r] * share[j];
+#pragma unroll
+                for (int o = 1; o < 16; o *= 2) s += __shfl_xor(s, o);
+                if ((lane & 15) == 0) joint[wq * T::BP + wp * T::TP + i * 16 + (lane >> 4) * 4 + r] = s;
+            }
+        __syncthreads();
+        for (int p = threadIdx.x; p < T::BP; p += T::THREADS) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < T::WQ; ++w) s += joint[w * T::BP + p];
+            if (p0 + p < a.db_pitch) a.db[tq * a.db_pitch + p0 + p] = s;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) {
+            const int64_t m = ml + i * 16;
+            uint16_t o[NP][4];
+            auto round = [&](float by) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (DT == DT_F32) split3(acc[i][j][r] * by, o[0][r], o[1][r], o[2][r]);
+                    else o[0][r] = to_bits<DT>(acc[i][j][r] * by);
+                }
+            };
+            round(1.0f);
+            if (a.g && n < a.t.rows && m * 2 < a.g_pitch)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) *(uint2*)(a.g + p * a.g_plane + n * a.g_pitch + m * 2) = *(const uint2*)o[p];
+            if (a.f.largest) round(share[j]);
+            if (a.gt && n * 2 < a.gt_pitch)
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i * 16 + r < left) *(uint16_t*)(a.gt + p * a.gt_plane + (m + r) * a.gt_pitch + n * 2) = o[p][r];
+        }
+    }
+}
+
+struct OutArgs {
+    MmOperand p, q;
+    int32_t kbytes, segments, tiles_p, tiles_q;
+    void* out;             // [q rows][p rows], the last step
+    float* sum;            // running sums over the pieces, or null
+    int32_t first, last, by_row;
+    Factor f;
+};
+
+template <class T, int DT>
+__device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
+    int tp, tq;
+    mm_place(id, a.tiles_p, a.tiles_q, tp, tq);
+    const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
+    typename T::acc_t acc[T::FP][T::FQ];
+    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
+    mm_tile<T>(a.p, a.q, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    const float all = a.by_row ? 0.0f : factor_all(a.f);
+    const int64_t width = a.p.rows;
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+        if (n >= a.q.rows) continue;
+        const float post = a.by_row ? factor_row(a.f, n) : all;
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) {
+            const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
+            const int64_t at = n * width + m;
+            f32x4 v = acc[i][j];
+            if ((width & 3) == 0 && m + 4 <= width) {
+                if (!a.first) v += *(const f32x4*)(a.sum + at);
+                if (!a.last) *(f32x4*)(a.sum + at) = v;
+                else store4<DT>(a.out, at, v[0] * post, v[1] * post, v[2] * post, v[3] * post);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m + r < width) {
+                        float u = v[r];
+                        if (!a.first) u += a.sum[at + r];
+                        if (!a.last) a.sum[at + r] = u;
+                        else store_scalar<DT>(a.out, at + r, u * post);
+                    }
+            }
+        }
+    }
+}
+
+struct BiasArgs {
+    const float* part;     // [tiles][pitch]
+    int64_t pitch, at;
+    int32_t tiles, classes;
+    void* out;
+    Factor f;
+};
+
+template <int DT>
+__device__ __forceinline__ void bias_block(const BiasArgs& a, int64_t m) {
+    if (m >= a.classes) return;
+    float s = 0.0f;
+    for (int t = 0; t < a.tiles; ++t) s += a.part[t * a.pitch + m];
+    store_scalar<DT>(a.out, a.at + m, s * factor_all(a.f));
+}
+
+// dx, dW and db of a piece in one launch: they share nothing but G, and small ones fill the chip together.
+template <class T, int DT>
+__global__ __launch_bounds__(T::THREADS) void k_ce_out(OutArgs a, OutArgs b, BiasArgs c, int blocks_a, int blocks_b) {
+    __shared__ __align__(16) char lds[T::LDS];
+    const int id = blockIdx.x;
+    if (id < blocks_a) out_tile<T, DT>(a, id, lds);
+    else if (id < blocks_a + blocks_b) out_tile<T, DT>(b, id - blocks_a, lds);
+    else bias_block<DT>(c, (int64_t)(id - blocks_a - blocks_b) * T::THREADS + threadIdx.x);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+typedef MmTile<256, 256, 2, 4, MM_BF16> BigB;
+typedef MmTile<256, 256, 2, 4, MM_F16> BigH;
+typedef MmTile<128, 128, 2, 2, MM_BF16> MidB;
+typedef MmTile<128, 128, 2, 2, MM_F16> MidH;
+typedef MmTile<64, 64, 2, 2, MM_BF16> SmallB;
+typedef MmTile<64, 64, 2, 2, MM_F16> SmallH;
+
+int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Tile edge for a product with p x q results: the largest whose tiles give every compute unit work.
+int tile_edge(int64_t p, int64_t q) {
+    auto tiles = [&](int64_t e) { return ((p + e - 1) / e) * ((q + e - 1) / e); };
+    if (tiles(256) >= 192) return 256;
+    if (tiles(128) >= 192) return 128;
+    return 64;
+}
+
+struct Layout {       // of the workspace, and the pieces of the classes
+    bool split, pack;   // float32; operands copied into rows of whole 16 bytes
+    int planes;
+    int64_t kpitch;     // bytes of an operand's row as the tile loop reads it (when packed)
+    int64_t piece;      // classes of a piece
+    int pieces;
+    int64_t bytes = 0;
+    int64_t xp = -1, wp = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1;                     // forward
+    int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1;                 // backward
+    int64_t take(int64_t n) {
+        const int64_t at = bytes;
+        bytes += round_up(n, 256);
+        return at;
+    }
+};
+
+bool aligned(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p & 15) == 0 && (pitch & 7) == 0 && (cols & 7) == 0; }
+
+void operand_layout(const az_linear_ce_args& a, Layout& l) {
+    l.split = a.dtype == AZ_DT_F32;
+    l.planes = l.split ? 3 : 1;
+    l.pack = l.split || !aligned(a.x, a.x_pitch, a.features) || !aligned(a.weight, a.weight_pitch, a.features);
+    l.kpitch = round_up(a.features, 8) * 2;
+}
+
+int forward_edge(const az_linear_ce_args& a) { return tile_edge(a.classes, a.rows); }
+
+Layout forward_layout(const az_linear_ce_args& a) {
+    Layout l;
+    operand_layout(a, l);
+    // a packed piece of the weight stays below 512 MB
+    int64_t piece = a.classes;
+    if (l.pack) piece = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
+    l.piece = piece < 256 ? 256 : piece;
+    if (l.piece > a.classes) l.piece = a.classes;
+    l.pieces = (int)((a.classes + l.piece - 1) / l.piece);
+    const int64_t edge = forward_edge(a), tiles = (a.classes + edge - 1) / edge;
+    if (l.pack) {
+        l.xp = l.take(a.rows * l.kpitch * l.planes);
+        l.wp = l.take(l.piece * l.kpitch * l.planes);
+    }
+    l.part = l.take(a.rows * tiles * 16);
+    l.ce = l.take(a.rows * 4);
+    if (a.target_dense) {
+        l.tpart = l.take(a.rows * tiles * 8);
+        l.tabs = l.take(a.rows * 4);
+    } else {
+        l.zt = l.take(a.rows * 4);
+    }
+    return l;
+}
+
+Layout backward_layout(const az_linear_ce_args& a) {
+    Layout l;
+    operand_layout(a, l);
+    const int64_t np = round_up(a.rows, 64);
+    // G and its transpose of a piece stay at about 1 GB: then the sums of dx that travel between pieces cost a few per cent
+    int64_t piece = (int64_t(1) << 30) / (np * 4 * l.planes) / 256 * 256;
+    if (l.pack) {
+        const int64_t w = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
+        if (w < piece) piece = w;
+    }
+    l.piece = piece < 256 ? 256 : piece;
+    if (l.piece > a.classes) l.piece = a.classes;
+    l.pieces = (int)((a.classes + l.piece - 1) / l.piece);
+    const int64_t vp = round_up(l.piece, 64);
+    if (l.pack) {
+        l.xp = l.take(a.rows * l.kpitch * l.planes);
+        l.wp = l.take(l.piece * l.kpitch * l.planes);
+    }
+    l.xt = l.take(a.features * np * 2 * l.planes);
+    l.wt = l.take(a.features * vp * 2 * l.planes);
+    l.g = l.take(a.rows * vp * 2 * l.planes);
+    l.gt = l.take(l.piece * np * 2 * l.planes);
+    l.db = l.take((a.rows + 63) / 64 * l.piece * 4);      // the smallest tiles make the most sums
+    if (l.pieces > 1) l.sum = l.take(a.rows * a.features * 4);
+    l.largest = l.take(16);
+    return l;
+}
+
+int check_args(const az_linear_ce_args* a) {
+    if (!a) return fail(AZ_ERR_ARG, "null argument");
+    if (a->dtype != AZ_DT_F32 && a->dtype != AZ_DT_BF16 && a->dtype != AZ_DT_F16) return fail(AZ_ERR_ARG, "dtype is float32, bfloat16 or float16");
+    if (a->rows < 1 || a->features < 1 || a->classes < 1) return fail(AZ_ERR_ARG, "rows, features and classes are at least 1");
+    if (a->rows > (1 << 30) || a->classes > (1 << 30)) return fail(AZ_ERR_ARG, "rows and classes are at most 2^30");
+    if (a->features * 2 > MM_MAX_PITCH - 16 || a->rows * 2 > MM_MAX_PITCH - 128) return fail(AZ_ERR_ARG, "features and rows are at most 4194000");
+    if (!a->x || !a->weight || !a->target) return fail(AZ_ERR_ARG, "null argument");
+    if (a->x_pitch < a->features || a->weight_pitch < a->features || (a->target_dense && a->target_pitch < a->classes))
+        return fail(AZ_ERR_ARG, "a row stride is smaller than the row");
+    const Layout l = [&] { Layout t; operand_layout(*a, t); return t; }();
+    if (!l.pack && (a->x_pitch * 2 > MM_MAX_PITCH || a->weight_pitch * 2 > MM_MAX_PITCH)) return fail(AZ_ERR_ARG, "a row stride is too large");
+    if (a->reduction < AZ_REDUCE_NONE || a->reduction > AZ_REDUCE_SUM) return fail(AZ_ERR_ARG, "reduction is none, mean or sum");
+    return AZ_OK;
+}
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+Rows rows_of(const az_linear_ce_args& a) {
+    Rows t;
+    t.index = a.target_dense ? nullptr : (const int64_t*)a.target;
+    t.dense = a.target_dense ? (const float*)a.target : nullptr;
+    t.dense_pitch = a.target_pitch;
+    t.ignore = a.ignore_index;
+    t.rows = (int)a.rows;
+    t.classes = (int)a.classes;
+    t.entropy = a.entropy_coeff;
+    return t;
+}
+
+template <int DT>
+void pack(PackArgs& a, hipStream_t st) {
+    a.end_w = a.w.blocks();
+    a.end_x = a.end_w + a.x.blocks();
+    a.end_wt = a.end_x + a.wt.blocks();
+    const int64_t n = a.end_wt + a.xt.blocks();
+    if (n) hipLaunchKernelGGL((k_pack<DT>), dim3((unsigned)n), dim3(256), 0, st, a);
+}
+
+template <class T, int DT>
+void launch_stats(const StatArgs& s, bool dense, bool ent, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)s.tiles_p * s.tiles_q)), block(T::THREADS);
+    if (dense && ent) hipLaunchKernelGGL((k_ce_stats<T, DT, true, true>), grid, block, 0, st, s);
+    else if (dense) hipLaunchKernelGGL((k_ce_stats<T, DT, true, false>), grid, block, 0, st, s);
+    else if (ent) hipLaunchKernelGGL((k_ce_stats<T, DT, false, true>), grid, block, 0, st, s);
+    else hipLaunchKernelGGL((k_ce_stats<T, DT, false, false>), grid, block, 0, st, s);
+}
+
+template <class T, int DT>
+void launch_grad(const GradArgs& s, bool dense, bool ent, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)s.tiles_p * s.tiles_q)), block(T::THREADS);
+    if (dense && ent) hipLaunchKernelGGL((k_ce_grad<T, DT, true, true>), grid, block, 0, st, s);
+    else if (dense) hipLaunchKernelGGL((k_ce_grad<T, DT, true, false>), grid, block, 0, st, s);
+    else if (ent) hipLaunchKernelGGL((k_ce_grad<T, DT, false, true>), grid, block, 0, st, s);
+    else hipLaunchKernelGGL((k_ce_grad<T, DT, false, false>), grid, block, 0, st, s);
+}
+
+template <int DT> struct Tiles { typedef BigB Big; typedef MidB Mid; typedef SmallB Small; };
+template <> struct Tiles<DT_F16> { typedef BigH Big; typedef MidH Mid; typedef SmallH Small; };
+
+struct Kept {      // what the forward pass leaves for the backward one
+    float *lse, *ent, *tsum, *scalars;
+    Kept(float* p, int64_t rows) : lse(p), ent(p + rows), tsum(p + 2 * rows), scalars(p + 3 * rows) {}
+};
+
+template <int DT>
+int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, float* ent, char* ws, hipStream_t st) {
+    const Layout l = forward_layout(a);
+    const int edge = forward_edge(a);
+    StatArgs s{};
+    s.t = rows_of(a);
+    s.bias = a.bias;
+    s.segments = l.split ? 6 : 1;
+    s.part = (f32x4*)(ws + l.part);
+    s.tpart = a.target_dense ? (float*)(ws + l.tpart) : nullptr;
+    s.zt = a.target_dense ? nullptr : (float*)(ws + l.zt);
+    s.tiles = (int)((a.classes + edge - 1) / edge);
+    s.tiles_q = (int)((a.rows + edge - 1) / edge);
+    s.kbytes = (int)(l.pack ? l.kpitch : a.features * 2);
+    for (int i = 0; i < l.pieces; ++i) {
+        const int64_t v0 = i * l.piece, nv = a.classes - v0 < l.piece ? a.classes - v0 : l.piece;
+        const char* w = (const char*)a.weight + v0 * a.weight_pitch * (l.split ? 4 : 2);
+        if (l.pack) {
+            PackArgs p{};
+            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch};
+            if (i == 0) p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch};
+            pack<DT>(p, st);
+            s.w = MmOperand{ws + l.wp, l.kpitch, l.piece * l.kpitch, (int)nv};
+            s.x = MmOperand{ws + l.xp, l.kpitch, a.rows * l.kpitch, (int)a.rows};
+        } else {
+            s.w = MmOperand{w, a.weight_pitch * 2, 0, (int)nv};
+            s.x = MmOperand{(const char*)a.x, a.x_pitch * 2, 0, (int)a.rows};
+        }
+        s.v0 = (int)v0;
+        s.tile0 = (int)(v0 / edge);
+        s.tiles_p = (int)((nv + edge - 1) / edge);
+        const bool d = a.target_dense, e = a.entropy_coeff != 0.0f || ent;
+        if (edge == 256) launch_stats<typename Tiles<DT>::Big, DT>(s, d, e, st);
+        else if (edge == 128) launch_stats<typename Tiles<DT>::Mid, DT>(s, d, e, st);
+        else launch_stats<typename Tiles<DT>::Small, DT>(s, d, e, st);
+        if (const int rc = launched("k_ce_stats")) return rc;
+    }
+    const Kept k(kept, a.rows);
+    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.lse, k.ent, k.tsum, k.scalars, (float*)(ws + l.ce),
+                     a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent};
+    if (a.rows <= 512 && s.tiles <= 64) {
+        hipLaunchKernelGGL(k_ce_join_reduce, dim3(1), dim3(1024), 0, st, j);
+    } else {
+        hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, j);
+        hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, j);
+    }
+    return launched("k_ce_join");
+}
+
+template <int DT>
+int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, void* gx, void* gw, void* gb, char* ws, hipStream_t st) {
+    const Layout l = backward_layout(a);
+    const int esize = l.split ? 4 : 2;
+    const int64_t np = round_up(a.rows, 64), vp = round_up(l.piece, 64);
+    const bool each = a.reduction == AZ_REDUCE_NONE;
+    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT == DT_F16};
+    if (each) hipLaunchKernelGGL(k_ce_largest, dim3(1), dim3(1024), 0, st, grad, (int)a.rows, (float*)(ws + l.largest));
+    GradArgs s{};
+    s.t = rows_of(a);
+    s.bias = a.bias;
+    s.segments = l.split ? 6 : 1;
+    s.kbytes = (int)(l.pack ? l.kpitch : a.features * 2);
+    s.lse = kept.lse;
+    s.ent = kept.ent;
+    s.tsum = kept.tsum;
+    s.f = f;
+    s.g = gx ? ws + l.g : nullptr;
+    s.g_pitch = vp * 2;
+    s.g_plane = a.rows * vp * 2;
+    s.gt = gw ? ws + l.gt : nullptr;
+    s.gt_pitch = np * 2;
+    s.gt_plane = l.piece * np * 2;
+    s.db = gb ? (float*)(ws + l.db) : nullptr;
+    for (int i = 0; i < l.pieces; ++i) {
+        const int64_t v0 = i * l.piece, nv = a.classes - v0 < l.piece ? a.classes - v0 : l.piece;
+        const char* w = (const char*)a.weight + v0 * a.weight_pitch * esize;
+        const int64_t vpi = round_up(nv, 64);    // k of dx in this piece
+        PackArgs p{};
+        if (l.pack) {
+            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch};
+            if (i == 0) p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch};
+            s.w = MmOperand{ws + l.wp, l.kpitch, l.piece * l.kpitch, (int)nv};
+            s.x = MmOperand{ws + l.xp, l.kpitch, a.rows * l.kpitch, (int)a.rows};
+        } else {
+            s.w = MmOperand{w, a.weight_pitch * 2, 0, (int)nv};
+            s.x = MmOperand{(const char*)a.x, a.x_pitch * 2, 0, (int)a.rows};
+        }
+        if (gx) p.wt = TurnJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wt, vpi * 2, a.features * vpi * 2, nullptr, 0};
+        if (gw && i == 0) p.xt = TurnJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xt, np * 2, a.features * np * 2, s.t.index, a.ignore_index};
+        pack<DT>(p, st);
+        s.g_pitch = vpi * 2;
+        s.g_plane = a.rows * vpi * 2;
+        s.v0 = (int)v0;
+        s.db_pitch = nv;
+        const int edge = tile_edge(nv, a.rows);
+        s.tiles_p = (int)((nv + edge - 1) / edge);
+        s.tiles_q = (int)((a.rows + edge - 1) / edge);
+        const bool d = a.target_dense, e = a.entropy_coeff != 0.0f;
+        if (edge == 256) launch_grad<typename Tiles<DT>::Big, DT>(s, d, e, st);
+        else if (edge == 128) launch_grad<typename Tiles<DT>::Mid, DT>(s, d, e, st);
+        else launch_grad<typename Tiles<DT>::Small, DT>(s, d, e, st);
+        if (const int rc = launched("k_ce_grad")) return rc;
+        OutArgs ox{}, ow{};
+        ox.p = MmOperand{ws + l.wt, vpi * 2, a.features * vpi * 2, (int)a.features};
+        ox.q = MmOperand{ws + l.g, vpi * 2, a.rows * vpi * 2, (int)a.rows};
+        ox.kbytes = (int)(vpi * 2);
+        ox.out = gx;
+        ox.sum = l.pieces > 1 ? (float*)(ws + l.sum) : nullptr;
+        ox.first = i == 0;
+        ox.last = i == l.pieces - 1;
+        ow.p = MmOperand{ws + l.xt, np * 2, a.features * np * 2, (int)a.features};
+        ow.q = MmOperand{ws + l.gt, np * 2, l.piece * np * 2, (int)nv};
+        ow.kbytes = (int)(np * 2);
+        ow.out = (char*)gw + v0 * a.features * esize;
+        ow.first = ow.last = 1;
+        ox.segments = ow.segments = s.segments;
+        ox.f = ow.f = f;
+        ox.by_row = each;
+        const int64_t q = (gx ? a.rows : 0) + (gw ? nv : 0);
+        const int oe = tile_edge(a.features, q);
+        auto size = [&](OutArgs& o, bool wanted) {
+            o.tiles_p = (int)((o.p.rows + oe - 1) / oe);
+            o.tiles_q = (int)((o.q.rows + oe - 1) / oe);
+            return wanted ? (int64_t)o.tiles_p * o.tiles_q : 0;
+        };
+        const int64_t bx = size(ox, gx), bw = size(ow, gw);
+        BiasArgs ob{s.db, s.db_pitch, v0, s.tiles_q, gb ? (int)nv : 0, gb, f};
+        auto run = [&](auto tile) {
+            typedef decltype(tile) T;
+            const int64_t bb = (ob.classes + T::THREADS - 1) / T::THREADS;
+            hipLaunchKernelGGL((k_ce_out<T, DT>), dim3((unsigned)(bx + bw + bb)), dim3(T::THREADS), 0, st, ox, ow, ob, (int)bx, (int)bw);
+        };
+        if (oe == 256) run(typename Tiles<DT>::Big{});
+        else if (oe == 128) run(typename Tiles<DT>::Mid{});
+        else run(typename Tiles<DT>::Small{});
+        if (const int rc = launched("k_ce_out")) return rc;
+    }
+    return AZ_OK;
+}
+
+}  // namespace
+}  // namespace az
+
+using namespace az;
+
+extern "C" int64_t az_linear_ce_workspace(const az_linear_ce_args* args, int32_t backward) {
+    if (const int rc = check_args(args)) return rc;
+    return (backward ? backward_layout(*args) : forward_layout(*args)).bytes;
+}
+
+extern "C" int az_linear_ce_forward(const az_linear_ce_args* args, float* kept, float* loss, float* ce, float* ent, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+    if (const int rc = check_args(args)) return rc;
+    if (!kept || !loss || !workspace) return fail(AZ_ERR_ARG, "null argument");
+    if (workspace_bytes < forward_layout(*args).bytes || ((uintptr_t)workspace & 255)) return fail(AZ_ERR_ARG, "workspace too small or not at a multiple of 256");
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    if (args->dtype == AZ_DT_F32) return forward<DT_F32>(*args, kept, loss, ce, ent, ws, st);
+    if (args->dtype == AZ_DT_BF16) return forward<DT_BF16>(*args, kept, loss, ce, ent, ws, st);
+    return forward<DT_F16>(*args, kept, loss, ce, ent, ws, st);
+}
+
+extern "C" int az_linear_ce_backward(const az_linear_ce_args* args, const float* kept, const float* grad, void* grad_x, void* grad_weight,
+                                     void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (const int rc = check_args(args)) return rc;
+    if (!kept || !grad || !workspace) return fail(AZ_ERR_ARG, "null argument");
+    if (!grad_x && !grad_weight && !grad_bias) return AZ_OK;
+    if (((uintptr_t)grad_x | (uintptr_t)grad_weight) & 15) return fail(AZ_ERR_ARG, "gradients start at a multiple of 16 bytes");
+    if (workspace_bytes < backward_layout(*args).bytes || ((uintptr_t)workspace & 255)) return fail(AZ_ERR_ARG, "workspace too small or not at a multiple of 256");
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    const Kept k(const_cast<float*>(kept), args->rows);
+    if (args->dtype == AZ_DT_F32) return backward<DT_F32>(*args, k, grad, grad_x, grad_weight, grad_bias, ws, st);
+    if (args->dtype == AZ_DT_BF16) return backward<DT_BF16>(*args, k, grad, grad_x, grad_weight, grad_bias, ws, st);
+    return backward<DT_F16>(*args, k, grad, grad_x, grad_weight, grad_bias, ws, st);
+}

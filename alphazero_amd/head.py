@@ -1,0 +1,281 @@
+"""Operators around a network's last matrix product, as HIP kernels of libazamd: the loss of a linear layer over many classes
+with its gradient (the logits are never stored), dropout from a counter-based generator (the mask is never stored), and the product
+in 8-bit integers with a scale for each token and channel.
+
+They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the tensors' device; there is no CPU
+fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two."""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+_DTYPES = {torch.float32: N.AZ_DT_F32, torch.bfloat16: N.AZ_DT_BF16, torch.float16: N.AZ_DT_F16}
+_HERE = contextlib.nullcontext()
+_REDUCE = {"none": N.AZ_REDUCE_NONE, "mean": N.AZ_REDUCE_MEAN, "sum": N.AZ_REDUCE_SUM}
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_gpu(name: str, x: torch.Tensor, *others):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise N.NativeError(f"alphazero_amd.head.{name} needs tensors on a GPU (no CPU fallback)")
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., n] as [rows, n] with neighbouring columns; a copy only where the layout asks for one."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _device(device):
+    """The device made current for native calls; nothing to do where it already is."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _scratch(size: int, device) -> torch.Tensor:
+    return torch.empty(max(1, size), dtype=torch.uint8, device=device)
+
+
+# ------------------------------------------------------------------------------------------------ loss of a linear layer
+def _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff):
+    dense = target.dim() == 2
+    return N.AzLinearCeArgs(x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr(), x.shape[0], x.shape[1], weight.shape[0], _pitch(x),
+                            _pitch(weight), _pitch(target) if dense else 0, ignore_index, _DTYPES[x.dtype], dense, _REDUCE[reduction], entropy_coeff)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction, entropy_coeff, parts):
+        a = _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff)
+        rows, dev = x.shape[0], x.device
+        shape = (rows,) if reduction == "none" else ()
+        out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
+        kept = torch.empty(3 * rows + 2, dtype=torch.float32, device=dev)
+        L = N.lib()
+        with _device(dev):
+            ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 0), "az_linear_ce_workspace"), dev)
+            N.check(L.az_linear_ce_forward(C.byref(a), kept.data_ptr(), out[0].data_ptr(), out[1].data_ptr() if parts else None,
+                                           out[2].data_ptr() if parts else None, ws.data_ptr(), ws.numel(), _stream(dev)), "az_linear_ce_forward")
+        ctx.save_for_backward(x, weight, bias, target, kept)
+        ctx.args = (ignore_index, reduction, entropy_coeff)
+        if parts:
+            ctx.mark_non_differentiable(out[1], out[2])
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, *_parts):
+        if grad is None:
+            return (None,) * 8
+        x, weight, bias, target, kept = ctx.saved_tensors
+        a = _ce_args(x, weight, bias, target, *ctx.args)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = x.device
+        grad = grad.to(torch.float32).contiguous()
+        gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
+        gb = torch.empty(bias.shape, dtype=x.dtype, device=dev) if bias is not None and need_b else None
+        L = N.lib()
+        with _device(dev):
+            ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 1), "az_linear_ce_workspace"), dev)
+            N.check(L.az_linear_ce_backward(C.byref(a), kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), ws.numel(),
+                                            _stream(dev)), "az_linear_ce_backward")
+        return gx, gw, gb, None, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100, reduction: str = "mean", entropy_coeff: float = 0.0,
+                         parts: bool = False):
+    """Cross entropy of softmax(x weight^T + bias) minus entropy_coeff times that softmax' entropy, without ever holding the logits.
+
+    x [..., features], weight [classes, features], bias [classes] or None: one dtype (float32, bfloat16, float16; under autocast they
+    are cast to its dtype like the operands of a linear layer). target: int64 class indices of x's leading shape, or floating target
+    weights [..., classes] (a search's visit distribution; they need not sum to one; no gradient). Rows whose index is ignore_index
+    count nowhere: loss and gradient zero whatever they hold, and the mean is over the other rows. reduction "mean", "sum" or
+    "none". Returns the float32 loss; with parts=True (loss, cross entropy, entropy), the last two without gradient.
+
+    An index outside 0..classes-1 that is not ignore_index gives a NaN loss and NaN gradients (the check is on the device, nothing
+    waits for it). Everything is accumulated in float32; the gradient of the logits is rounded to the inputs' 16-bit type between the
+    products (float32 inputs keep 24 bits). Scratch memory for the backward pass stays near 1 GB whatever the number of classes."""
+    _on_gpu("linear_cross_entropy", x, weight, target, bias)
+    _need(reduction in _REDUCE, 'reduction is "none", "mean" or "sum"')
+    _need(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1], f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, "classes and features are at least 1")
+    _need(bias is None or tuple(bias.shape) == (weight.shape[0],), "bias has one value per class")
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
+    _need(x.dtype in _DTYPES, f"x is float32, bfloat16 or float16, not {x.dtype}")
+    _need(weight.dtype == x.dtype and (bias is None or bias.dtype == x.dtype), "x, weight and bias have one dtype")
+    lead = x.shape[:-1]
+    if target.is_floating_point():
+        _need(target.shape == (*lead, weight.shape[0]), f"target weights {tuple(target.shape)} do not fit {(*lead, weight.shape[0])}")
+        _need(not (target.requires_grad and torch.is_grad_enabled()), "the target has no gradient: detach it")
+        target = _rows(target.to(torch.float32))
+    else:
+        _need(target.dtype == torch.int64, f"class indices are int64, not {target.dtype}")
+        _need(target.shape == lead, f"target {tuple(target.shape)} does not fit {tuple(lead)}")
+        target = target.reshape(-1).contiguous()
+    x2 = _rows(x)
+    if x2.shape[0] == 0:      # no rows: an empty sum, a mean of nothing
+        zero = (x2.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
+        one = x2.new_zeros(lead, dtype=torch.float32) + zero if reduction == "none" else zero / 0 if reduction == "mean" else zero
+        return (one, one.detach(), one.detach()) if parts else one
+    out = _LinearCrossEntropy.apply(x2, _rows(weight), bias if bias is None else bias.contiguous(), target, int(ignore_index), reduction,
+                                    float(entropy_coeff), bool(parts))
+    if reduction == "none" and len(lead) != 1:
+        out = tuple(t.reshape(lead) for t in out)
+    return out if parts else out[0]
+
+
+# ------------------------------------------------------------------------------------------------ dropout
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, seed_tensor, threshold, seed, offset):
+        ctx.save_for_backward(seed_tensor)
+        ctx.args = (threshold, seed, offset)
+        return _dropout(x, residual, seed_tensor, threshold, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = _dropout(grad.contiguous(), None, ctx.saved_tensors[0], *ctx.args)
+        return gx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def _dropout(x, residual, seed_tensor, threshold, seed, offset):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _device(x.device):
+        N.check(N.lib().az_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], threshold, seed,
+                                   _ptr(seed_tensor), offset, _stream(x.device)), "az_dropout")
+    return y
+
+
+def dropout(x, p: float, seed, offset: int = 0, *, residual=None):
+    """x with every element dropped (zero) with probability p and the others scaled by 1 / (1 - p), plus `residual`.
+
+    The mask is a function of (seed, offset, position), made again in the backward pass instead of being stored: Philox4x32-10 with key
+    `seed` and counter (position // 8 in row-major order, offset), 16 bits per element, so p is taken to the nearest 1 / 65536. Use
+    another offset for every call that shall have another mask. seed and offset: whole numbers below 2^64; seed may also be an int64
+    tensor of one element on x's device, read when the kernel runs (a captured graph then replays with whatever it holds; it has to
+    hold the same value in the backward pass). What is dropped is selected away, never multiplied: it may be infinite or NaN."""
+    _on_gpu("dropout", x, residual)
+    _need(x.dtype in _DTYPES, f"x is float32, bfloat16 or float16, not {x.dtype}")
+    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "residual has x's shape and dtype")
+    _need(0.0 <= p <= 1.0, "p is a probability")
+    _need(0 <= int(offset) < 1 << 64, "offset is 0..2^64-1")
+    seed_tensor, number = None, 0
+    if isinstance(seed, torch.Tensor):
+        _need(seed.dtype == torch.int64 and seed.numel() == 1 and seed.device == x.device, "a seed tensor is one int64 on x's device")
+        seed_tensor = seed
+    else:
+        number = int(seed)
+        _need(0 <= number < 1 << 64, "seed is 0..2^64-1")
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    threshold = round(65536 * float(p))
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, seed_tensor, threshold, number, int(offset))
+    return _dropout(x, residual, seed_tensor, threshold, number, int(offset))
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit integers
+def quantize_rows(x):
+    """(q int8 [..., n], scale float32 [...]) with x ~ q * scale: scale = max|row| / 127, q = the nearest whole number of
+    127 x / max|row| (ties to even). A row of zeros has scale 0; a row with an infinity or NaN has q = 0 and scale NaN."""
+    _on_gpu("quantize_rows", x)
+    _need(x.dtype in _DTYPES, f"x is float32, bfloat16 or float16, not {x.dtype}")
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, "a row has at least one element")
+    x2 = _rows(x.detach())
+    q = torch.empty(x2.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
+    with _device(x.device):
+        N.check(N.lib().az_quantize_rows(x2.data_ptr(), _DTYPES[x.dtype], x2.shape[0], x2.shape[1], _pitch(x2), q.data_ptr(), q.shape[1],
+                                         scale.data_ptr(), _stream(x.device)), "az_quantize_rows")
+    return q.reshape(x.shape), scale.reshape(x.shape[:-1])
+
+
+def int8_linear(x, qweight, weight_scale, bias=None, *, x_scale=None, out_dtype=None):
+    """y[..., n] = x_scale[...] * weight_scale[n] * sum_k x[..., k] qweight[n, k] + bias[n], the sum in 32-bit integers.
+
+    x: float32, bfloat16 or float16, quantised row by row on the way as quantize_rows does it, or int8 with its x_scale (float32,
+    x's leading shape). qweight int8 [channels, features] (at most 131071 features), weight_scale float32 [channels]. The output has
+    x's dtype (float32 for int8 x) or out_dtype. Rows of qweight that start at multiples of 16 bytes are read in place. There is no
+    gradient."""
+    _on_gpu("int8_linear", x, qweight, weight_scale, bias, x_scale)
+    _need(x.dtype in _DTYPES or x.dtype == torch.int8, f"x is float32, bfloat16, float16 or int8, not {x.dtype}")
+    _need(qweight.dtype == torch.int8 and qweight.dim() == 2, "qweight is an int8 matrix")
+    _need(x.dim() >= 1 and x.shape[-1] == qweight.shape[1], f"x {tuple(x.shape)} and qweight {tuple(qweight.shape)} do not fit")
+    _need(qweight.shape[0] >= 1 and 1 <= qweight.shape[1] <= 131071, "channels are at least 1, features 1..131071")
+    _need(weight_scale.dtype == torch.float32 and tuple(weight_scale.shape) == (qweight.shape[0],), "weight_scale is one float32 per channel")
+    _need(bias is None or (bias.dtype in _DTYPES and tuple(bias.shape) == (qweight.shape[0],)), "bias is one floating value per channel")
+    _need((x_scale is not None) == (x.dtype == torch.int8), "x_scale comes with an int8 x, and only with it")
+    _need(x_scale is None or (x_scale.dtype == torch.float32 and x_scale.shape == x.shape[:-1]), "x_scale is one float32 per row of x")
+    _need(out_dtype is None or out_dtype in _DTYPES, f"out_dtype is float32, bfloat16 or float16, not {out_dtype}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+        raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with detached tensors")
+    out_dtype = out_dtype or (torch.float32 if x.dtype == torch.int8 else x.dtype)
+    dev, channels = x.device, qweight.shape[0]
+    y = torch.empty((*x.shape[:-1], channels), dtype=out_dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    x2, w = _rows(x), _rows(qweight)
+    scale, wscale = None if x_scale is None else x_scale.reshape(-1).contiguous(), weight_scale.contiguous()
+    b = None if bias is None else bias.contiguous()
+    a = N.AzInt8Args(x=x2.data_ptr(), weight=w.data_ptr(), x_scale=_ptr(scale), weight_scale=wscale.data_ptr(), bias=_ptr(b), y=y.data_ptr(),
+                     tokens=x2.shape[0], features=x2.shape[1], channels=channels, x_pitch=_pitch(x2), weight_pitch=_pitch(w),
+                     x_dtype=N.AZ_DT_I8 if x.dtype == torch.int8 else _DTYPES[x.dtype], bias_dtype=_DTYPES[b.dtype] if b is not None else 0,
+                     y_dtype=_DTYPES[out_dtype])
+    L = N.lib()
+    with _device(dev):
+        size = N.check(L.az_int8_workspace(C.byref(a)), "az_int8_workspace")
+        ws = _scratch(size, dev) if size else None
+        N.check(L.az_int8_linear(C.byref(a), _ptr(ws), size, _stream(dev)), "az_int8_linear")
+    return y
+
+
+class Int8Linear(nn.Module):
+    """A linear layer whose weights are held in 8 bits with a scale per output channel and whose input is quantised per row: the
+    serving form of a trained nn.Linear (on a GPU). Rows are laid out at multiples of 16 bytes once, here."""
+
+    def __init__(self, linear: nn.Linear):
+        super().__init__()
+        _on_gpu("Int8Linear", linear.weight)
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        q, scale = quantize_rows(linear.weight)
+        store = torch.zeros((self.out_features, (self.in_features + 15) // 16 * 16), dtype=torch.int8, device=q.device)
+        store[:, :self.in_features] = q
+        self.register_buffer("qweight", store)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+
+    def forward(self, x):
+        return int8_linear(x.detach(), self.qweight[:, :self.in_features], self.weight_scale, self.bias)

@@ -3,6 +3,7 @@ keys (go_zero/model.py:43-97) so checkpoints interchange; inference on the GPU g
 kernels of libazamd (NativeNet), training goes through torch autograd."""
 from __future__ import annotations
 
+import copy
 import ctypes as C
 
 import numpy as np
@@ -10,6 +11,7 @@ import torch
 from torch import nn
 
 from . import _native as N
+from .head import Int8Linear
 
 
 def feature_planes(history_len: int) -> int:
@@ -75,8 +77,17 @@ class AlphaZeroNet(nn.Module):
 
     def forward(self, x):
         """(policy_logits [b, A], value [b])  -- model.py:89-97."""
+        feats, values = self.policy_features(x)
+        return self.policy_fc(feats), values
+
+    def policy_features(self, x):
+        """(inputs of policy_fc [b, 2 n n], value [b]): for a loss that takes the last layer itself (head.linear_cross_entropy)."""
         t = self.tower(self.stem(x))
-        return self.policy_fc(self.policy_head(t).flatten(1)), self.value_head(t).squeeze(1)
+        return self.policy_head(t).flatten(1), self.value_head(t).squeeze(1)
+
+    def int8_heads(self) -> "Int8HeadsNet":
+        """An inference copy whose two wide head layers hold 8-bit weights."""
+        return Int8HeadsNet(self)
 
     # ------------------------------------------------------------------ native inference
     def flat_parameters(self) -> np.ndarray:
@@ -108,6 +119,25 @@ class AlphaZeroNet(nn.Module):
             ent = (fp, NativeNet(self._hyper, self.flat_parameters(), precision, key[1]))
             self._native[key] = ent
         return ent[1]
+
+
+class Int8HeadsNet(nn.Module):
+    """AlphaZeroNet for inference with policy_fc and the first value layer as 8-bit integer products (head.Int8Linear); the rest is a
+    copy of the network's float modules. Called like any evaluator: planes [b, C, n, n] -> (logits, values), MCTS(model=...)."""
+
+    def __init__(self, net: AlphaZeroNet):
+        super().__init__()
+        self.board_size, self.action_dim = net.board_size, net.action_dim
+        self.policy_fc = Int8Linear(net.policy_fc)
+        at = next(i for i, m in enumerate(net.value_head) if isinstance(m, nn.Linear))
+        first = Int8Linear(net.value_head[at])
+        self.stem, self.tower, self.policy_head = (copy.deepcopy(m) for m in (net.stem, net.tower, net.policy_head))
+        self.value_head = nn.Sequential(*(first if i == at else copy.deepcopy(m) for i, m in enumerate(net.value_head)))
+        self.eval().requires_grad_(False)
+
+    def forward(self, x):
+        t = self.tower(self.stem(x))
+        return self.policy_fc(self.policy_head(t).flatten(1)), self.value_head(t).squeeze(1)
 
 
 def _native_auto(self, device=None, shared: bool = True) -> "NativeNet":

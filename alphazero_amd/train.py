@@ -67,6 +67,8 @@ _ENGINE_SPEC = [
     ("lockstep_games", 0, "value"),      # device game slots per GPU (0: as many as the iteration has games, at most 4096)
     ("selfplay_lanes", 0, "value"),      # independent lanes (0: 2 from 256 game slots on, else 1)
     ("no_dedup_leaves", False, "flag"),  # evaluate a leaf reached by several descents of a batch every time, as upstream does
+    ("fused_policy_loss", False, "flag"),  # training step: policy layer and its loss in one operator (head.linear_cross_entropy)
+    ("head_dropout", 0.0, "value"),      # training step: dropout in front of the policy layer (head.dropout)
 ]
 UPSTREAM_FIELDS = tuple(n for n, _, _ in _SPEC)
 ENGINE_FIELDS = tuple(n for n, _, _ in _ENGINE_SPEC)
@@ -438,10 +440,12 @@ def train_candidate(candidate, buffer: ReplayBuffer, cfg):
     when the model lives there; gradients are averaged over the ranks under torch.distributed."""
     from .train_step import DataParallelTrainer
     dev = next(candidate.parameters()).device
+    drop = getattr(cfg, "head_dropout", 0.0)
     trainer = DataParallelTrainer(candidate, lr=cfg.lr, weight_decay=cfg.weight_decay, total_steps=cfg.train_steps_per_iter,
                                   grad_clip_norm=cfg.grad_clip_norm, huber_delta=cfg.value_huber_delta,
                                   entropy_coeff=cfg.policy_entropy_coeff, target_smoothing=cfg.policy_target_smoothing,
-                                  use_amp=cfg.use_amp and str(cfg.device).startswith("cuda"))
+                                  use_amp=cfg.use_amp and str(cfg.device).startswith("cuda"), fused_policy_loss=getattr(cfg, "fused_policy_loss", False),
+                                  head_dropout=drop, dropout_seed=int(torch.randint(1 << 62, ())) if drop > 0.0 else 0)
     use_mirror = dev.type == "cuda"
     if use_mirror:
         try:

@@ -12,6 +12,9 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from . import _native as N
+from .head import dropout, linear_cross_entropy
+
 
 def loss_terms(logits, values, target_policies, target_values, huber_delta=1.0, entropy_coeff=1e-3):
     """train.py:537-541 -> (loss, policy_loss, value_loss)."""
@@ -20,6 +23,13 @@ def loss_terms(logits, values, target_policies, target_values, huber_delta=1.0, 
     value_loss = F.huber_loss(values, target_values, delta=huber_delta)
     entropy = -(F.softmax(logits, dim=1) * logp).sum(dim=1).mean()
     return policy_loss + value_loss - entropy_coeff * entropy, policy_loss, value_loss
+
+
+def head_loss_terms(feats, policy_fc, values, target_policies, target_values, huber_delta=1.0, entropy_coeff=1e-3):
+    """loss_terms with the policy layer taken into the loss (head.linear_cross_entropy): same terms, the logits are not stored."""
+    policy, policy_loss, _ = linear_cross_entropy(feats, policy_fc.weight, target_policies, policy_fc.bias, entropy_coeff=entropy_coeff, parts=True)
+    value_loss = F.huber_loss(values, target_values, delta=huber_delta)
+    return policy + value_loss, policy_loss, value_loss
 
 
 def _staged(dist, t, group):
@@ -53,8 +63,16 @@ def all_reduce_(dist, t, op=None, group=None):
 
 class DataParallelTrainer:
     def __init__(self, model, lr=1e-3, weight_decay=1e-4, total_steps=800, grad_clip_norm=1.0, huber_delta=1.0,
-                 entropy_coeff=1e-3, target_smoothing=0.0, use_amp=False, process_group=None):
+                 entropy_coeff=1e-3, target_smoothing=0.0, use_amp=False, process_group=None, fused_policy_loss=False, head_dropout=0.0, dropout_seed=0):
+        """fused_policy_loss: the policy layer and its loss in one operator; head_dropout: dropout in front of the policy layer, its
+        masks a function of (dropout_seed, rank, step). Both run on a GPU only; without them the step is upstream's."""
         self.model = model
+        self.fused, self.drop = bool(fused_policy_loss), float(head_dropout)
+        if not 0.0 <= self.drop < 1.0:
+            raise ValueError("head_dropout is at least 0 and below 1")
+        if (self.fused or self.drop > 0.0) and next(model.parameters()).device.type != "cuda":
+            raise N.NativeError("fused_policy_loss and head_dropout need the model on a GPU (no CPU fallback)")
+        self.steps = 0
         self.opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=weight_decay)            # train.py:505
         self.sched = torch.optim.lr_scheduler.CosineAnnealingLR(self.opt, T_max=max(1, total_steps), eta_min=lr * 0.1)
         self.clip, self.delta, self.ent = grad_clip_norm, huber_delta, entropy_coeff
@@ -66,6 +84,9 @@ class DataParallelTrainer:
         self.dist = dist if (dist.is_available() and dist.is_initialized()) else None
         self.group = process_group
         self.world = self.dist.get_world_size(process_group) if self.dist else 1
+        # ranks see other samples and take other masks: the generator's key is the seed, its counter (rank, step)
+        self.drop_seed = int(dropout_seed) % (1 << 64)
+        self.rank = self.dist.get_rank(process_group) if self.dist else 0
         # under an initialised process group the gradients always go through the flat buffer and the collective, also with
         # one rank (an identity there): a one-GPU run then executes the code path the N-GPU run takes
         self.reduce = self.dist is not None
@@ -102,8 +123,17 @@ class DataParallelTrainer:
         else:
             self.opt.zero_grad(set_to_none=True)
         with torch.autocast(device_type="cuda", enabled=self.amp):
-            logits, values = self.model(states)
-            loss, pl, vl = loss_terms(logits, values, target_policies, target_values, self.delta, self.ent)
+            if self.fused or self.drop > 0.0:
+                feats, values = self.model.policy_features(states)
+                if self.drop > 0.0:
+                    feats = dropout(feats, self.drop, self.drop_seed, (self.rank << 40) + self.steps)
+                if self.fused:
+                    loss, pl, vl = head_loss_terms(feats, self.model.policy_fc, values, target_policies, target_values, self.delta, self.ent)
+                else:
+                    loss, pl, vl = loss_terms(self.model.policy_fc(feats), values, target_policies, target_values, self.delta, self.ent)
+            else:
+                logits, values = self.model(states)
+                loss, pl, vl = loss_terms(logits, values, target_policies, target_values, self.delta, self.ent)
         self.scaler.scale(loss).backward()
         if self.reduce:   # before unscale_: every rank then sees the same overflow verdict and the same scale
             self._allreduce_grads()
@@ -112,4 +142,5 @@ class DataParallelTrainer:
         self.scaler.step(self.opt)
         self.scaler.update()
         self.sched.step()
+        self.steps += 1
         return float(loss.item()), float(pl.item()), float(vl.item())

@@ -335,6 +335,72 @@ int az_replay_gather(const uint8_t* bits, const float* caps, const float* pi, co
 int az_pack_planes(const float* planes, int32_t count, int32_t board_size, int32_t history_len, int32_t row_bytes, uint8_t* bits,
                    float* caps, void* stream);
 
+/* ---- operators around a network's last matrix product ------------------------------------------------------------------
+ * No counterpart upstream: the loss there is log_softmax of stored logits (train.py:537-541). Row-major matrices whose rows may be
+ * further apart than they are long (pitches in elements); every call enqueues on `stream` and allocates nothing: scratch memory is
+ * the caller's `workspace` (256-byte aligned, contents undefined before and after, not shared by calls that may overlap). */
+typedef enum { AZ_DT_F32 = 0, AZ_DT_BF16 = 1, AZ_DT_F16 = 2, AZ_DT_I8 = 3 } az_dtype;
+typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2 } az_reduce;
+
+/* Cross entropy of softmax(x weight^T + bias) against class indices or against rows of target weights, minus entropy_coeff times
+ * the softmax' entropy; the logits are never stored. Rows whose index is ignore_index cost nothing, get zero gradients and stay
+ * out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
+ * -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax and gives NaN. */
+typedef struct {
+    const void* x;            /* [rows, features] of dtype */
+    const void* weight;       /* [classes, features] of dtype */
+    const void* bias;         /* [classes] of dtype, or NULL */
+    const void* target;       /* int64 [rows], or float [rows, classes] with target_dense */
+    int64_t rows, features, classes;            /* at least 1; rows, classes <= 2^30, rows, features <= 4194000 */
+    int64_t x_pitch, weight_pitch, target_pitch;
+    int64_t ignore_index;
+    int32_t dtype;            /* AZ_DT_F32 / BF16 / F16 */
+    int32_t target_dense;
+    int32_t reduction;        /* az_reduce; NONE: one gradient per row is handed to the backward call */
+    float entropy_coeff;
+} az_linear_ce_args;
+
+/* Bytes of scratch memory of a forward (backward = 0) or backward call, or a negative az_status. */
+int64_t az_linear_ce_workspace(const az_linear_ce_args* args, int32_t backward);
+
+/* kept: float [3 * rows + 2], for the backward call. loss, ce, ent: the loss, its cross entropy and the softmax' entropy, one
+ * float each (mean or sum over the rows that count), or [rows] with AZ_REDUCE_NONE; ce and ent may be NULL. */
+int az_linear_ce_forward(const az_linear_ce_args* args, float* kept, float* loss, float* ce, float* ent, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* Gradients (of dtype, contiguous, 16-byte aligned; any may be NULL) for `grad`, the gradient of the loss: one float, or [rows]
+ * with AZ_REDUCE_NONE. The arguments are the forward call's. */
+int az_linear_ce_backward(const az_linear_ce_args* args, const float* kept, const float* grad, void* grad_x, void* grad_weight,
+                          void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = residual + (kept ? x * 65536 / (65536 - threshold) : 0) over `count` elements (residual may be NULL). Position i is kept
+ * where 16 bits of Philox4x32-10 reach the threshold: bits i % 8 (low half of a word first) of counter (i / 8, offset) under the
+ * key seed, or *seed_dev, read when the kernel runs, where that is not NULL. */
+int az_dropout(const void* x, const void* residual, void* y, int64_t count, int32_t dtype, int32_t threshold, uint64_t seed,
+               const uint64_t* seed_dev, uint64_t offset, void* stream);
+
+/* q = rint(127 x / max|x|) (ties to even) and scale = max|x| / 127 for each row; pitch in elements, q_pitch in bytes. A row of zeros
+ * has scale 0, a row with an infinity or NaN has q = 0 and scale NaN. */
+int az_quantize_rows(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t pitch, int8_t* q, int64_t q_pitch, float* scale,
+                     void* stream);
+
+/* y[m][n] = x_scale[m] * weight_scale[n] * sum_k x[m][k] weight[n][k] + bias[n], the sum in 32-bit integers. x is int8 with
+ * x_scale, or floating and quantised row by row on the way (x_scale unused). */
+typedef struct {
+    const void* x;            /* [tokens, features] of x_dtype */
+    const int8_t* weight;     /* [channels, features] */
+    const float* x_scale;     /* [tokens], x_dtype AZ_DT_I8 only */
+    const float* weight_scale;  /* [channels] */
+    const void* bias;         /* [channels] of bias_dtype, or NULL */
+    void* y;                  /* [tokens, channels] of y_dtype, contiguous, 16-byte aligned */
+    int64_t tokens, features, channels;     /* at least 1; features <= 131071 */
+    int64_t x_pitch, weight_pitch;
+    int32_t x_dtype, bias_dtype, y_dtype;
+} az_int8_args;
+
+int64_t az_int8_workspace(const az_int8_args* args);
+int az_int8_linear(const az_int8_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

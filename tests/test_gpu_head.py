@@ -1,0 +1,587 @@
+"""The operators of alphazero_amd.head on the GPU against plain forms in 64 bits (head_ref.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import head_ref as R
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = [F32, BF16, F16]
+ids = lambda v: str(v).replace("torch.", "").replace(" ", "")  # noqa: E731
+
+
+def _head():
+    from alphazero_amd import head
+    return head
+
+
+def _inputs(rows, feats, classes, dtype, dense, bias, seed=0, device="cuda"):
+    g = torch.Generator(device=device).manual_seed(1000 * rows + 10 * feats + classes + seed)
+    x = torch.randn((rows, feats), generator=g, device=device).to(dtype)
+    w = (torch.randn((classes, feats), generator=g, device=device) * (2.0 / math.sqrt(feats))).to(dtype)
+    b = (torch.randn(classes, generator=g, device=device) * 0.3).to(dtype) if bias else None
+    if dense:
+        t = torch.rand((rows, classes), generator=g, device=device) ** 4
+        t = torch.where(t < 0.3, 0.0, t) + 1e-3
+        t = t / t.sum(1, keepdim=True) * (0.5 + torch.rand((rows, 1), generator=g, device=device))      # need not sum to one
+    else:
+        t = torch.randint(classes, (rows,), generator=g, device=device)
+        if rows > 2:
+            t[torch.rand(rows, generator=g, device=device) < 0.2] = -100
+            t[0] = classes - 1
+    return x, w, b, t
+
+
+def _run(x, w, b, t, grad=None, **kw):
+    """(loss, ce, ent, gx, gw, gb) of the operator with fresh leaves."""
+    leaves = [v.detach().clone().requires_grad_(True) if v is not None else None for v in (x, w, b)]
+    loss, ce, ent = _head().linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], parts=True, **kw)
+    loss.backward(torch.ones_like(loss) if grad is None else grad)
+    return (loss.detach(), ce, ent, *(v.grad if v is not None else None for v in leaves))
+
+
+def _check(x, w, b, t, c=0.0, reduction="mean", grad=None, ignore=-100):
+    got = _run(x, w, b, t, grad, entropy_coeff=c, reduction=reduction, ignore_index=ignore)
+    ref = R.loss_reference(x, w, t, b, ignore, c, reduction, torch.ones((), device=x.device) if grad is None else grad)
+    counts = slice(None) if t.is_floating_point() or reduction != "none" else t != ignore
+    for name, v in zip(("loss", "ce", "ent"), got):
+        pick = counts if v.dim() else ()
+        R.close(name, v[pick], (ref[name][0][pick], ref[name][1][pick]))
+    for name, v in zip(("gx", "gw", "gb"), got[3:]):
+        if v is not None:
+            R.close(name, v, ref[name])
+    return got
+
+
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 5, 7), (64, 64, 64), (65, 72, 130), (256, 162, 82), (17, 1000, 300), (300, 200, 513), (130, 722, 362)]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_loss_and_gradients(size, dtype, dense):
+    x, w, b, t = _inputs(*size, dtype, dense, bias=size[0] % 2 == 1 or size[0] == 256)
+    scale = 256.0 if dtype == F16 else 1.0
+    _check(x, w, b, t, grad=torch.tensor(scale, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_entropy_and_reductions(dtype, dense, reduction):
+    x, w, b, t = _inputs(200, 96, 150, dtype, dense, True)
+    g = torch.linspace(-3, 5, 200, device="cuda") if reduction == "none" else torch.tensor(7.0, device="cuda")
+    _check(x, w, b, t, c=0.05, reduction=reduction, grad=g)
+
+
+@pytest.mark.parametrize("size", [(520, 64, 20000), (2048, 128, 3000), (5000, 40, 700)], ids=ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_large_and_middle_tiles(size, dtype):
+    x, w, b, t = _inputs(*size, dtype, False, True)
+    _check(x, w, b, t, c=0.01, grad=torch.tensor(512.0 if dtype == F16 else 1.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16], ids=ids)
+def test_dense_large_tiles(dtype):
+    x, w, b, t = _inputs(4096, 48, 3300, dtype, True, True)
+    _check(x, w, b, t, c=0.01, grad=torch.tensor(512.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+def test_pieces_of_the_classes(dtype):
+    rows, classes = (2800, 33000) if dtype == F32 else (8200, 33000)     # more than one piece: 1 GB / (4 bytes x planes x rows)
+    x, w, b, t = _inputs(rows, 16, classes, dtype, False, True)
+    _check(x, w, b, t)
+
+
+def test_gradient_by_differences():
+    """Float32 gradients against central differences of the 64-bit loss along random directions."""
+    x, w, b, t = _inputs(40, 33, 57, F32, True, True)
+    _, _, _, gx, gw, gb = _run(x, w, b, t, entropy_coeff=0.1)
+
+    def f(dx, dw, db, h):
+        logp = torch.log_softmax((x.double() + h * dx) @ (w.double() + h * dw).t() + b.double() + h * db, 1)
+        return (-(t.double() * logp).sum(1) + 0.1 * (logp.exp() * logp).sum(1)).mean()
+
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        d = [torch.randn(v.shape, generator=g, device="cuda", dtype=torch.float64) for v in (x, w, b)]
+        h = 1e-5
+        want = (f(*d, h) - f(*d, -h)) / (2 * h)
+        have = sum((a.double() * v).sum() for a, v in zip((gx, gw, gb), d))
+        # differences are off by h^2 times the third derivative (~1e-8 here), the gradients by 2^-20 of their magnitude
+        size = sum((a.double().abs() * v.abs()).sum() for a, v in zip((gx, gw, gb), d))
+        assert abs(float(want - have)) <= 2.0 ** -18 * float(size) + 1e-7
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_rows_that_do_not_count_may_hold_anything(dtype):
+    x, w, b, t = _inputs(70, 40, 90, dtype, False, True)
+    out = (t == -100).nonzero()[:, 0]
+    assert len(out) >= 3
+    x[out[0]], x[out[1]], x[out[2], 3] = float("nan"), float("inf"), -float("inf")
+    got = _check(x, w, b, t, c=0.01)
+    assert (got[3][out] == 0).all()
+    none = _run(x, w, b, t, reduction="none")
+    assert (none[0][out] == 0).all()
+
+
+def test_no_row_counts():
+    x, w, b, t = _inputs(20, 16, 30, BF16, False, True)
+    t[:] = -100
+    loss, _, _, gx, gw, gb = _run(x, w, b, t)
+    assert math.isnan(float(loss))                      # a mean of nothing, as in torch
+    assert not gx.any() and not gw.any() and not gb.any()
+    assert float(_run(x, w, b, t, reduction="sum")[0]) == 0.0
+
+
+def test_other_ignore_index_and_last_row():
+    x, w, b, t = _inputs(33, 16, 30, F32, False, True)
+    t[t == -100] = 5
+    t[32] = 7
+    _check(x, w, b, t, ignore=5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_classes_that_cannot_be(dtype, dense):
+    x, w, b, t = _inputs(50, 24, 200, dtype, dense, True)
+    shut = torch.arange(200, device="cuda") % 3 == 0
+    shut[64:192] = True                                  # whole tiles of them
+    b[shut] = -float("inf")
+    if dense:
+        t = torch.where(shut, 0.0, t)
+    else:
+        t = torch.where(t == -100, t, torch.where(shut[t.clamp(min=0)], 1, t))
+    got = _check(x, w, b, t, c=0.05)
+    assert not got[5][shut].any() and not got[4][shut].any()
+    b[:] = torch.finfo(dtype).min                        # the type's lowest value everywhere is still a softmax
+    loss = _run(x * 0, w, b, t, reduction="none")[1]
+    live = slice(None) if dense else t != -100
+    total = t.sum(1) if dense else 1.0
+    # logits of 1e38 have steps of 1e31: only finiteness and, with equal logits, log(classes) up to that step can be asked for
+    assert torch.isfinite(loss[live]).all()
+    if dtype == F16:                                     # 65504 has steps of 2^-8 in float32
+        assert ((loss - total * math.log(200)).abs()[live] <= 2.0 ** -7 * 200 * 2.0 ** -8 + 0.05).all()
+
+
+def test_row_without_a_softmax():
+    x, w, b, t = _inputs(5, 8, 12, F32, False, True)
+    t[:] = torch.tensor([1, 2, 3, 4, -100], device="cuda")
+    b[:] = -float("inf")
+    loss = _run(x, w, b, t, reduction="none")[0]
+    assert torch.isnan(loss[:4]).all() and float(loss[4]) == 0.0
+    b[:] = 0
+    b[3] = -float("inf")                                 # the target itself cannot be: an infinite loss, the others stay
+    loss = _run(x, w, b, t, reduction="none")[0]
+    assert float(loss[2]) == float("inf") and torch.isfinite(loss[:2]).all()
+
+
+def test_index_outside_the_classes():
+    x, w, b, t = _inputs(40, 16, 30, BF16, False, True)
+    for wrong in (30, -1, 1 << 40, -(1 << 62)):
+        u = t.clone()
+        u[3] = wrong
+        rows = _run(x, w, b, u, reduction="none")[0]
+        assert math.isnan(float(rows[3])) and torch.isfinite(rows[torch.arange(40) != 3]).all()
+        loss, _, _, gx, gw, gb = _run(x, w, b, u)
+        assert math.isnan(float(loss)) and torch.isnan(gx[3]).all() and torch.isnan(gw).any() and torch.isnan(gb).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_layouts(dtype):
+    head = _head()
+    x, w, b, t = _inputs(60, 40, 70, dtype, True, True)
+    want = _run(x, w, b, t, entropy_coeff=0.01)
+    big = torch.full((80, 64), float("nan"), device="cuda", dtype=dtype)
+    wide = torch.full((90, 56), float("nan"), device="cuda", dtype=dtype)
+    tt = torch.full((60, 99), float("nan"), device="cuda")
+    for dr, dc in ((0, 0), (3, 8), (5, 1)):              # aligned rows of a larger matrix, and rows that start anywhere
+        big[dr:dr + 60, dc:dc + 40] = x
+        wide[dr:dr + 70, dc:dc + 40] = w
+        tt[:, dc:dc + 70] = t
+        got = _run_views(big[dr:dr + 60, dc:dc + 40], wide[dr:dr + 70, dc:dc + 40], b, tt[:, dc:dc + 70])
+        for a, v in zip(want, got):
+            assert torch.equal(a, v)
+    xt = x.t().contiguous().t()                          # columns first
+    assert torch.equal(head.linear_cross_entropy(xt, w, t, b, entropy_coeff=0.01), want[0])
+    x3 = x.reshape(3, 20, 40)
+    assert torch.equal(head.linear_cross_entropy(x3, w, t.reshape(3, 20, 70), b, entropy_coeff=0.01), want[0])
+    rows = head.linear_cross_entropy(x3, w, t.reshape(3, 20, 70), b, reduction="none")
+    assert rows.shape == (3, 20)
+    one = x[:1].expand(60, 40)                           # a row many times: stride 0
+    assert torch.equal(head.linear_cross_entropy(one, w, t, b), head.linear_cross_entropy(one.contiguous(), w, t, b))
+
+
+def _run_views(x, w, b, t):
+    x, w, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True), b.detach().clone().requires_grad_(True)
+    loss, ce, ent = _head().linear_cross_entropy(x, w, t, b, entropy_coeff=0.01, parts=True)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    return loss.detach(), ce, ent, gx, gw, gb
+
+
+def test_some_gradients_only():
+    x, w, b, t = _inputs(100, 48, 77, BF16, False, True)
+    full = _run(x, w, b, t)
+    for k in range(3):
+        leaves = [v.detach().clone().requires_grad_(i == k) for i, v in enumerate((x, w, b))]
+        loss = _head().linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        (g,) = torch.autograd.grad(loss, leaves[k])
+        assert torch.equal(g, full[3 + k])
+
+
+def test_same_bits_every_time_and_broadcast_gradient():
+    x, w, b, t = _inputs(500, 100, 3000, F16, False, True)
+    first = _run(x, w, b, t, entropy_coeff=0.01)
+    for a, v in zip(first, _run(x, w, b, t, entropy_coeff=0.01)):
+        assert torch.equal(a, v)
+    xs = x.clone().requires_grad_(True)
+    rows = _head().linear_cross_entropy(xs, w, t, b, reduction="none")
+    rows.sum().backward()                                # the gradient of a sum is one value with stride 0
+    ref = R.loss_reference(x, w, t, b, grad=torch.ones(500, device="cuda"), reduction="none")
+    R.close("gx", xs.grad, ref["gx"])
+
+
+def test_autocast_like_a_linear_layer():
+    x, w, b, t = _inputs(64, 32, 50, F32, True, True)
+    w.requires_grad_(True)
+    with torch.autocast("cuda", dtype=BF16):
+        loss = _head().linear_cross_entropy(x, w, t, b)
+    loss.backward()
+    assert w.grad.dtype == F32
+    assert torch.equal(loss, _head().linear_cross_entropy(x.bfloat16(), w.bfloat16(), t, b.bfloat16()))
+
+
+def test_no_rows():
+    head = _head()
+    w = torch.randn(5, 4, device="cuda", requires_grad=True)
+    x = torch.empty(0, 4, device="cuda", requires_grad=True)
+    t = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert math.isnan(float(head.linear_cross_entropy(x, w, t).detach()))
+    s = head.linear_cross_entropy(x, w, t, reduction="sum")
+    s.backward()
+    assert float(s.detach()) == 0.0 and not w.grad.any() and x.grad.shape == (0, 4)
+    assert head.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------------ dropout
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("count", [1, 7, 8, 9, 255, 2048, 2049, 100003])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(dtype, count, p):
+    head = _head()
+    g = torch.Generator(device="cuda").manual_seed(count)
+    x, r, gy = (torch.randn(count, generator=g, device="cuda").to(dtype) for _ in range(3))
+    seed, offset = 0x0123456789ABCDEF ^ (count << 33), count * 977 + (1 << 40)
+    kept = torch.from_numpy(R.philox_kept(count, p, seed, offset)[0]).cuda()
+    t = round(65536 * p)
+    scale = 65536 / (65536 - t) if t < 65536 else 0.0
+    for residual in (None, r):
+        xs = x.clone().requires_grad_(True)
+        rs = None if residual is None else residual.clone().requires_grad_(True)
+        y = head.dropout(xs, p, seed, offset, residual=rs)
+        want = torch.where(kept, x.double() * scale, 0.0) + (0 if residual is None else r.double())
+        mag = torch.where(kept, (x.double() * scale).abs(), 0.0) + (0 if residual is None else r.double().abs())
+        R.close("y", y.detach(), (want, R.U[dtype] * want.abs() + 4 * R.F32 * mag + R.TINY[dtype]))
+        y.backward(gy)
+        gw = torch.where(kept, gy.double() * scale, 0.0)
+        R.close("gx", xs.grad, (gw, R.U[dtype] * gw.abs() + 4 * R.F32 * gw.abs() + R.TINY[dtype]))
+        assert not xs.grad[~kept].any()
+        if rs is not None:
+            assert torch.equal(rs.grad, gy)
+
+
+def test_dropout_layouts_and_masks():
+    head = _head()
+    x = torch.randn(64, 37, device="cuda")
+    y = head.dropout(x, 0.3, 5)
+    assert torch.equal(head.dropout(x.t().contiguous().t(), 0.3, 5), y)                    # by position, not by address
+    buf = torch.zeros(64 * 37 + 1, device="cuda")
+    buf[1:] = x.reshape(-1)
+    assert torch.equal(head.dropout(buf[1:].view(64, 37), 0.3, 5), y)                      # not at a multiple of 16 bytes
+    assert not torch.equal(head.dropout(x, 0.3, 6), y) and not torch.equal(head.dropout(x, 0.3, 5, 1), y)
+    seed = torch.tensor([5], device="cuda")
+    assert torch.equal(head.dropout(x, 0.3, seed), y)
+    negative = torch.tensor(-1, device="cuda")
+    assert torch.equal(head.dropout(x, 0.3, negative), head.dropout(x, 0.3, (1 << 64) - 1))
+    bad = x.clone()
+    dropped = y == 0
+    bad[dropped] = float("nan")
+    assert torch.equal(head.dropout(bad, 0.3, 5), y)
+    xs = x.clone().requires_grad_(True)
+    head.dropout(xs, 0.3, 5).sum().backward()                                              # a gradient with stride 0
+    assert torch.equal(xs.grad == 0, dropped)
+    assert head.dropout(torch.empty(0, 3, device="cuda"), 0.3, 5).shape == (0, 3)
+    share = float((head.dropout(torch.ones(1 << 20, device="cuda"), 0.1, 3) == 0).float().mean())
+    assert abs(share - 0.1) < 6 * math.sqrt(0.09 / (1 << 20))                              # six standard deviations
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit integers
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("size", [(1, 1), (3, 15), (5, 16), (4, 162), (2, 4097), (3, 23104)], ids=ids)
+def test_quantize_rows(dtype, size):
+    g = torch.Generator(device="cuda").manual_seed(size[1])
+    x = torch.randn(size, generator=g, device="cuda").to(dtype)
+    if size[1] > 8:
+        x[-1] = 0
+        x[0, :4] = torch.tensor([127.0, 0.5, 1.5, -2.5])                                   # ties, with max 127 at least
+        x[0, 4:] = x[0, 4:].clamp(-100, 100)
+    q, s = _head().quantize_rows(x)
+    rq, rs = R.quantize_reference(x)
+    assert torch.equal(q.cpu(), rq) and torch.equal(s.cpu(), rs)
+
+
+def test_quantize_rows_near_halves_and_odd_values():
+    head = _head()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    top = torch.rand(64, 1, generator=g, device="cuda") * 3 + 0.1
+    x = (top.double() * (torch.randint(-127, 127, (64, 200), generator=g, device="cuda") + 0.5) / 127).float()    # as near to a half as float32 gets
+    x[:, :1] = top
+    q, s = head.quantize_rows(x)
+    rq, rs = R.quantize_reference(x)
+    assert torch.equal(q.cpu(), rq) and torch.equal(s.cpu(), rs)
+    x = torch.tensor([[1e-40, -2e-40, 0.0], [3e38, -1e38, 0.0], [float("inf"), 1.0, 2.0], [float("nan"), 1.0, 2.0], [0.0, -0.0, 0.0]], device="cuda")
+    q, s = head.quantize_rows(x)
+    # 1e-40 and 2e-40 are 71362 and 142725 of float32's smallest steps: 127 * 71362 / 142725 = 63.49956
+    assert q.cpu().tolist() == [[63, -127, 0], [127, -42, 0], [0, 0, 0], [0, 0, 0], [0, 0, 0]]
+    assert torch.isnan(s[2:4]).all() and float(s[4]) == 0.0
+    y = head.int8_linear(x, torch.ones(4, 3, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"))
+    assert torch.isnan(y[2:4]).all() and torch.isfinite(y[[0, 1, 4]]).all()
+
+
+def _int8_check(x, qw, ws, b, y, q, s):
+    dt = y.dtype
+    sums = q.double() @ qw.double().t()
+    want = sums * s.double()[..., None] * ws.double() + (0 if b is None else b.double())
+    mag = (sums * s.double()[..., None] * ws.double()).abs() + (0 if b is None else b.double().abs())
+    R.close("y", y, (want, R.U[dt] * want.abs() + 8 * R.F32 * mag + R.TINY[dt]))
+
+
+INT8 = [(1, 1, 1), (1, 64, 16), (1, 4096, 1024), (5, 100, 33), (16, 130, 50), (17, 2000, 83), (33, 77, 300), (64, 512, 128), (65, 64, 64), (70, 1000, 90),
+        (256, 3000, 256), (300, 129, 517), (1024, 200, 2500), (2304, 256, 5632)]
+
+
+@pytest.mark.parametrize("size", INT8, ids=ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_int8_linear(size, dtype):
+    head = _head()
+    m, k, n = size
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x = torch.randn((m, k), generator=g, device="cuda").to(dtype)
+    qw = torch.randint(-127, 128, (n, k), generator=g, device="cuda").to(torch.int8)
+    ws = torch.rand(n, generator=g, device="cuda") / 127
+    b = torch.randn(n, generator=g, device="cuda").to(dtype) if n % 2 else None
+    q, s = head.quantize_rows(x)
+    y = head.int8_linear(x, qw, ws, b)
+    assert y.dtype == dtype
+    _int8_check(x, qw, ws, b, y, q, s)
+    y8 = head.int8_linear(q, qw, ws, b, x_scale=s, out_dtype=dtype)
+    assert torch.equal(y8, y)                                                              # the sum is exact on every path
+    assert head.int8_linear(q, qw, ws, x_scale=s).dtype == F32
+
+
+def test_int8_extremes_and_layouts():
+    head = _head()
+    k = 131071
+    for m in (1, 100):
+        x = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+        w = torch.full((70, k), -128, dtype=torch.int8, device="cuda")
+        y = head.int8_linear(x, w, torch.ones(70, device="cuda"), x_scale=torch.ones(m, device="cuda"))
+        assert (y.double() == float(np.float32(k * 16384))).all()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for m in (3, 100):
+        x = torch.randn((m, 200), generator=g, device="cuda")
+        w = torch.randint(-127, 128, (90, 200), generator=g, device="cuda").to(torch.int8)
+        ws = torch.rand(90, generator=g, device="cuda")
+        want = head.int8_linear(x, w, ws)
+        for dc, width in ((0, 208), (16, 256), (5, 233), (1, 201)):
+            big = torch.full((90, width), 77, dtype=torch.int8, device="cuda")
+            big[:, dc:dc + 200] = w
+            xb = torch.full((m, 300), float("nan"), device="cuda")
+            xb[:, dc:dc + 200] = x
+            assert torch.equal(head.int8_linear(xb[:, dc:dc + 200], big[:, dc:dc + 200], ws), want)
+        assert torch.equal(head.int8_linear(x.reshape(m, 1, 200), w, ws), want.reshape(m, 1, 90))
+        assert torch.equal(head.int8_linear(x, w.t().contiguous().t(), ws), want)
+    assert head.int8_linear(torch.empty(0, 200, device="cuda"), w, ws).shape == (0, 90)
+
+
+def test_int8_layer():
+    head = _head()
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(163, 83).cuda()
+    q = head.Int8Linear(lin)
+    x = torch.randn(40, 163, device="cuda")
+    y = q(x)
+    # each product is off by half a step of both operands: |x| w_step / 2 + |w| x_step / 2 + a quarter of their product
+    xs, wsc = x.abs().amax(1, keepdim=True) / 127, lin.weight.abs().amax(1) / 127
+    tol = x.abs().sum(1, keepdim=True) * wsc / 2 + xs * lin.weight.abs().sum(1) / 2 + 163 * xs * wsc / 4
+    assert ((y - lin(x)).abs() <= tol * 1.0001 + 1e-5).all()
+    other = head.Int8Linear(torch.nn.Linear(163, 83).cuda())
+    other.load_state_dict(q.state_dict())
+    assert torch.equal(other(x), y)
+
+
+# ------------------------------------------------------------------------------------------------ together, streams, graphs
+def test_training_step_of_a_head():
+    """Dropout with a residual, then the loss, and back: against the same in 64 bits with the operator's own mask."""
+    head = _head()
+    x, w, b, t = _inputs(128, 64, 90, F32, True, True)
+    r = torch.randn(128, 64, device="cuda")
+    leaves = [v.clone().requires_grad_(True) for v in (x, r, w, b)]
+    h = head.dropout(leaves[0], 0.25, 11, 4, residual=leaves[1])
+    loss = head.linear_cross_entropy(h, leaves[2], t, leaves[3], entropy_coeff=0.01)
+    loss.backward()
+    ref = R.loss_reference(h.detach(), w, t, b, c=0.01, grad=torch.ones((), device="cuda"))
+    R.close("loss", loss.detach(), ref["loss"])
+    kept = torch.from_numpy(R.philox_kept(128 * 64, 0.25, 11, 4)[0]).cuda().view(128, 64)
+    gx, tol = ref["gx"]
+    R.close("residual", leaves[1].grad, (gx, tol))
+    scale = 65536 / (65536 - round(65536 * 0.25))
+    R.close("x", leaves[0].grad, (torch.where(kept, gx * scale, 0.0), torch.where(kept, tol * scale + 4 * R.F32 * gx.abs(), 0.0)))
+    R.close("w", leaves[2].grad, ref["gw"])
+    with torch.no_grad():        # the served form of the same layer
+        lin = torch.nn.Linear(64, 90).cuda()
+        lin.weight.copy_(w)
+        lin.bias.copy_(b)
+        y = head.Int8Linear(lin)(h)
+    assert y.shape == (128, 90)
+
+
+def test_other_streams_at_once():
+    head = _head()
+    x, w, b, t = _inputs(600, 96, 2000, BF16, False, True)
+    want = _run(x, w, b, t)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(_run(x, w, b, t))
+    torch.cuda.synchronize()
+    for g in got:
+        for a, v in zip(want, g):
+            assert torch.equal(a, v)
+
+
+def test_captured_and_replayed():
+    """Forward and backward of dropout + loss in one graph, replayed with other inputs and seeds, eager work between."""
+    head = _head()
+    x, w, b, t = _inputs(300, 72, 500, F16, False, True)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    seed = torch.tensor([1], device="cuda")
+    g1 = torch.tensor(64.0, device="cuda")
+
+    def step():
+        h = head.dropout(x, 0.2, seed)
+        loss = head.linear_cross_entropy(h, w, t, b, entropy_coeff=0.01)
+        gx, gw = torch.autograd.grad(loss, (x, w), g1)
+        with torch.no_grad():
+            y = head.int8_linear(h.detach(), q, ws)
+        return loss.detach(), gx, gw, y
+
+    q, ws = head.quantize_rows(w.detach())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.cuda.graph(second):      # another one, with scratch memory of its own pool
+        out2 = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(300, 72, device="cuda") + k)
+        seed.fill_(100 + k)
+        want = [v.clone() for v in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        for a, v, u in zip(want, out, out2):
+            assert torch.equal(a, v) and torch.equal(a, u)
+
+
+# ------------------------------------------------------------------------------------------------ the framework's own callers
+def _net_and_batch(seed=0, n=5, rows=48):
+    import stubnets
+    from alphazero_amd.model import AlphaZeroNet
+    torch.manual_seed(seed)
+    net = AlphaZeroNet(board_size=n, channels=32, num_blocks=1).cuda()
+    x = torch.from_numpy(stubnets.synthetic_planes(rows, 21, n, seed=seed + 1)).cuda()
+    pi = torch.softmax(2 * torch.randn(rows, n * n + 1, device="cuda"), 1)
+    z = torch.rand(rows, device="cuda") * 2 - 1
+    return net, x, pi, z
+
+
+@pytest.mark.parametrize("amp", [False, True])
+def test_training_step_with_the_fused_policy_loss(amp):
+    import copy
+    from alphazero_amd.train_step import DataParallelTrainer, head_loss_terms, loss_terms
+    net, x, pi, z = _net_and_batch()
+    net.train()
+    with torch.autocast("cuda", enabled=amp):
+        feats, v = net.policy_features(x)
+        feats, v = feats.detach(), v.detach()
+        fused = head_loss_terms(feats, net.policy_fc, v, pi, z)
+        plain = loss_terms(net.policy_fc(feats), v, pi, z)
+    ref = R.loss_reference(feats, net.policy_fc.weight.to(feats.dtype), pi, net.policy_fc.bias.to(feats.dtype), c=1e-3)
+    R.close("policy loss", fused[1].detach(), ref["ce"])
+    assert torch.equal(fused[2], plain[2])
+    # under autocast the stored logits are rounded to float16: half a step of the largest, twice (logit and normaliser)
+    step = 2 * 2.0 ** -11 * 8 if amp else 1e-5
+    assert abs(float(fused[0].detach() - plain[0].detach())) <= step
+    runs = []
+    for kw in (dict(fused_policy_loss=True), dict(fused_policy_loss=True), dict(fused_policy_loss=True, head_dropout=0.2, dropout_seed=3),
+               dict(fused_policy_loss=True, head_dropout=0.2, dropout_seed=3), dict(head_dropout=0.2, dropout_seed=4)):
+        m = copy.deepcopy(net)
+        t = DataParallelTrainer(m, use_amp=amp, **kw)
+        losses = [t.step(x, pi, z) for _ in range(3)]
+        assert all(np.isfinite(v).all() for v in losses)
+        assert any(not torch.equal(a, b) for a, b in zip(m.parameters(), net.parameters()))
+        runs.append(losses)
+    assert abs(runs[0][0][1] - float(ref["ce"][0])) <= 1e-2 and runs[2][0] != runs[0][0] and runs[4][0] != runs[2][0]
+    assert runs[0][0] == runs[1][0] and runs[2][0] == runs[3][0]
+
+
+def test_command_line_knobs_reach_the_step():
+    from alphazero_amd import train as T
+    cfg = T.parse_args(["--device", "cuda", "--board-size", "5", "--channels", "32", "--num-blocks", "1", "--train-steps-per-iter", "2", "--batch-size", "16",
+                        "--fused-policy-loss", "--head-dropout", "0.1"])
+    assert cfg.fused_policy_loss and cfg.head_dropout == 0.1
+    import stubnets
+    buf = T.ReplayBuffer(64)
+    planes = stubnets.synthetic_planes(32, 21, 5, seed=3)
+    rng = np.random.RandomState(0)
+    buf.extend([(planes[i], rng.dirichlet(np.ones(26)).astype(np.float32), float(rng.uniform(-1, 1)), 1.0) for i in range(32)])
+    T.set_seed(1)
+    model = T.build_model(cfg).to("cuda")
+    loss = T.train_candidate(model, buf, cfg)
+    assert np.isfinite(loss).all()
+
+
+def test_network_with_int8_heads():
+    net, x, _, _ = _net_and_batch(n=9, rows=70)
+    net.eval()
+    q = net.int8_heads()
+    with torch.no_grad():
+        feats, _ = net.policy_features(x)
+        lg, v = net(x)
+        lq, vq = q(x)
+    w = net.policy_fc.weight.detach()
+    xs, ws = feats.abs().amax(1, keepdim=True) / 127, w.abs().amax(1) / 127
+    tol = feats.abs().sum(1, keepdim=True) * ws / 2 + xs * w.abs().sum(1) / 2 + w.shape[1] * xs * ws / 4
+    assert ((lq - lg).abs() <= tol * 1.001 + 1e-5).all()
+    assert vq.shape == v.shape and torch.isfinite(vq).all() and (vq.abs() <= 1).all()
+    net.native("f32")
+    assert torch.equal(net.int8_heads()(x)[0], lq)        # also from a network with native handles
+    from alphazero_amd.go import GoState
+    from alphazero_amd.mcts import MCTS
+    pi, action = MCTS(model=q, device="cuda", num_simulations=16, inference_batch_size=4).run(GoState.new_game(9), temperature=1e-6, add_exploration_noise=False)[:2]
+    assert abs(float(np.sum(pi)) - 1) < 1e-6
