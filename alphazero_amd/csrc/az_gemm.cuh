@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace az {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -55,6 +57,7 @@ struct MmTile {
     static constexpr int LP = BP / 8 / WAVES, LQ = BQ / 8 / WAVES;   // 1 KB loads of a wave per stage
     static constexpr int STAGE = (BP + BQ) * 128;
     static constexpr int LDS = 2 * STAGE;
+    static_assert((STAGE & (STAGE - 1)) == 0, "stages are told apart by one bit");
     static_assert(BP % (8 * WAVES) == 0 && BQ % (8 * WAVES) == 0 && TP % 16 == 0 && TQ % 16 == 0, "tile shape");
     typedef typename MmAcc<KIND>::type acc_t;
 };
@@ -88,7 +91,9 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     const int64_t pext = ((int64_t)P.rows - p0 - 1) * P.pitch + kbytes, qext = ((int64_t)Q.rows - q0 - 1) * Q.pitch + kbytes;
     int ks = split ? k_first / ksteps : 0;      // segment and step within it of the next stage to fetch
     int kk = k_first - ks * ksteps;
+    int left = k_last - k_first;                // stages still to fetch
 
+    // A stage past the last one is fetched too, out of range of an empty matrix: zeros arrive and the loop needs no branch.
     auto fetch = [&](int stage) {
         const int k = kk << 7;
         const char* pb = pbase + k;
@@ -98,18 +103,20 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
             qb += mm_plane_q(ks) * Q.plane;
         }
         const int64_t pn = pext - k, qn = qext - k;
-        const int pr = pn < 0 ? 0 : (pn > 0x7fffffff ? 0x7fffffff : (int)pn), qr = qn < 0 ? 0 : (qn > 0x7fffffff ? 0x7fffffff : (int)qn);
+        const bool none = left <= 0;
+        const int pr = pn < 0 || none ? 0 : (pn > 0x7fffffff ? 0x7fffffff : (int)pn), qr = qn < 0 || none ? 0 : (qn > 0x7fffffff ? 0x7fffffff : (int)qn);
         const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)pb, 0, pr, 0x00020000);
         const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, qr, 0x00020000);
         // pieces behind the row's end would read the next row: sent out of range instead
         const int past = k + piece * 16 >= kbytes ? (int)0x80000000 : 0;
-        char* dst = lds + stage * T::STAGE + wave * 1024;
+        char* dst = lds + stage + wave * 1024;
 #pragma unroll
         for (int i = 0; i < T::LP; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + i * T::WAVES * 1024), 16, offp[i] | past, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < T::LQ; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(dst + T::BP * 128 + i * T::WAVES * 1024), 16, offq[i] | past, 0, 0, 0);
+        --left;
         if (++kk == ksteps) {
             kk = 0;
             ++ks;
@@ -119,12 +126,12 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     const int frow = lane & 15, fq4 = lane >> 4;
     const int sw0 = ((fq4 ^ (frow & 7)) * 16), sw1 = (((4 + fq4) ^ (frow & 7)) * 16);
     const int rdp = (wp * T::TP + frow) * 128, rdq = T::BP * 128 + (wq * T::TQ + frow) * 128;
-    auto read = [&](int stage, int h, i32x4 (&a)[T::FP], i32x4 (&b)[T::FQ]) {
-        const char* s = lds + stage * T::STAGE + (h ? sw1 : sw0);
-#pragma unroll
-        for (int i = 0; i < T::FP; ++i) a[i] = *(const i32x4*)(s + rdp + i * 2048);
+    auto read = [&](int stage, int sw, i32x4 (&a)[T::FP], i32x4 (&b)[T::FQ]) {
+        const char* s = lds + stage + sw;
 #pragma unroll
         for (int j = 0; j < T::FQ; ++j) b[j] = *(const i32x4*)(s + rdq + j * 2048);
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) a[i] = *(const i32x4*)(s + rdp + i * 2048);
     };
     auto multiply = [&](const i32x4 (&a)[T::FP], const i32x4 (&b)[T::FQ]) {
 #pragma unroll
@@ -132,8 +139,22 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
 #pragma unroll
             for (int j = 0; j < T::FQ; ++j) acc[i][j] = mm_mfma<T::KIND>(a[i], b[j], acc[i][j]);
     };
-    // every load of this wave has landed and every fragment read has returned, for all waves
-    auto meet = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // every load of this wave has landed and every fragment read has returned, for all waves; nothing is moved across
+    auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // half a step: fragment reads spread among the products (and, in the second half, the loads of the next stage)
+    auto weave = [](auto loads) {
+        constexpr int R = T::FP + T::FQ, M = T::FP * T::FQ, L = decltype(loads)::value, PER = M / R > 0 ? M / R : 1;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                       // a read
+            if (i < L) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);            // a load
+            __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);                     // products
+        }
+    };
 
 #pragma unroll
     for (int i = 0; i < T::FP; ++i)
@@ -144,20 +165,82 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     i32x4 a0[T::FP], b0[T::FQ], a1[T::FP], b1[T::FQ];
     fetch(0);
     meet();
-    if (n > 1) fetch(1);
-    read(0, 0, a0, b0);
+    fetch(T::STAGE);
+    read(0, sw0, a0, b0);
     int s = 0;
     for (int t = 0; t < n; ++t) {
-        read(s, 1, a1, b1);
+        read(s, sw1, a1, b1);
         multiply(a0, b0);
+        weave(std::integral_constant<int, 0>{});
         meet();                              // stage t + 1 is in LDS, stage t has been read by all
-        if (t + 2 < n) fetch(s);
-        s ^= 1;
-        if (t + 1 < n) read(s, 0, a0, b0);
+        fetch(s);
+        s ^= T::STAGE;
+        read(s, sw0, a0, b0);
         multiply(a1, b1);
+        weave(std::integral_constant<int, T::LP + T::LQ>{});
+        __builtin_amdgcn_sched_barrier(0);
     }
     meet();
 #endif
+}
+
+// ---- 16-bit results of a tile on their way to memory --------------------------------------------------------------------
+// The lanes hold four neighbouring p of a q; written directly, an instruction would touch 16 rows with 32 bytes each. The tile goes
+// through the LDS of its stages instead (all waves are past their last fragment read) and leaves in whole 16-byte pieces, 512
+// bytes of a row after another. Piece c of image row r sits at c ^ r, so neither side meets a bank twice.
+// bits(i, j) gives the four values of fragment (i, j) as two words.
+template <class T, class F>
+__device__ __forceinline__ void mm_stage(char* lds, F bits) {      // image [q][p]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int q = wq * T::TQ + j * 16 + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) {
+            const int c = (wp * T::TP + i * 16) / 8 + (lane >> 5);
+            *(uint2*)(lds + q * (T::BP * 2) + ((c ^ (q & (T::BP / 8 - 1))) * 16) + ((lane >> 4) & 1) * 8) = bits(i, j);
+        }
+    }
+}
+template <class T, class F>
+__device__ __forceinline__ void mm_stage_turned(char* lds, F bits) {   // image [p][q]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    const bool odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < T::FQ; ++j) {
+        const int q = wq * T::TQ + j * 16 + (lane & 14);
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) {
+            // neighbouring lanes hold neighbouring q: the even one takes both values of the first two p, the odd one of the last two
+            const uint2 v = bits(i, j);
+            const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? v.x : v.y), 0xB1, 0xF, 0xF, true);
+            const uint32_t lo = odd ? got : v.x, hi = odd ? v.y : got;
+            const int p = wp * T::TP + i * 16 + (lane >> 4) * 4 + (odd ? 2 : 0), c = q >> 3;
+            char* at = lds + p * (T::BQ * 2) + (q & 7) * 2;
+            *(uint32_t*)(at + ((c ^ (p & (T::BQ / 8 - 1))) * 16)) = (lo & 0xffffu) | (hi << 16);
+            *(uint32_t*)(at + T::BQ * 2 + ((c ^ ((p + 1) & (T::BQ / 8 - 1))) * 16)) = (lo >> 16) | (hi & 0xffff0000u);
+        }
+    }
+}
+// An image of ROWS x COLS to dst: rows and bytes beyond `rows` / `bytes` are left out; whole = dst rows start at multiples of 16.
+template <class T, int ROWS, int COLS>
+__device__ __forceinline__ void mm_unstage(const char* lds, char* dst, int64_t pitch, int64_t rows, int64_t bytes, bool whole) {
+    constexpr int C = COLS / 8;
+#pragma unroll
+    for (int k = 0; k < ROWS * C / T::THREADS; ++k) {
+        const int at = k * T::THREADS + threadIdx.x, r = at / C, c = at % C;
+        if (r >= rows || c * 16 >= bytes) continue;
+        const uint4 v = *(const uint4*)(lds + r * (COLS * 2) + ((c ^ (r & (C - 1))) * 16));
+        char* o = dst + r * pitch + c * 16;
+        if (whole && c * 16 + 16 <= bytes) {
+            *(uint4*)o = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c * 16 + e * 2 < bytes) *(uint16_t*)(o + e * 2) = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+    }
 }
 
 // Workgroup id -> tile (p, q): consecutive ids go round the 8 XCDs, so each XCD gets a contiguous stretch of the walk, and the

@@ -6,8 +6,7 @@
 //   G_ij = dL_i/dz_ij = T_i p_ij - pi_ij + c p_ij (log p_ij + H_i)
 //   dx = G W,  dW = G^T x,  db_j = sum_i G_ij
 //
-// Forward: one product whose tiles end in (max, sum of exp, sum of exp * (z - max), sum of pi z) per row, joined per row by a second
-// kernel. Backward: the classes in pieces; per piece the logits are made again, turned into G (16 bits, in both orientations), and
+// Forward: one product whose tiles end in a few sums per row (Part), joined per row by a second kernel. Backward: the classes in pieces; per piece the logits are made again, turned into G (16 bits, in both orientations), and
 // two products take it to dx and dW. Bound by the matrix instructions: 2 N V D forward, 6 N V D backward.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -24,12 +23,30 @@ int fail(int code, const std::string& msg);
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ------------------------------------------------------------------------------------------------ operands
 // Copies a [rows, cols] matrix (any row stride, any alignment) into rows of `pitch` bytes, zeros behind the last column; float32
 // is split into three planes. One thread writes 16 bytes per plane. Bound by memory; only operands that the tile loop cannot read
 // in place come here (float32, rows that do not start at multiples of 16 bytes).
+// Eight neighbours from element `at` on, `left` of them in the row (the others zero), as 16-bit planes. The 16 or 32 bytes may start
+// anywhere.
+template <int DT>
+__device__ __forceinline__ void load_planes(const void* src, int64_t at, int left, uint16_t (&h)[3][8]) {
+    if constexpr (DT == DT_F32) {
+        float v[8] = {};
+        if (left >= 8) __builtin_memcpy(v, (const float*)src + at, 32);
+        else
+            for (int e = 0; e < 8; ++e) v[e] = e < left ? ((const float*)src)[at + e] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split3(v[e], h[0][e], h[1][e], h[2][e]);
+    } else {
+        if (left >= 8) __builtin_memcpy(h[0], (const uint16_t*)src + at, 16);
+        else
+            for (int e = 0; e < 8; ++e) h[0][e] = e < left ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
+    }
+}
+
 struct PackJob {
     const void* src;
     int64_t src_pitch;    // elements
@@ -47,16 +64,7 @@ __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block) {
     const int64_t r = at / pieces;
     const int c0 = (int)(at - r * pieces) * 8;
     __align__(16) uint16_t h[3][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int c = c0 + e;
-        if constexpr (DT == DT_F32) {
-            const float v = c < j.cols ? ((const float*)j.src)[r * j.src_pitch + c] : 0.0f;
-            split3(v, h[0][e], h[1][e], h[2][e]);
-        } else {
-            h[0][e] = c < j.cols ? ((const uint16_t*)j.src)[r * j.src_pitch + c] : (uint16_t)0;
-        }
-    }
+    load_planes<DT>(j.src, r * j.src_pitch + c0, j.cols - c0, h);
 #pragma unroll
     for (int p = 0; p < (DT == DT_F32 ? 3 : 1); ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + c0 * 2) = *(const uint4*)h[p];
 }
@@ -81,15 +89,14 @@ __device__ __forceinline__ void turn_block(const TurnJob& j, int64_t block, uint
     const int across = (j.cols + 63) / 64;
     const int64_t r0 = block / across * 64;
     const int c0 = (int)(block % across) * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        const bool in = r0 + r < j.rows && c0 + c < j.cols && !(j.target && j.target[r0 + r] == j.ignore);
-        if constexpr (DT == DT_F32) {
-            const float v = in ? ((const float*)j.src)[(r0 + r) * j.src_pitch + c0 + c] : 0.0f;
-            split3(v, tile[0][r][c], tile[1][r][c], tile[2][r][c]);
-        } else {
-            tile[0][r][c] = in ? ((const uint16_t*)j.src)[(r0 + r) * j.src_pitch + c0 + c] : (uint16_t)0;
-        }
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int r = i >> 3, c = (i & 7) * 8;
+        __align__(16) uint16_t h[3][8];
+        load_planes<DT>(j.src, (r0 + r) * j.src_pitch + c0 + c, r0 + r < j.rows && !(j.target && j.target[r0 + r] == j.ignore) ? j.cols - c0 - c : 0, h);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) *(uint32_t*)&tile[p][r][c + e] = (uint32_t)h[p][e] | (uint32_t)h[p][e + 1] << 16;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
@@ -123,16 +130,38 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ shared arguments
-// Adds a part (max, sum e, sum e (z - max), sum pi z) to one whose maximum o[0] is already the largest of all.
-__device__ __forceinline__ void join_part(f32x4& o, const f32x4& v) {
-    if (v[0] == -INFINITY) {
-        o[1] += v[1];       // nothing, or the NaN of a logit that is none
+// A softmax is summed as 2^t, t = z log2(e) - reference. The reference of a part of a row is its largest z log2(e) rounded to a whole
+// number: then one fused multiply-add gives t with a single rounding, and references differ by whole numbers, so joining parts
+// multiplies by exact powers of two. Beyond |z| = 2^17 (masks of a type's lowest value, say) the products would overflow; there the
+// reference is the largest z itself. One float tells which: half of the whole number (below 2^17), or the z.
+struct Reference {
+    float off, whole;      // t = (z - off) * log2(e) - whole
+    __device__ __forceinline__ explicit Reference(float v) : off(fabsf(v) < 131072.0f ? 0.0f : v), whole(fabsf(v) < 131072.0f ? 2.0f * v : 0.0f) {}
+    __device__ __forceinline__ float t(float z) const { return __builtin_fmaf(z - off, LOG2E, -whole); }
+};
+__device__ __forceinline__ float reference_of(float top) { return fabsf(top) < 131072.0f ? 0.5f * rintf(top * LOG2E) : top; }
+// References in one order, and the difference a - b in units of t.
+__device__ __forceinline__ float reference_size(float v) { return fabsf(v) < 131072.0f ? v * (2.0f * LN2) : v; }
+__device__ __forceinline__ float reference_minus(float a, float b) {
+    return fabsf(a) < 131072.0f && fabsf(b) < 131072.0f ? 2.0f * (a - b) : (reference_size(a) - reference_size(b)) * LOG2E;
+}
+
+// Sums of a part of a row: its reference (-inf: no class that can be), sum 2^t, sum 2^t t, sum pi t, sum pi.
+struct Part {
+    float ref, l, s, dot, pi;
+};
+// Adds a part to one whose reference is already the largest of all.
+__device__ __forceinline__ void join_part(Part& o, const Part& v) {
+    if (v.ref == -INFINITY) {
+        o.l += v.l;       // nothing, or the NaN of a logit that is none
+        o.dot += v.dot;
     } else {
-        const float d = v[0] - o[0], e = __builtin_amdgcn_exp2f(d * LOG2E);
-        o[1] += v[1] * e;
-        o[2] += e == 0.0f ? 0.0f : (v[2] + v[1] * d) * e;
+        const float d = reference_minus(v.ref, o.ref), e = __builtin_amdgcn_exp2f(d);
+        o.l += v.l * e;
+        o.s += e == 0.0f ? 0.0f : (v.s + v.l * d) * e;
+        o.dot += v.pi == 0.0f ? v.dot : v.dot + v.pi * d;
     }
-    o[3] += v[3];
+    o.pi += v.pi;
 }
 
 struct Rows {               // what a row's target says
@@ -151,7 +180,7 @@ struct StatArgs {
     int32_t kbytes, segments;
     int32_t v0;             // first class of the piece that w starts at
     int32_t tile0, tiles;   // first tile of the piece, tiles of all classes
-    f32x4* part;            // [rows][tiles] (max, sum e, sum e (z - max), sum pi z)
+    f32x4* part;            // [rows][tiles] ref, l, s, dot
     float* tpart;           // dense: [rows][tiles][2] sum pi, sum |pi|
     float* zt;              // index: [rows] logit of the target
     int32_t tiles_p, tiles_q;
@@ -186,6 +215,15 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     add_bias<T, DT>(a.bias, p0, wp, lane, a.v0, a.t.classes, acc);
     const int left = a.t.classes - a.v0 - (int)p0 - wp * T::TP - (lane >> 4) * 4;   // classes from this lane's first one on
+    if (p0 + T::BP > a.t.classes - a.v0) {          // the last tile
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (i * 16 + r >= left)
+#pragma unroll
+                    for (int j = 0; j < T::FQ; ++j) acc[i][j][r] = -INFINITY;
+    }
     f32x4* const joint = (f32x4*)lds;                       // [WP][BQ]
     float* const jt = (float*)(lds + T::WP * T::BQ * 16);   // [WP][BQ][2]
 #pragma unroll
@@ -195,47 +233,38 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
 #pragma unroll
         for (int i = 0; i < T::FP; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (i * 16 + r >= left) acc[i][j][r] = -INFINITY;
-                top = fmaxf(top, acc[i][j][r]);
-            }
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float ref = reference_of(top);
+        const Reference at(top == -INFINITY ? 0.0f : ref);
         float l = 0.0f, s = 0.0f, dot = 0.0f, pi_sum = 0.0f, pi_abs = 0.0f;
+        if (!DENSE && n < a.t.rows) {
+            const int64_t hit = a.t.index[n] - (a.v0 + p0 + wp * T::TP + (lane >> 4) * 4);
+            if (hit >= 0 && hit < T::TP && hit < left) {
+#pragma unroll
+                for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (hit == i * 16 + r) a.zt[n] = acc[i][j][r];
+            }
+        }
+        const float* pi = DENSE && n < a.t.rows ? a.t.dense + n * a.t.dense_pitch + a.v0 + p0 + wp * T::TP + (lane >> 4) * 4 : nullptr;
 #pragma unroll
         for (int i = 0; i < T::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float d = acc[i][j][r] - base;
-                const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+                const float t = at.t(acc[i][j][r]);
+                const float e = __builtin_amdgcn_exp2f(t);
                 l += e;
-                if constexpr (ENT) s += e == 0.0f ? 0.0f : e * d;   // 0 * -inf of a class that cannot be
+                if constexpr (ENT) s += e == 0.0f ? 0.0f : e * t;   // 0 * -inf of a class that cannot be
+                if constexpr (DENSE) {
+                    const float v = pi && i * 16 + r < left ? pi[i * 16 + r] : 0.0f;
+                    pi_sum += v;
+                    pi_abs += fabsf(v);
+                    dot += v == 0.0f ? 0.0f : v * t;
+                }
             }
-        if constexpr (DENSE) {
-            if (n < a.t.rows) {
-                const float* pi = a.t.dense + n * a.t.dense_pitch + a.v0 + p0 + wp * T::TP + (lane >> 4) * 4;
-#pragma unroll
-                for (int i = 0; i < T::FP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (i * 16 + r < left) {
-                            const float v = pi[i * 16 + r];
-                            pi_sum += v;
-                            pi_abs += fabsf(v);
-                            dot += v == 0.0f ? 0.0f : v * acc[i][j][r];
-                        }
-            }
-        } else if (n < a.t.rows) {
-            const int64_t at = a.t.index[n] - (a.v0 + p0 + wp * T::TP + (lane >> 4) * 4);
-            if (at >= 0 && at < T::TP && at < left) {
-#pragma unroll
-                for (int i = 0; i < T::FP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (at == i * 16 + r) a.zt[n] = acc[i][j][r];
-            }
-        }
 #pragma unroll
         for (int o = 16; o < 64; o *= 2) {
             l += __shfl_xor(l, o);
@@ -248,7 +277,7 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
         }
         if (lane < 16) {
             const int q = wp * T::BQ + wq * T::TQ + j * 16 + lane;
-            joint[q] = f32x4{top, l, s, dot};
+            joint[q] = f32x4{ref, l, s, dot};
             if constexpr (DENSE) {
                 jt[2 * q] = pi_sum;
                 jt[2 * q + 1] = pi_abs;
@@ -258,27 +287,22 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
     __syncthreads();
     for (int q = threadIdx.x; q < T::BQ; q += T::THREADS) {
         if (q0 + q >= a.t.rows) break;
-        f32x4 v[T::WP];
-        float top = -INFINITY;
+        Part v[T::WP];
+        float ta = 0.0f;
+        Part o = {-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < T::WP; ++w) {
-            v[w] = joint[w * T::BQ + q];
-            top = fmaxf(top, v[w][0]);
+            const f32x4 u = joint[w * T::BQ + q];
+            v[w] = Part{u[0], u[1], u[2], u[3], DENSE ? jt[2 * (w * T::BQ + q)] : 0.0f};
+            if (DENSE) ta += jt[2 * (w * T::BQ + q) + 1];
+            if (reference_size(v[w].ref) > reference_size(o.ref)) o.ref = v[w].ref;
         }
-        f32x4 o = {top, 0.0f, 0.0f, 0.0f};
-        float ts = 0.0f, ta = 0.0f;
 #pragma unroll
-        for (int w = 0; w < T::WP; ++w) {
-            join_part(o, v[w]);
-            if constexpr (DENSE) {
-                ts += jt[2 * (w * T::BQ + q)];
-                ta += jt[2 * (w * T::BQ + q) + 1];
-            }
-        }
+        for (int w = 0; w < T::WP; ++w) join_part(o, v[w]);
         const int64_t at = (q0 + q) * a.tiles + a.tile0 + tp;
-        a.part[at] = o;
+        a.part[at] = f32x4{o.ref, o.l, o.s, o.dot};
         if constexpr (DENSE) {
-            a.tpart[2 * at] = ts;
+            a.tpart[2 * at] = o.pi;
             a.tpart[2 * at + 1] = ta;
         }
     }
@@ -290,52 +314,61 @@ struct JoinArgs {
     const float* tpart;
     const float* zt;
     int32_t tiles, reduction;
-    float *lse, *ent, *tsum, *scalars;       // kept for the backward pass
-    float *ce, *tabs;                        // per row
+    float *ref, *inv, *mean, *tsum, *scalars;   // kept for the backward pass: reference, 1 / l, s / l, sum pi
+    float *ce, *ent, *tabs;                     // per row
     float *loss, *out_ce, *out_ent;          // results, per row or one; the last two may be null
 };
 
-// One wave per row over the row's tiles.
-__device__ __forceinline__ void join_row(const JoinArgs& a, int64_t n) {
-    const int lane = threadIdx.x & 63;
-    const f32x4* part = a.part + n * a.tiles;
-    float top = -INFINITY;
-    for (int i = lane; i < a.tiles; i += 64) top = fmaxf(top, part[i][0]);
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
-    f32x4 v = {top, 0.0f, 0.0f, 0.0f};
-    float ts = 0.0f, ta = 0.0f;
-    for (int i = lane; i < a.tiles; i += 64) {
-        join_part(v, part[i]);
-        if (a.t.dense) {
-            ts += a.tpart[2 * (n * a.tiles + i)];
-            ta += a.tpart[2 * (n * a.tiles + i) + 1];
+__device__ __forceinline__ Part part_at(const JoinArgs& a, int64_t at) {
+    const f32x4 u = a.part[at];
+    return Part{u[0], u[1], u[2], u[3], a.t.dense ? a.tpart[2 * at] : 0.0f};
+}
+
+// LANES lanes per row, each over its share of the row's tiles.
+template <int LANES>
+__device__ __forceinline__ void join_row(const JoinArgs& a, int64_t n, int lane) {
+    const int64_t first = n * a.tiles;
+    Part v = {-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
+    float top = -INFINITY, ta = 0.0f;      // top: the largest reference's place in the order
+    auto larger = [&](float ref) {
+        if (reference_size(ref) > top) {
+            top = reference_size(ref);
+            v.ref = ref;
         }
+    };
+    for (int i = lane; i < a.tiles; i += LANES) larger(a.part[first + i][0]);
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) larger(__shfl_xor(v.ref, o));
+    for (int i = lane; i < a.tiles; i += LANES) {
+        join_part(v, part_at(a, first + i));
+        if (a.t.dense) ta += a.tpart[2 * (first + i) + 1];
     }
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        v[1] += __shfl_xor(v[1], o);
-        v[2] += __shfl_xor(v[2], o);
-        v[3] += __shfl_xor(v[3], o);
-        ts += __shfl_xor(ts, o);
+    for (int o = 1; o < LANES; o *= 2) {
+        v.l += __shfl_xor(v.l, o);
+        v.s += __shfl_xor(v.s, o);
+        v.dot += __shfl_xor(v.dot, o);
+        v.pi += __shfl_xor(v.pi, o);
         ta += __shfl_xor(ta, o);
     }
     if (lane) return;
-    // every logit of the row is -inf: no softmax exists
-    const float lse = top == -INFINITY ? NAN : top + logf(v[1]);
-    const float h = top == -INFINITY ? NAN : logf(v[1]) - v[2] / v[1];
+    const bool none = v.ref == -INFINITY;      // every logit of the row is -inf: no softmax exists
+    const float bits = none ? NAN : __builtin_amdgcn_logf(v.l), inv = 1.0f / v.l, mean = v.s * inv;   // log2 of the sum
+    const float h = none ? NAN : LN2 * (bits - mean);
     float ce;
     bool counts = true;
     if (a.t.dense) {
-        ce = ts * lse - v[3];
-        a.tsum[n] = ts;
+        ce = LN2 * (v.pi * bits - v.dot);
+        a.tsum[n] = v.pi;
         a.tabs[n] = ta;
     } else {
         const int64_t t = a.t.index[n];
         counts = t != a.t.ignore;
-        ce = t >= 0 && t < a.t.classes ? lse - a.zt[n] : NAN;   // a class that does not exist: a loss that nobody overlooks
+        ce = t >= 0 && t < a.t.classes ? LN2 * (bits - Reference(v.ref).t(a.zt[n])) : NAN;   // a class that does not exist: nobody overlooks it
     }
-    a.lse[n] = lse;
+    a.ref[n] = v.ref;
+    a.inv[n] = inv;
+    a.mean[n] = mean;
     a.ent[n] = h;
     a.ce[n] = ce;
     if (a.reduction == AZ_REDUCE_NONE) {
@@ -392,14 +425,20 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
     if (a.out_ent) a.out_ent[0] = (float)(h / d);
 }
 
+// A wave per row where a row has many tiles, four lanes where it has few.
 __global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n < a.t.rows) join_row(a, n);
+    if (a.tiles > 32) {
+        const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+        if (n < a.t.rows) join_row<64>(a, n, threadIdx.x & 63);
+    } else {
+        const int64_t n = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2);
+        if (n < a.t.rows) join_row<4>(a, n, threadIdx.x & 3);
+    }
 }
 __global__ __launch_bounds__(1024) void k_ce_reduce(JoinArgs a) { reduce_rows(a); }
-// Few rows: both in one launch.
+// Few rows with few tiles: both in one launch.
 __global__ __launch_bounds__(1024) void k_ce_join_reduce(JoinArgs a) {
-    for (int n = threadIdx.x >> 6; n < a.t.rows; n += 16) join_row(a, n);
+    for (int64_t n = threadIdx.x >> 2; n < a.t.rows; n += 256) join_row<4>(a, n, threadIdx.x & 3);
     __threadfence_block();
     __syncthreads();
     reduce_rows(a);
@@ -451,7 +490,7 @@ struct GradArgs {
     const void* bias;
     int32_t kbytes, segments, v0;
     int32_t tiles_p, tiles_q;
-    const float *lse, *ent, *tsum;
+    const float *ref, *inv, *mean, *tsum;
     Factor f;
     char* g;               // [rows][g_pitch] per plane, or null (no dx wanted)
     int64_t g_pitch, g_plane;
@@ -482,33 +521,52 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
         const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
         const bool row = n < a.t.rows;
         int64_t target = 0;
-        float lse = 0.0f, h = 0.0f, total = 1.0f, f = hold;
+        float ref = 0.0f, inv = 0.0f, mean = 0.0f, total = 1.0f, f = hold;
         bool counts = false;
         share[j] = 1.0f;
         if (row) {
-            lse = a.lse[n];
-            if constexpr (ENT) h = a.ent[n];
+            ref = a.ref[n];
+            inv = a.inv[n];
+            if constexpr (ENT) mean = a.mean[n];
             if constexpr (DENSE) total = a.tsum[n];
             else target = a.t.index[n];
             counts = DENSE || target != a.t.ignore;
             if (a.f.largest) share[j] = *a.f.largest > 0.0f || *a.f.largest != *a.f.largest ? a.f.grad[n] / *a.f.largest : 0.0f;
             if (!DENSE && (target < 0 || target >= a.t.classes)) f = NAN;
         }
-        const int64_t at = target - a.v0 - ml;
+        const Reference at(ref);
         const float* pi = DENSE && row ? a.t.dense + n * a.t.dense_pitch + a.v0 + ml : nullptr;
+        const float scale = (DENSE ? total * inv : inv) * f, c = a.t.entropy * LN2 * inv * f;
 #pragma unroll
         for (int i = 0; i < T::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float lp = acc[i][j][r] - lse;
-                const float p = __builtin_amdgcn_exp2f(lp * LOG2E);
-                float g = p;
-                const bool in = i * 16 + r < left;
-                if constexpr (DENSE) g = total * p - (in && row ? pi[i * 16 + r] : 0.0f);
-                else g = at == i * 16 + r ? p - 1.0f : p;
-                if constexpr (ENT) g += p == 0.0f ? 0.0f : a.t.entropy * p * (lp + h);
-                acc[i][j][r] = in && counts ? g * f : 0.0f;
+                const float t = at.t(acc[i][j][r]);
+                const float e = __builtin_amdgcn_exp2f(t);
+                float g = e * scale;
+                if constexpr (DENSE) g -= pi && i * 16 + r < left ? pi[i * 16 + r] * f : 0.0f;
+                if constexpr (ENT) g += e == 0.0f ? 0.0f : c * e * (t - mean);
+                acc[i][j][r] = counts ? g : 0.0f;
             }
+        if constexpr (!DENSE) {
+            const int64_t hit = target - a.v0 - ml;
+            if (counts && hit >= 0 && hit < T::TP) {
+#pragma unroll
+                for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (hit == i * 16 + r) acc[i][j][r] -= f;
+            }
+        }
+    }
+    if (p0 + T::BP > a.t.classes - a.v0) {          // classes behind the last one
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (i * 16 + r >= left)
+#pragma unroll
+                    for (int j = 0; j < T::FQ; ++j) acc[i][j][r] = 0.0f;
     }
     if (a.db) {
         float* const joint = (float*)lds;      // [WQ][BP]
@@ -530,32 +588,32 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
             for (int w = 0; w < T::WQ; ++w) s += joint[w * T::BP + p];
             if (p0 + p < a.db_pitch) a.db[tq * a.db_pitch + p0 + p] = s;
         }
+        __syncthreads();
     }
+    auto bits = [&](int i, int j, int plane, float by) {
+        const f32x4 v = acc[i][j] * by;
+        if constexpr (DT == DT_F32) {
+            uint16_t o[4][3];
 #pragma unroll
-    for (int j = 0; j < T::FQ; ++j) {
-        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+            for (int r = 0; r < 4; ++r) split3(v[r], o[r][0], o[r][1], o[r][2]);
+            return make_uint2((uint32_t)o[0][plane] | (uint32_t)o[1][plane] << 16, (uint32_t)o[2][plane] | (uint32_t)o[3][plane] << 16);
+        } else {
+            return pack4<DT>(v[0], v[1], v[2], v[3]);
+        }
+    };
 #pragma unroll
-        for (int i = 0; i < T::FP; ++i) {
-            const int64_t m = ml + i * 16;
-            uint16_t o[NP][4];
-            auto round = [&](float by) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (DT == DT_F32) split3(acc[i][j][r] * by, o[0][r], o[1][r], o[2][r]);
-                    else o[0][r] = to_bits<DT>(acc[i][j][r] * by);
-                }
-            };
-            round(1.0f);
-            if (a.g && n < a.t.rows && m * 2 < a.g_pitch)
-#pragma unroll
-                for (int p = 0; p < NP; ++p) *(uint2*)(a.g + p * a.g_plane + n * a.g_pitch + m * 2) = *(const uint2*)o[p];
-            if (a.f.largest) round(share[j]);
-            if (a.gt && n * 2 < a.gt_pitch)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (i * 16 + r < left) *(uint16_t*)(a.gt + p * a.gt_plane + (m + r) * a.gt_pitch + n * 2) = o[p][r];
+    for (int p = 0; p < NP; ++p) {
+        if (a.g) {
+            mm_stage<T>(lds, [&](int i, int j) { return bits(i, j, p, 1.0f); });
+            __syncthreads();
+            mm_unstage<T, T::BQ, T::BP>(lds, a.g + p * a.g_plane + q0 * a.g_pitch + p0 * 2, a.g_pitch, a.t.rows - q0, a.g_pitch - p0 * 2, true);
+            __syncthreads();
+        }
+        if (a.gt) {
+            mm_stage_turned<T>(lds, [&](int i, int j) { return bits(i, j, p, share[j]); });
+            __syncthreads();
+            mm_unstage<T, T::BP, T::BQ>(lds, a.gt + p * a.gt_plane + p0 * a.gt_pitch + q0 * 2, a.gt_pitch, a.w.rows - p0, a.gt_pitch - q0 * 2, true);
+            __syncthreads();
         }
     }
 }
@@ -583,28 +641,46 @@ __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
 #pragma unroll
     for (int j = 0; j < T::FQ; ++j) {
         const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
-        if (n >= a.q.rows) continue;
-        const float post = a.by_row ? factor_row(a.f, n) : all;
+        const bool row = n < a.q.rows;
+        const float post = !row ? 0.0f : a.by_row ? factor_row(a.f, n) : all;
 #pragma unroll
         for (int i = 0; i < T::FP; ++i) {
             const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
             const int64_t at = n * width + m;
-            f32x4 v = acc[i][j];
-            if ((width & 3) == 0 && m + 4 <= width) {
-                if (!a.first) v += *(const f32x4*)(a.sum + at);
-                if (!a.last) *(f32x4*)(a.sum + at) = v;
-                else store4<DT>(a.out, at, v[0] * post, v[1] * post, v[2] * post, v[3] * post);
-            } else {
+            if (row && (width & 3) == 0) {
+                if (m < width) {
+                    if (!a.first) acc[i][j] += *(const f32x4*)(a.sum + at);
+                    if (!a.last) *(f32x4*)(a.sum + at) = acc[i][j];
+                }
+            } else if (row) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (m + r < width) {
-                        float u = v[r];
-                        if (!a.first) u += a.sum[at + r];
-                        if (!a.last) a.sum[at + r] = u;
-                        else store_scalar<DT>(a.out, at + r, u * post);
+                        if (!a.first) acc[i][j][r] += a.sum[at + r];
+                        if (!a.last) a.sum[at + r] = acc[i][j][r];
                     }
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] *= post;
+            if constexpr (DT == DT_F32) {       // 16 bytes per lane already
+                if (a.last && row) {
+                    float* o = (float*)a.out + at;
+                    if ((width & 3) == 0) {
+                        if (m < width) *(f32x4*)o = acc[i][j];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (m + r < width) o[r] = acc[i][j][r];
+                    }
+                }
+            }
         }
+    }
+    if constexpr (DT != DT_F32) {
+        if (!a.last) return;
+        mm_stage<T>(lds, [&](int i, int j) { return pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]); });
+        __syncthreads();
+        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.out + (q0 * width + p0) * 2, width * 2, a.q.rows - q0, (width - p0) * 2, (width & 7) == 0);
     }
 }
 
@@ -694,7 +770,7 @@ Layout forward_layout(const az_linear_ce_args& a) {
         l.wp = l.take(l.piece * l.kpitch * l.planes);
     }
     l.part = l.take(a.rows * tiles * 16);
-    l.ce = l.take(a.rows * 4);
+    l.ce = l.take(a.rows * 8);       // cross entropy, entropy
     if (a.target_dense) {
         l.tpart = l.take(a.rows * tiles * 8);
         l.tabs = l.take(a.rows * 4);
@@ -795,8 +871,8 @@ template <int DT> struct Tiles { typedef BigB Big; typedef MidB Mid; typedef Sma
 template <> struct Tiles<DT_F16> { typedef BigH Big; typedef MidH Mid; typedef SmallH Small; };
 
 struct Kept {      // what the forward pass leaves for the backward one
-    float *lse, *ent, *tsum, *scalars;
-    Kept(float* p, int64_t rows) : lse(p), ent(p + rows), tsum(p + 2 * rows), scalars(p + 3 * rows) {}
+    float *ref, *inv, *mean, *tsum, *scalars;
+    Kept(float* p, int64_t rows) : ref(p), inv(p + rows), mean(p + 2 * rows), tsum(p + 3 * rows), scalars(p + 4 * rows) {}
 };
 
 template <int DT>
@@ -837,12 +913,13 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
         if (const int rc = launched("k_ce_stats")) return rc;
     }
     const Kept k(kept, a.rows);
-    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.lse, k.ent, k.tsum, k.scalars, (float*)(ws + l.ce),
+    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
                      a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent};
-    if (a.rows <= 512 && s.tiles <= 64) {
+    if (a.rows <= 512 && s.tiles <= 32) {
         hipLaunchKernelGGL(k_ce_join_reduce, dim3(1), dim3(1024), 0, st, j);
     } else {
-        hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, j);
+        const int per = s.tiles > 32 ? 4 : 64;
+        hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((a.rows + per - 1) / per)), dim3(256), 0, st, j);
         hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, j);
     }
     return launched("k_ce_join");
@@ -861,8 +938,9 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     s.bias = a.bias;
     s.segments = l.split ? 6 : 1;
     s.kbytes = (int)(l.pack ? l.kpitch : a.features * 2);
-    s.lse = kept.lse;
-    s.ent = kept.ent;
+    s.ref = kept.ref;
+    s.inv = kept.inv;
+    s.mean = kept.mean;
     s.tsum = kept.tsum;
     s.f = f;
     s.g = gx ? ws + l.g : nullptr;

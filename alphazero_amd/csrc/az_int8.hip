@@ -178,11 +178,51 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
             for (int j = 0; j < T::FQ; ++j) o[(i * T::FQ + j) * T::THREADS] = acc[i][j];
         return;
     }
+    float sx[T::FQ];
 #pragma unroll
-    for (int j = 0; j < T::FQ; ++j)
+    for (int j = 0; j < T::FQ; ++j) {
+        const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+        sx[j] = a.s.x[n < a.s.tokens ? n : a.s.tokens - 1];
+    }
+    f32x4 v[T::FP][T::FQ];
 #pragma unroll
-        for (int i = 0; i < T::FP; ++i)
-            finish4<DT>(a.s, q0 + wq * T::TQ + j * 16 + (lane & 15), p0 + wp * T::TP + i * 16 + (lane >> 4) * 4, acc[i][j]);
+    for (int i = 0; i < T::FP; ++i) {
+        float w[4], b[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4 + r, c = m < a.s.channels ? m : a.s.channels - 1;
+            w[r] = a.s.w[c];
+            b[r] = bias_at(a.s, c);
+        }
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[i][j][r] = (float)acc[i][j][r] * sx[j] * w[r] + b[r];
+    }
+    if constexpr (DT == DT_F32) {       // 16 bytes per lane already
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) {
+            const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+            if (n >= a.s.tokens) continue;
+#pragma unroll
+            for (int i = 0; i < T::FP; ++i) {
+                const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
+                float* o = (float*)a.s.y + n * a.s.channels + m;
+                if ((a.s.channels & 3) == 0) {
+                    if (m < a.s.channels) *(f32x4*)o = v[i][j];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < a.s.channels) o[r] = v[i][j][r];
+                }
+            }
+        }
+    } else {
+        mm_stage<T>(lds, [&](int i, int j) { return pack4<DT>(v[i][j][0], v[i][j][1], v[i][j][2], v[i][j][3]); });
+        __syncthreads();
+        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.s.y + (q0 * a.s.channels + p0) * 2, (int64_t)a.s.channels * 2, a.s.tokens - q0, (a.s.channels - p0) * 2,
+                                    (a.s.channels & 7) == 0);
+    }
 }
 
 // Joins the pieces of k: thread t of block (tile, fragment) adds what thread t of each piece's workgroup left.

@@ -20,6 +20,9 @@ template <int DT> __device__ __forceinline__ float from_bits(uint16_t b) {
     if constexpr (DT == DT_BF16) return bf16_value(b);
     else return (float)__builtin_bit_cast(_Float16, b);
 }
+template <int DT> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    return make_uint2((uint32_t)to_bits<DT>(a) | (uint32_t)to_bits<DT>(b) << 16, (uint32_t)to_bits<DT>(c) | (uint32_t)to_bits<DT>(d) << 16);
+}
 template <int DT> __device__ __forceinline__ float load_scalar(const void* p, int64_t i) {
     if constexpr (DT == DT_F32) return ((const float*)p)[i];
     else return from_bits<DT>(((const uint16_t*)p)[i]);

@@ -76,7 +76,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         rows, dev = x.shape[0], x.device
         shape = (rows,) if reduction == "none" else ()
         out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
-        kept = torch.empty(3 * rows + 2, dtype=torch.float32, device=dev)
+        kept = torch.empty(4 * rows + 2, dtype=torch.float32, device=dev)
         L = N.lib()
         with _device(dev):
             ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 0), "az_linear_ce_workspace"), dev)

@@ -162,10 +162,8 @@ def test_classes_that_cannot_be(dtype, dense):
     loss = _run(x * 0, w, b, t, reduction="none")[1]
     live = slice(None) if dense else t != -100
     total = t.sum(1) if dense else 1.0
-    # logits of 1e38 have steps of 1e31: only finiteness and, with equal logits, log(classes) up to that step can be asked for
-    assert torch.isfinite(loss[live]).all()
-    if dtype == F16:                                     # 65504 has steps of 2^-8 in float32
-        assert ((loss - total * math.log(200)).abs()[live] <= 2.0 ** -7 * 200 * 2.0 ** -8 + 0.05).all()
+    # equal logits, whatever they are: log(classes) from a sum of ones, to the rounding of a logarithm and two products
+    assert ((loss - total * math.log(200)).abs()[live] <= 8 * 2.0 ** -23 * 6).all()
 
 
 def test_row_without_a_softmax():
