@@ -3,7 +3,7 @@
 //
 // A workgroup owns BP x BQ results and walks k in steps of 128 bytes (64 16-bit or 128 8-bit values). A step's BP + BQ rows of
 // 128 bytes go from global memory to LDS without passing through registers (buffer_load_dwordx4 ... lds, 1 KB = 8 rows per wave
-// and instruction), two stages in LDS. The load writes a wave's 64 x 16 bytes contiguously, so the bank permutation is made on
+// and instruction), STAGES stages in LDS of which all but the one in use are on their way. The load writes a wave's 64 x 16 bytes contiguously, so the bank permutation is made on
 // the global side: the lane that writes 16-byte piece c of row r fetches piece c ^ (r & 7), and a fragment read (16 rows, one
 // piece each) then touches all banks evenly. Reads behind the last row or the last k of a matrix are turned into zeros by the
 // buffer descriptor's range check, so ragged sizes need no other code.
@@ -12,18 +12,20 @@
 // 16 x 16 tile, i.e. four neighbouring p of one q. Callers put the axis that is contiguous in their output (classes, features)
 // on P, and a softmax over P is mostly inside a lane.
 //
-// float32 operands come as three 16-bit planes (az_split3): h + m + l with 8 significant bits each. Six of the nine products of
-// planes are summed (the other three are below 2^-25 of the result), smallest first, by walking k six times with other plane
-// pairs: 2.5 PFLOP/s / 6 against the 0.16 PFLOP/s of the float32 matrix instructions.
+// float32 operands come as two float16 planes, v = h + m / 2048 (split2), scaled by powers of two beforehand. k is walked three times,
+// first with the plane pairs (h, m) and (m, h), whose sum is then divided by 2048, then with (h, h); (m, m) / 2^22 is below
+// 2^-24 of the result and left out. Each product keeps 22 bits or more, the sum is float32's: 2.5 PFLOP/s / 3 against the 0.16
+// PFLOP/s of the float32 matrix instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <type_traits>
 
+#include "az_types.cuh"
+
 namespace az {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -48,27 +50,28 @@ __device__ __forceinline__ typename MmAcc<KIND>::type mm_mfma(i32x4 a, i32x4 b, 
     else return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-template <int BP_, int BQ_, int WP_, int WQ_, int KIND_>
+template <int BP_, int BQ_, int WP_, int WQ_, int STAGES_, int KIND_>
 struct MmTile {
-    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, KIND = KIND_;
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STAGES = STAGES_, KIND = KIND_;
     static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
     static constexpr int TP = BP / WP, TQ = BQ / WQ;          // a wave's share
     static constexpr int FP = TP / 16, FQ = TQ / 16;
     static constexpr int LP = BP / 8 / WAVES, LQ = BQ / 8 / WAVES;   // 1 KB loads of a wave per stage
     static constexpr int STAGE = (BP + BQ) * 128;
-    static constexpr int LDS = 2 * STAGE;
-    static_assert((STAGE & (STAGE - 1)) == 0, "stages are told apart by one bit");
+    static constexpr int LDS = STAGES * STAGE;
+    static_assert(LDS <= 160 * 1024 && BP * BQ * 2 <= LDS && (STAGES - 1) * (LP + LQ) < 64, "LDS, the results' image in it, the counter of loads");
     static_assert(BP % (8 * WAVES) == 0 && BQ % (8 * WAVES) == 0 && TP % 16 == 0 && TQ % 16 == 0, "tile shape");
     typedef typename MmAcc<KIND>::type acc_t;
 };
 
-// Planes of step s of 6 (P, Q), smallest product first: (l,h) (h,l) (m,m) (m,h) (h,m) (h,h).
-__device__ __forceinline__ int mm_plane_p(int s) { return (0x001102 >> (4 * s)) & 3; }
-__device__ __forceinline__ int mm_plane_q(int s) { return (0x010120 >> (4 * s)) & 3; }
+// Planes of segment s of 3: (h, m) (m, h) (h, h).
+constexpr int MM_SEGMENTS = 3;
+__device__ __forceinline__ int mm_plane_p(int s) { return s == 1; }
+__device__ __forceinline__ int mm_plane_q(int s) { return s == 0; }
 
 // One tile: acc[i][j] = results p = p0 + wp * TP + 16 i + 4 (lane >> 4) + 0..3, q = q0 + wq * TQ + 16 j + (lane & 15), where
 // wave = wp * WQ + wq. kbytes: bytes of k per row (a multiple of 16). k_first / k_last: the 128-byte steps [k_first, k_last) of
-// the walk over `segments` times ceil(kbytes / 128) steps that this workgroup takes. All lanes of the workgroup call it; on
+// the walk of ceil(kbytes / 128) steps (three times that many for float32, `split`) that this workgroup takes. All lanes of the workgroup call it; on
 // return every wave has read its last fragment and passed a barrier, so the LDS may be used for something else.
 template <class T>
 __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, int64_t p0, int64_t q0, int kbytes, int k_first, int k_last,
@@ -139,10 +142,11 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
 #pragma unroll
             for (int j = 0; j < T::FQ; ++j) acc[i][j] = mm_mfma<T::KIND>(a[i], b[j], acc[i][j]);
     };
-    // every load of this wave has landed and every fragment read has returned, for all waves; nothing is moved across
-    auto meet = [] {
+    // all but the last `flying` stages' loads of this wave have landed and every fragment read has returned, for all waves; nothing is
+    // moved across
+    auto meet = [](auto flying) {
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(flying)::value * (T::LP + T::LQ)) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
     // half a step: fragment reads spread among the products (and, in the second half, the loads of the next stage)
@@ -163,24 +167,36 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     const int n = k_last - k_first;
     if (n <= 0) return;
     i32x4 a0[T::FP], b0[T::FQ], a1[T::FP], b1[T::FQ];
-    fetch(0);
-    meet();
-    fetch(T::STAGE);
+#pragma unroll
+    for (int i = 0; i < T::STAGES; ++i) fetch(i * T::STAGE);
+    meet(std::integral_constant<int, T::STAGES - 1>{});
     read(0, sw0, a0, b0);
     int s = 0;
+    const int turn = split ? 2 * ksteps - k_first : -1;      // the step that the (h, h) segment starts with
+    auto lower = [&] {
+        if constexpr (T::KIND == MM_F16)
+#pragma unroll
+            for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                for (int j = 0; j < T::FQ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] *= 1.0f / 2048.0f;
+    };
     for (int t = 0; t < n; ++t) {
+        if (t == turn) lower();
         read(s, sw1, a1, b1);
         multiply(a0, b0);
         weave(std::integral_constant<int, 0>{});
-        meet();                              // stage t + 1 is in LDS, stage t has been read by all
+        meet(std::integral_constant<int, T::STAGES - 2>{});     // stage t + 1 is in LDS, stage t has been read by all
         fetch(s);
-        s ^= T::STAGE;
+        s = s == (T::STAGES - 1) * T::STAGE ? 0 : s + T::STAGE;
         read(s, sw0, a0, b0);
         multiply(a1, b1);
         weave(std::integral_constant<int, T::LP + T::LQ>{});
         __builtin_amdgcn_sched_barrier(0);
     }
-    meet();
+    meet(std::integral_constant<int, 0>{});
+    if (split && turn >= n) lower();      // a piece of the walk that ends before it
 #endif
 }
 
@@ -241,6 +257,22 @@ __device__ __forceinline__ void mm_unstage(const char* lds, char* dst, int64_t p
                 if (c * 16 + e * 2 < bytes) *(uint16_t*)(o + e * 2) = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
         }
     }
+}
+
+// The lane, as a value that the compiler knows nothing of: what is computed from it stays behind the tile loop, instead of taking
+// registers through it.
+__device__ __forceinline__ int mm_lane_after() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+template <class T>
+__device__ __forceinline__ void mm_opaque(typename T::acc_t (&acc)[T::FP][T::FQ]) {
+#pragma unroll
+    for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) asm volatile("" : "+v"(acc[i][j]));
 }
 
 // Workgroup id -> tile (p, q): consecutive ids go round the 8 XCDs, so each XCD gets a contiguous stretch of the walk, and the

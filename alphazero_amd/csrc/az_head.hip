@@ -26,73 +26,110 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ------------------------------------------------------------------------------------------------ operands
-// Copies a [rows, cols] matrix (any row stride, any alignment) into rows of `pitch` bytes, zeros behind the last column; float32
-// is split into three planes. One thread writes 16 bytes per plane. Bound by memory; only operands that the tile loop cannot read
-// in place come here (float32, rows that do not start at multiples of 16 bytes).
-// Eight neighbours from element `at` on, `left` of them in the row (the others zero), as 16-bit planes. The 16 or 32 bytes may start
-// anywhere.
-template <int DT>
-__device__ __forceinline__ void load_planes(const void* src, int64_t at, int left, uint16_t (&h)[3][8]) {
-    if constexpr (DT == DT_F32) {
-        float v[8] = {};
-        if (left >= 8) __builtin_memcpy(v, (const float*)src + at, 32);
-        else
-            for (int e = 0; e < 8; ++e) v[e] = e < left ? ((const float*)src)[at + e] : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split3(v[e], h[0][e], h[1][e], h[2][e]);
-    } else {
-        if (left >= 8) __builtin_memcpy(h[0], (const uint16_t*)src + at, 16);
-        else
-            for (int e = 0; e < 8; ++e) h[0][e] = e < left ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
-    }
-}
+__device__ __forceinline__ float larger(float top, float v) { return v > top || v != v ? v : top; }      // a NaN stays
 
+// Copies a [rows, cols] matrix (any row stride, any alignment) into rows of `pitch` bytes, zeros behind the last column. float32 is
+// scaled by a power of two and split into two planes: in the forward pass each row by its own (its reciprocal goes to `own`), in the
+// backward pass all rows by the one of the largest (`all`), since there a sum also runs over the rows. Rows that do not count become
+// zeros. Bound by memory; only operands that the tile loop cannot read in place come here (float32, rows that do not start at
+// multiples of 16 bytes).
 struct PackJob {
     const void* src;
     int64_t src_pitch;    // elements
     int32_t rows, cols;
     char* dst;
     int64_t pitch, plane;   // bytes
-    __host__ __device__ int64_t blocks() const { return (rows * (pitch >> 4) + 255) / 256; }
+    float* own;
+    const float* all;
+    const int64_t* target;  // null: every row counts
+    int64_t ignore;
+    __host__ __device__ int64_t blocks() const { return own ? (rows + 3) / 4 : (rows * (pitch >> 4) + 255) / 256; }
+    __device__ __forceinline__ bool counts(int64_t r) const { return !(target && target[r] == ignore); }
 };
+
+// Eight neighbours from element `at` on, `left` of them in the row (the others zero). They may start anywhere.
+__device__ __forceinline__ void load8(const float* src, int64_t at, int left, float (&v)[8]) {
+    if (left >= 8) __builtin_memcpy(v, src + at, 32);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? src[at + e] : 0.0f;
+}
+// The same as 16-bit planes; float32 times `scale`.
+template <int DT>
+__device__ __forceinline__ void load_planes(const void* src, int64_t at, int left, float scale, uint16_t (&h)[2][8]) {
+    if constexpr (DT == DT_F32) {
+        float v[8];
+        load8((const float*)src, at, left, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split2(v[e] * scale, h[0][e], h[1][e]);
+    } else {
+        if (left >= 8) __builtin_memcpy(h[0], (const uint16_t*)src + at, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[0][e] = e < left ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
+    }
+}
 
 template <int DT>
 __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block) {
+    constexpr int NP = DT == DT_F32 ? 2 : 1;
     const int pieces = (int)(j.pitch >> 4);
-    const int64_t at = block * 256 + threadIdx.x;
-    if (at >= (int64_t)j.rows * pieces) return;
-    const int64_t r = at / pieces;
-    const int c0 = (int)(at - r * pieces) * 8;
-    __align__(16) uint16_t h[3][8];
-    load_planes<DT>(j.src, r * j.src_pitch + c0, j.cols - c0, h);
+    __align__(16) uint16_t h[2][8];
+    auto put = [&](int64_t r, int piece, float scale) {
+        load_planes<DT>(j.src, r * j.src_pitch + piece * 8, j.counts(r) ? j.cols - piece * 8 : 0, scale, h);
 #pragma unroll
-    for (int p = 0; p < (DT == DT_F32 ? 3 : 1); ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + c0 * 2) = *(const uint4*)h[p];
+        for (int p = 0; p < NP; ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + piece * 16) = *(const uint4*)h[p];
+    };
+    if (DT == DT_F32 && j.own) {       // a wave per row
+        const int64_t r = block * 4 + (threadIdx.x >> 6);
+        const int lane = threadIdx.x & 63;
+        if (r >= j.rows) return;
+        float top = 0.0f;
+        if (j.counts(r))
+            for (int i = lane; i < pieces; i += 64) {
+                float v[8];
+                load8((const float*)j.src, r * j.src_pitch + i * 8, j.cols - i * 8, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = larger(top, fabsf(v[e]));
+            }
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) top = larger(top, __shfl_xor(top, o));
+        const float un = unscale_of(top);
+        if (lane == 0) j.own[r] = un;
+        for (int i = lane; i < pieces; i += 64) put(r, i, 1.0f / un);
+    } else {
+        const int64_t at = block * 256 + threadIdx.x;
+        if (at < (int64_t)j.rows * pieces) put(at / pieces, (int)(at % pieces), DT == DT_F32 ? 1.0f / *j.all : 1.0f);
+    }
 }
 
 // The same, transposed: dst row c = column c of the source, rows behind the last one (up to the pitch, a multiple of 128 bytes) zero;
-// rows that do not count (target equal to ignore) become zeros too, so that whatever a padded row holds - NaN included - stays out of
-// dW. 64 x 64 elements per workgroup through LDS.
+// rows that do not count become zeros, so that whatever a padded row holds - NaN included - stays out of dW. 64 x 64 elements per
+// workgroup through LDS.
 struct TurnJob {
     const void* src;
     int64_t src_pitch;
     int32_t rows, cols;
     char* dst;
     int64_t pitch, plane;
-    const int64_t* target;   // null: every row counts
+    const float* all;
+    const int64_t* target;
     int64_t ignore;
     __host__ __device__ int64_t blocks() const { return (int64_t)((cols + 63) / 64) * (pitch / 128); }
 };
 
 template <int DT>
 __device__ __forceinline__ void turn_block(const TurnJob& j, int64_t block, uint16_t (*tile)[64][66]) {
-    constexpr int NP = DT == DT_F32 ? 3 : 1;
+    constexpr int NP = DT == DT_F32 ? 2 : 1;
     const int across = (j.cols + 63) / 64;
     const int64_t r0 = block / across * 64;
     const int c0 = (int)(block % across) * 64;
+    const float scale = DT == DT_F32 ? 1.0f / *j.all : 1.0f;
+    __align__(16) uint16_t h[2][8];
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
         const int r = i >> 3, c = (i & 7) * 8;
-        __align__(16) uint16_t h[3][8];
-        load_planes<DT>(j.src, (r0 + r) * j.src_pitch + c0 + c, r0 + r < j.rows && !(j.target && j.target[r0 + r] == j.ignore) ? j.cols - c0 - c : 0, h);
+        const bool in = r0 + r < j.rows && !(j.target && j.target[r0 + r] == j.ignore);
+        load_planes<DT>(j.src, (r0 + r) * j.src_pitch + c0 + c, in ? j.cols - c0 - c : 0, scale, h);
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
@@ -104,10 +141,9 @@ __device__ __forceinline__ void turn_block(const TurnJob& j, int64_t block, uint
         if (c0 + c >= j.cols) continue;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            __align__(16) uint16_t h[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = tile[p][piece * 8 + e][c];
-            *(uint4*)(j.dst + p * j.plane + (int64_t)(c0 + c) * j.pitch + (r0 + piece * 8) * 2) = *(const uint4*)h;
+            for (int e = 0; e < 8; ++e) h[0][e] = tile[p][piece * 8 + e][c];
+            *(uint4*)(j.dst + p * j.plane + (int64_t)(c0 + c) * j.pitch + (r0 + piece * 8) * 2) = *(const uint4*)h[0];
         }
     }
 }
@@ -121,7 +157,7 @@ struct PackArgs {
 
 template <int DT>
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-    __shared__ __align__(16) uint16_t tile[DT == DT_F32 ? 3 : 1][64][66];
+    __shared__ __align__(16) uint16_t tile[DT == DT_F32 ? 2 : 1][64][66];
     const int64_t id = blockIdx.x;
     if (id < a.end_w) pack_block<DT>(a.w, id);
     else if (id < a.end_x) pack_block<DT>(a.x, id - a.end_w);
@@ -177,7 +213,9 @@ struct StatArgs {
     MmOperand w, x;
     Rows t;
     const void* bias;
-    int32_t kbytes, segments;
+    int32_t kbytes;
+    const float *un_w, *un_x;   // float32: what the operands were divided by, per class of the piece and per row (un_step 1) or for all (0)
+    int32_t un_step;
     int32_t v0;             // first class of the piece that w starts at
     int32_t tile0, tiles;   // first tile of the piece, tiles of all classes
     f32x4* part;            // [rows][tiles] ref, l, s, dot
@@ -186,20 +224,45 @@ struct StatArgs {
     int32_t tiles_p, tiles_q;
 };
 
-template <class T, int DT>
-__device__ __forceinline__ void add_bias(const void* bias, int64_t p0, int wp, int lane, int v0, int classes, typename T::acc_t (&acc)[T::FP][T::FQ]) {
-    if (bias) {
+// The tile's logits in acc.
+template <class T, int DT, class A>
+__device__ __forceinline__ void logits(const A& a, int64_t p0, int64_t q0, char* lds, typename T::acc_t (&acc)[T::FP][T::FQ]) {
+    constexpr bool SPLIT = DT == DT_F32;
+    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, ((a.kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), SPLIT, lds, acc);
+#ifdef __HIP_DEVICE_COMPILE__
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    const int ml = wp * T::TP + (lane >> 4) * 4;
+    const int64_t here = a.w.rows - p0;       // classes of the piece from the tile's first one on
+    if constexpr (SPLIT) {
+        float un[T::FQ];
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) {
+            const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
+            un[j] = a.un_x[(n < a.x.rows ? n : a.x.rows - 1) * a.un_step];
+        }
+        const AxisView un_w(a.un_w + p0 * a.un_step, a.un_step ? here : 0);
 #pragma unroll
         for (int i = 0; i < T::FP; ++i) {
-            const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4 + v0;
+            f32x4 u = un_w.four(ml + i * 16);
+            if (!a.un_step) u = f32x4{1.0f, 1.0f, 1.0f, 1.0f} * *a.un_w;
+#pragma unroll
+            for (int j = 0; j < T::FQ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = acc[i][j][r] * u[r] * un[j];
+        }
+    }
+    if (a.bias) {
+        const AxisView bias((const char*)a.bias + (a.v0 + p0) * (DT == DT_F32 ? 4 : 2), here * (DT == DT_F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float b = m + r < classes ? load_scalar<DT>(bias, m + r) : 0.0f;
+                const float b = bias.one<DT>(ml + i * 16 + r);
 #pragma unroll
                 for (int j = 0; j < T::FQ; ++j) acc[i][j][r] += b;
             }
-        }
     }
+#endif
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -210,10 +273,8 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
     mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
-    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
-    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
-    add_bias<T, DT>(a.bias, p0, wp, lane, a.v0, a.t.classes, acc);
+    logits<T, DT>(a, p0, q0, lds, acc);
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     const int left = a.t.classes - a.v0 - (int)p0 - wp * T::TP - (lane >> 4) * 4;   // classes from this lane's first one on
     if (p0 + T::BP > a.t.classes - a.v0) {          // the last tile
 #pragma unroll
@@ -317,6 +378,7 @@ struct JoinArgs {
     float *ref, *inv, *mean, *tsum, *scalars;   // kept for the backward pass: reference, 1 / l, s / l, sum pi
     float *ce, *ent, *tabs;                     // per row
     float *loss, *out_ce, *out_ent;          // results, per row or one; the last two may be null
+    const float *un_x, *un_w;                // float32: what each row, each class was divided by; or null
 };
 
 __device__ __forceinline__ Part part_at(const JoinArgs& a, int64_t at) {
@@ -383,6 +445,7 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
     __shared__ double sums[2][16];
     __shared__ float tops[16];
     __shared__ int numbers[16];
+    __shared__ float uns[2][16];
     double ce = 0.0, h = 0.0;
     float top = 0.0f;
     int count = 0;
@@ -392,6 +455,17 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
         ce += a.ce[n];
         h += a.ent[n];
         if (a.t.dense) top = fmaxf(top, a.tabs[n]);
+    }
+    float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides all rows by it
+    if (a.un_x) {
+        for (int n = threadIdx.x; n < a.t.rows; n += 1024) ux = fmaxf(ux, a.un_x[n]);
+#pragma unroll 8
+        for (int m = threadIdx.x; m < a.t.classes; m += 1024) uw = fmaxf(uw, a.un_w[m]);
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            ux = fmaxf(ux, __shfl_xor(ux, o));
+            uw = fmaxf(uw, __shfl_xor(uw, o));
+        }
     }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
@@ -406,6 +480,8 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
         sums[1][w] = h;
         tops[w] = top;
         numbers[w] = count;
+        uns[0][w] = ux;
+        uns[1][w] = uw;
     }
     __syncthreads();
     if (threadIdx.x) return;
@@ -414,6 +490,14 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
         h += sums[1][w];
         top = fmaxf(top, tops[w]);
         count += numbers[w];
+    }
+    if (a.un_x) {
+        for (int w = 1; w < 16; ++w) {
+            ux = fmaxf(ux, uns[0][w]);
+            uw = fmaxf(uw, uns[1][w]);
+        }
+        a.scalars[2] = ux;
+        a.scalars[3] = uw;
     }
     a.scalars[0] = (float)count;
     // |G| <= 2 sum |pi| + |c| (1/e + log classes)
@@ -449,7 +533,7 @@ __global__ __launch_bounds__(1024) void k_ce_join_reduce(JoinArgs a) {
 // rounded wherever it can: rounded with it, the -1 at every row's target would be off by the same relative amount in every row, and
 // that would not average out. With one factor for all rows it multiplies the products' results. With a factor for each row it does so
 // for dx, and for dW, whose sum runs over the rows, G^T holds factor / largest factor.
-// float16 has too few exponents for small p: there G is held times the power of two that takes its bound to at most 2^14, so that
+// float16 (and the two planes of float32) has too few exponents for small p: there G is held times the power of two that takes its bound to at most 2^14, so that
 // values down to 2^-27 of the bound keep all their bits.
 __device__ __forceinline__ float hold_scale(const float* scalars) {
     return ldexpf(1.0f, 14 - (ilogbf(fmaxf(scalars[1], 1e-30f)) + 1));
@@ -474,21 +558,26 @@ __global__ __launch_bounds__(1024) void k_ce_largest(const float* grad, int rows
 struct Factor {
     const float *grad, *scalars, *largest;   // largest: one gradient per row
     int32_t mean, half;                      // half: G is held times hold_scale
+    const float* un;                         // float32: what the other operand was divided by, or null
 };
 __device__ __forceinline__ float factor_all(const Factor& f) {            // dW, db, and dx with one factor
     float v = f.largest ? *f.largest : f.grad[0];
     if (f.mean) v = f.scalars[0] > 0.0f ? v / f.scalars[0] : 0.0f;     // no row counts: G is zero
+    if (f.un) v *= *f.un;
     return f.half ? v / hold_scale(f.scalars) : v;
 }
 __device__ __forceinline__ float factor_row(const Factor& f, int64_t n) {  // dx with one factor per row
-    return f.half ? f.grad[n] / hold_scale(f.scalars) : f.grad[n];
+    const float v = f.un ? f.grad[n] * *f.un : f.grad[n];
+    return f.half ? v / hold_scale(f.scalars) : v;
 }
 
 struct GradArgs {
     MmOperand w, x;
     Rows t;
     const void* bias;
-    int32_t kbytes, segments, v0;
+    int32_t kbytes;
+    const float *un_w, *un_x;
+    int32_t un_step, v0;
     int32_t tiles_p, tiles_q;
     const float *ref, *inv, *mean, *tsum;
     Factor f;
@@ -503,15 +592,13 @@ struct GradArgs {
 template <class T, int DT, bool DENSE, bool ENT>
 __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
     __shared__ __align__(16) char lds[T::LDS];
-    constexpr int NP = DT == DT_F32 ? 3 : 1;
+    constexpr int NP = DT == DT_F32 ? 2 : 1;
     int tp, tq;
     mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
-    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
-    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
-    add_bias<T, DT>(a.bias, p0, wp, lane, a.v0, a.t.classes, acc);
+    logits<T, DT>(a, p0, q0, lds, acc);
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     const int ml = (int)p0 + wp * T::TP + (lane >> 4) * 4;        // class of the piece
     const int left = a.t.classes - a.v0 - ml;
     const float hold = a.f.half ? hold_scale(a.f.scalars) : 1.0f;
@@ -593,16 +680,19 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
     auto bits = [&](int i, int j, int plane, float by) {
         const f32x4 v = acc[i][j] * by;
         if constexpr (DT == DT_F32) {
-            uint16_t o[4][3];
+            uint16_t h[4], m[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) split3(v[r], o[r][0], o[r][1], o[r][2]);
-            return make_uint2((uint32_t)o[0][plane] | (uint32_t)o[1][plane] << 16, (uint32_t)o[2][plane] | (uint32_t)o[3][plane] << 16);
+            for (int r = 0; r < 4; ++r) split2(v[r], h[r], m[r]);
+            const uint2 a = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+            const uint2 b = make_uint2((uint32_t)m[0] | (uint32_t)m[1] << 16, (uint32_t)m[2] | (uint32_t)m[3] << 16);
+            return plane ? b : a;
         } else {
             return pack4<DT>(v[0], v[1], v[2], v[3]);
         }
     };
-#pragma unroll
+#pragma unroll 1
     for (int p = 0; p < NP; ++p) {
+        if constexpr (NP > 1) mm_opaque<T>(acc);       // the planes are made one after another: both would not fit the registers
         if (a.g) {
             mm_stage<T>(lds, [&](int i, int j) { return bits(i, j, p, 1.0f); });
             __syncthreads();
@@ -620,50 +710,55 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
 
 struct OutArgs {
     MmOperand p, q;
-    int32_t kbytes, segments, tiles_p, tiles_q;
-    void* out;             // [q rows][p rows], the last step
-    float* sum;            // running sums over the pieces, or null
+    int32_t kbytes, tiles_p, tiles_q;
+    int32_t splits, per;   // the walk over k in `splits` pieces of `per` steps
+    float* part;           // [splits][q rows][p rows] with more than one: k_ce_out_join adds them
+    void* out;             // [q rows][p rows]
+    float* sum;            // running sums over the pieces of the classes, or null
     int32_t first, last, by_row;
     Factor f;
 };
 
 template <class T, int DT>
 __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
+    const int tiles = a.tiles_p * a.tiles_q, split = id / tiles;
     int tp, tq;
-    mm_place(id, a.tiles_p, a.tiles_q, tp, tq);
+    mm_place(id - split * tiles, a.tiles_p, a.tiles_q, tp, tq);
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
-    const int steps = ((a.kbytes + 127) >> 7) * a.segments;
-    mm_tile<T>(a.p, a.q, p0, q0, a.kbytes, 0, steps, a.segments > 1, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
-    const float all = a.by_row ? 0.0f : factor_all(a.f);
+    const int steps = ((a.kbytes + 127) >> 7) * (DT == DT_F32 ? MM_SEGMENTS : 1), begin = split * a.per;
+    mm_tile<T>(a.p, a.q, p0, q0, a.kbytes, begin, begin + a.per < steps ? begin + a.per : steps, DT == DT_F32, lds, acc);
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     const int64_t width = a.p.rows;
+    const bool first = a.first || a.splits > 1, last = a.last && a.splits == 1;
+    float* const sum = a.splits > 1 ? a.part + (int64_t)split * a.q.rows * width : a.sum;
+    const float all = a.by_row || !last ? 0.0f : factor_all(a.f);
 #pragma unroll
     for (int j = 0; j < T::FQ; ++j) {
         const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
         const bool row = n < a.q.rows;
-        const float post = !row ? 0.0f : a.by_row ? factor_row(a.f, n) : all;
+        const float post = !row || !last ? 0.0f : a.by_row ? factor_row(a.f, n) : all;
 #pragma unroll
         for (int i = 0; i < T::FP; ++i) {
             const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
             const int64_t at = n * width + m;
             if (row && (width & 3) == 0) {
                 if (m < width) {
-                    if (!a.first) acc[i][j] += *(const f32x4*)(a.sum + at);
-                    if (!a.last) *(f32x4*)(a.sum + at) = acc[i][j];
+                    if (!first) acc[i][j] += *(const f32x4*)(sum + at);
+                    if (!last) *(f32x4*)(sum + at) = acc[i][j];
                 }
             } else if (row) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (m + r < width) {
-                        if (!a.first) acc[i][j][r] += a.sum[at + r];
-                        if (!a.last) a.sum[at + r] = acc[i][j][r];
+                        if (!first) acc[i][j][r] += sum[at + r];
+                        if (!last) sum[at + r] = acc[i][j][r];
                     }
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] *= post;
             if constexpr (DT == DT_F32) {       // 16 bytes per lane already
-                if (a.last && row) {
+                if (last && row) {
                     float* o = (float*)a.out + at;
                     if ((width & 3) == 0) {
                         if (m < width) *(f32x4*)o = acc[i][j];
@@ -677,11 +772,26 @@ __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
         }
     }
     if constexpr (DT != DT_F32) {
-        if (!a.last) return;
+        if (!last) return;
         mm_stage<T>(lds, [&](int i, int j) { return pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]); });
         __syncthreads();
         mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.out + (q0 * width + p0) * 2, width * 2, a.q.rows - q0, (width - p0) * 2, (width & 7) == 0);
     }
+}
+
+// Adds the pieces of split walks, in their order: one thread per result.
+template <int DT>
+__global__ __launch_bounds__(256) void k_ce_out_join(OutArgs a, OutArgs b, int64_t blocks_a) {
+    const bool one = (int64_t)blockIdx.x < blocks_a;
+    const OutArgs& o = one ? a : b;
+    const int64_t at = ((int64_t)blockIdx.x - (one ? 0 : blocks_a)) * 256 + threadIdx.x, size = (int64_t)o.p.rows * o.q.rows;
+    if (at >= size) return;
+    float v = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < o.splits; ++i) v += o.part[i * size + at];
+    if (!o.first) v += o.sum[at];
+    if (!o.last) o.sum[at] = v;
+    else store_scalar<DT>(o.out, at, v * (o.by_row ? factor_row(o.f, at / o.p.rows) : factor_all(o.f)));
 }
 
 struct BiasArgs {
@@ -711,12 +821,15 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_out(OutArgs a, OutArgs b, Bia
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-typedef MmTile<256, 256, 2, 4, MM_BF16> BigB;
-typedef MmTile<256, 256, 2, 4, MM_F16> BigH;
-typedef MmTile<128, 128, 2, 2, MM_BF16> MidB;
-typedef MmTile<128, 128, 2, 2, MM_F16> MidH;
-typedef MmTile<64, 64, 2, 2, MM_BF16> SmallB;
-typedef MmTile<64, 64, 2, 2, MM_F16> SmallH;
+// float32 goes as planes of float16. Four stages for the small tile: its workgroups wait for memory more than they compute (eight gain
+// nothing for few tiles and cost a resident workgroup for many: 4096 x 722 -> 362 20.5 against 14.8 us).
+template <int KIND> struct TilesOf {
+    typedef MmTile<256, 256, 2, 4, 2, KIND> Big;
+    typedef MmTile<128, 128, 2, 2, 2, KIND> Mid;
+    typedef MmTile<64, 64, 2, 2, 4, KIND> Small;
+};
+template <int DT> struct Tiles : TilesOf<MM_F16> {};
+template <> struct Tiles<DT_BF16> : TilesOf<MM_BF16> {};
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -730,13 +843,13 @@ int tile_edge(int64_t p, int64_t q) {
 
 struct Layout {       // of the workspace, and the pieces of the classes
     bool split, pack;   // float32; operands copied into rows of whole 16 bytes
-    int planes;
+    int planes;         // 16-bit planes of an operand
     int64_t kpitch;     // bytes of an operand's row as the tile loop reads it (when packed)
     int64_t piece;      // classes of a piece
     int pieces;
     int64_t bytes = 0;
-    int64_t xp = -1, wp = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1;                     // forward
-    int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1;                 // backward
+    int64_t xp = -1, wp = -1, ux = -1, uw = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1;                     // forward
+    int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1, px = -1, pw = -1;                 // backward
     int64_t take(int64_t n) {
         const int64_t at = bytes;
         bytes += round_up(n, 256);
@@ -748,7 +861,7 @@ bool aligned(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p 
 
 void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.split = a.dtype == AZ_DT_F32;
-    l.planes = l.split ? 3 : 1;
+    l.planes = l.split ? 2 : 1;
     l.pack = l.split || !aligned(a.x, a.x_pitch, a.features) || !aligned(a.weight, a.weight_pitch, a.features);
     l.kpitch = round_up(a.features, 8) * 2;
 }
@@ -769,6 +882,10 @@ Layout forward_layout(const az_linear_ce_args& a) {
         l.xp = l.take(a.rows * l.kpitch * l.planes);
         l.wp = l.take(l.piece * l.kpitch * l.planes);
     }
+    if (l.split) {
+        l.ux = l.take(a.rows * 4);
+        l.uw = l.take(a.classes * 4);
+    }
     l.part = l.take(a.rows * tiles * 16);
     l.ce = l.take(a.rows * 8);       // cross entropy, entropy
     if (a.target_dense) {
@@ -778,6 +895,35 @@ Layout forward_layout(const az_linear_ce_args& a) {
         l.zt = l.take(a.rows * 4);
     }
     return l;
+}
+
+// How dx = G W and dW = G^T x of a piece of nv classes go over the chip: one tile size for both, and the longer walk split where the
+// walks are so long, or so few, that the chip would wait for the last ones. A workgroup's walk is at most half of what a compute unit
+// does in all, but not below 8 steps, where fetching the first stage costs as much as the products.
+struct OutPlan {
+    int edge;
+    struct Job {
+        int tiles_p, tiles_q, splits, per;
+    } x, w;
+};
+OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
+    OutPlan o;
+    o.edge = tile_edge(a.features, a.rows + nv);
+    const int walks = l.split ? MM_SEGMENTS : 1;
+    const int64_t steps_x = round_up(nv, 64) / 64 * walks, steps_w = round_up(a.rows, 64) / 64 * walks;
+    auto tiles = [&](int64_t n) { return (int)((n + o.edge - 1) / o.edge); };
+    o.x = {tiles(a.features), tiles(a.rows), 1, (int)steps_x};
+    o.w = {tiles(a.features), tiles(nv), 1, (int)steps_w};
+    const int64_t total = steps_x * o.x.tiles_p * o.x.tiles_q + steps_w * o.w.tiles_p * o.w.tiles_q;
+    const int64_t cap = total / 512 > 8 ? total / 512 : 8;
+    auto split = [&](OutPlan::Job& j, int64_t steps) {
+        if (steps <= 2 * cap) return;
+        j.per = (int)cap;
+        j.splits = (int)((steps + cap - 1) / cap);
+    };
+    split(o.x, steps_x);
+    split(o.w, steps_w);
+    return o;
 }
 
 Layout backward_layout(const az_linear_ce_args& a) {
@@ -804,6 +950,16 @@ Layout backward_layout(const az_linear_ce_args& a) {
     l.gt = l.take(l.piece * np * 2 * l.planes);
     l.db = l.take((a.rows + 63) / 64 * l.piece * 4);      // the smallest tiles make the most sums
     if (l.pieces > 1) l.sum = l.take(a.rows * a.features * 4);
+    // sums of split walks, for the piece that splits most
+    int64_t nx = 0, nw = 0;
+    for (int i = 0; i < l.pieces; i += l.pieces > 1 ? l.pieces - 1 : 1) {
+        const int64_t nv = i + 1 < l.pieces ? l.piece : a.classes - (l.pieces - 1) * l.piece;
+        const OutPlan o = out_plan(a, l, nv);
+        if (o.x.splits > 1 && o.x.splits * a.rows * a.features * 4 > nx) nx = o.x.splits * a.rows * a.features * 4;
+        if (o.w.splits > 1 && o.w.splits * nv * a.features * 4 > nw) nw = o.w.splits * nv * a.features * 4;
+    }
+    l.px = l.take(nx);
+    l.pw = l.take(nw);
     l.largest = l.take(16);
     return l;
 }
@@ -867,12 +1023,9 @@ void launch_grad(const GradArgs& s, bool dense, bool ent, hipStream_t st) {
     else hipLaunchKernelGGL((k_ce_grad<T, DT, false, false>), grid, block, 0, st, s);
 }
 
-template <int DT> struct Tiles { typedef BigB Big; typedef MidB Mid; typedef SmallB Small; };
-template <> struct Tiles<DT_F16> { typedef BigH Big; typedef MidH Mid; typedef SmallH Small; };
-
 struct Kept {      // what the forward pass leaves for the backward one
     float *ref, *inv, *mean, *tsum, *scalars;
-    Kept(float* p, int64_t rows) : ref(p), inv(p + rows), mean(p + 2 * rows), tsum(p + 3 * rows), scalars(p + 4 * rows) {}
+    Kept(float* p, int64_t rows) : ref(p), inv(p + rows), mean(p + 2 * rows), tsum(p + 3 * rows), scalars(p + 4 * rows) {}     // 4 of them
 };
 
 template <int DT>
@@ -882,7 +1035,8 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
     StatArgs s{};
     s.t = rows_of(a);
     s.bias = a.bias;
-    s.segments = l.split ? 6 : 1;
+    s.un_x = l.split ? (float*)(ws + l.ux) : nullptr;
+    s.un_step = 1;
     s.part = (f32x4*)(ws + l.part);
     s.tpart = a.target_dense ? (float*)(ws + l.tpart) : nullptr;
     s.zt = a.target_dense ? nullptr : (float*)(ws + l.zt);
@@ -894,9 +1048,13 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
         const char* w = (const char*)a.weight + v0 * a.weight_pitch * (l.split ? 4 : 2);
         if (l.pack) {
             PackArgs p{};
-            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch};
-            if (i == 0) p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch};
+            float* const uw = l.split ? (float*)(ws + l.uw) + v0 : nullptr;
+            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch, uw, nullptr, nullptr, 0};
+            if (i == 0)
+                p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch, l.split ? (float*)(ws + l.ux) : nullptr,
+                              nullptr, s.t.index, a.ignore_index};
             pack<DT>(p, st);
+            s.un_w = uw;
             s.w = MmOperand{ws + l.wp, l.kpitch, l.piece * l.kpitch, (int)nv};
             s.x = MmOperand{ws + l.xp, l.kpitch, a.rows * l.kpitch, (int)a.rows};
         } else {
@@ -914,7 +1072,8 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
     }
     const Kept k(kept, a.rows);
     const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
-                     a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent};
+                     a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent,
+                     l.split ? (float*)(ws + l.ux) : nullptr, l.split ? (float*)(ws + l.uw) : nullptr};
     if (a.rows <= 512 && s.tiles <= 32) {
         hipLaunchKernelGGL(k_ce_join_reduce, dim3(1), dim3(1024), 0, st, j);
     } else {
@@ -931,12 +1090,15 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     const int esize = l.split ? 4 : 2;
     const int64_t np = round_up(a.rows, 64), vp = round_up(l.piece, 64);
     const bool each = a.reduction == AZ_REDUCE_NONE;
-    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT == DT_F16};
+    const float *un_x = l.split ? kept.scalars + 2 : nullptr, *un_w = l.split ? kept.scalars + 3 : nullptr;
+    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT != DT_BF16, nullptr};
     if (each) hipLaunchKernelGGL(k_ce_largest, dim3(1), dim3(1024), 0, st, grad, (int)a.rows, (float*)(ws + l.largest));
     GradArgs s{};
     s.t = rows_of(a);
     s.bias = a.bias;
-    s.segments = l.split ? 6 : 1;
+    s.un_x = un_x;
+    s.un_w = un_w;
+    s.un_step = 0;
     s.kbytes = (int)(l.pack ? l.kpitch : a.features * 2);
     s.ref = kept.ref;
     s.inv = kept.inv;
@@ -956,16 +1118,17 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         const int64_t vpi = round_up(nv, 64);    // k of dx in this piece
         PackArgs p{};
         if (l.pack) {
-            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch};
-            if (i == 0) p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch};
+            p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch, nullptr, un_w, nullptr, 0};
+            if (i == 0)
+                p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch, nullptr, un_x, s.t.index, a.ignore_index};
             s.w = MmOperand{ws + l.wp, l.kpitch, l.piece * l.kpitch, (int)nv};
             s.x = MmOperand{ws + l.xp, l.kpitch, a.rows * l.kpitch, (int)a.rows};
         } else {
             s.w = MmOperand{w, a.weight_pitch * 2, 0, (int)nv};
             s.x = MmOperand{(const char*)a.x, a.x_pitch * 2, 0, (int)a.rows};
         }
-        if (gx) p.wt = TurnJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wt, vpi * 2, a.features * vpi * 2, nullptr, 0};
-        if (gw && i == 0) p.xt = TurnJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xt, np * 2, a.features * np * 2, s.t.index, a.ignore_index};
+        if (gx) p.wt = TurnJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wt, vpi * 2, a.features * vpi * 2, un_w, nullptr, 0};
+        if (gw && i == 0) p.xt = TurnJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xt, np * 2, a.features * np * 2, un_x, s.t.index, a.ignore_index};
         pack<DT>(p, st);
         s.g_pitch = vpi * 2;
         s.g_plane = a.rows * vpi * 2;
@@ -979,6 +1142,7 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         else if (edge == 128) launch_grad<typename Tiles<DT>::Mid, DT>(s, d, e, st);
         else launch_grad<typename Tiles<DT>::Small, DT>(s, d, e, st);
         if (const int rc = launched("k_ce_grad")) return rc;
+        const OutPlan plan = out_plan(a, l, nv);
         OutArgs ox{}, ow{};
         ox.p = MmOperand{ws + l.wt, vpi * 2, a.features * vpi * 2, (int)a.features};
         ox.q = MmOperand{ws + l.g, vpi * 2, a.rows * vpi * 2, (int)a.rows};
@@ -987,34 +1151,44 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         ox.sum = l.pieces > 1 ? (float*)(ws + l.sum) : nullptr;
         ox.first = i == 0;
         ox.last = i == l.pieces - 1;
+        ox.by_row = each;
+        ox.f = f;
+        ox.f.un = un_w;
+        ox.part = (float*)(ws + l.px);
         ow.p = MmOperand{ws + l.xt, np * 2, a.features * np * 2, (int)a.features};
         ow.q = MmOperand{ws + l.gt, np * 2, l.piece * np * 2, (int)nv};
         ow.kbytes = (int)(np * 2);
         ow.out = (char*)gw + v0 * a.features * esize;
         ow.first = ow.last = 1;
-        ox.segments = ow.segments = s.segments;
-        ox.f = ow.f = f;
-        ox.by_row = each;
-        const int64_t q = (gx ? a.rows : 0) + (gw ? nv : 0);
-        const int oe = tile_edge(a.features, q);
-        auto size = [&](OutArgs& o, bool wanted) {
-            o.tiles_p = (int)((o.p.rows + oe - 1) / oe);
-            o.tiles_q = (int)((o.q.rows + oe - 1) / oe);
-            return wanted ? (int64_t)o.tiles_p * o.tiles_q : 0;
+        ow.f = f;
+        ow.f.un = un_x;
+        ow.part = (float*)(ws + l.pw);
+        auto size = [](OutArgs& o, const OutPlan::Job& j, bool wanted) {
+            o.tiles_p = j.tiles_p;
+            o.tiles_q = j.tiles_q;
+            o.splits = j.splits;
+            o.per = j.per;
+            return wanted ? (int64_t)j.tiles_p * j.tiles_q * j.splits : 0;
         };
-        const int64_t bx = size(ox, gx), bw = size(ow, gw);
+        const int64_t bx = size(ox, plan.x, gx), bw = size(ow, plan.w, gw);
         BiasArgs ob{s.db, s.db_pitch, v0, s.tiles_q, gb ? (int)nv : 0, gb, f};
+        // the longer walks first
+        const bool swap = plan.w.per > plan.x.per;
+        const OutArgs &longer = swap ? ow : ox, &second = swap ? ox : ow;
+        const int64_t ba = swap ? bw : bx, bs = swap ? bx : bw;
         auto run = [&](auto tile) {
             typedef decltype(tile) T;
             const int64_t bb = (ob.classes + T::THREADS - 1) / T::THREADS;
-            hipLaunchKernelGGL((k_ce_out<T, DT>), dim3((unsigned)(bx + bw + bb)), dim3(T::THREADS), 0, st, ox, ow, ob, (int)bx, (int)bw);
+            hipLaunchKernelGGL((k_ce_out<T, DT>), dim3((unsigned)(ba + bs + bb)), dim3(T::THREADS), 0, st, longer, second, ob, (int)ba, (int)bs);
         };
-        if (oe == 256) run(typename Tiles<DT>::Big{});
-        else if (oe == 128) run(typename Tiles<DT>::Mid{});
+        if (plan.edge == 256) run(typename Tiles<DT>::Big{});
+        else if (plan.edge == 128) run(typename Tiles<DT>::Mid{});
         else run(typename Tiles<DT>::Small{});
         if (const int rc = launched("k_ce_out")) return rc;
+        const int64_t jx = bx && ox.splits > 1 ? (a.rows * a.features + 255) / 256 : 0, jw = bw && ow.splits > 1 ? (nv * a.features + 255) / 256 : 0;
+        if (jx + jw) hipLaunchKernelGGL((k_ce_out_join<DT>), dim3((unsigned)(jx + jw)), dim3(256), 0, st, ox, ow, jx);
     }
-    return AZ_OK;
+    return launched("k_ce_out_join");
 }
 
 }  // namespace

@@ -28,78 +28,117 @@ struct QuantArgs {
     int32_t cols;
     int64_t rows;
     int8_t* q;
-    int64_t q_pitch;    // bytes; behind the last column zeros up to the pitch rounded down to 16
+    int64_t q_pitch;    // bytes
+    int64_t pad;        // columns to write, those behind the last one as zeros
     float* scale;
 };
 
-// One workgroup per row: the maximum, then the quotients (the second read of the row comes from L1 / L2).
-// The nearest whole number of the real quotient 127 x / max: the product with the reciprocal is off by less than 127 * 2^-23, so
-// only where it comes within 1e-4 of a half does a division in 64 bits (127 x exact there) decide.
+// A lane's share of a row at a time: 16 bytes of the input. It may start anywhere; columns behind the last one are zero.
+template <int DT> struct Chunk {
+    static constexpr int N = DT == DT_F32 ? 4 : 8;
+};
 template <int DT>
-__global__ __launch_bounds__(256) void k_quantize(QuantArgs a) {
-    __shared__ float tops[4];
-    const int64_t row = blockIdx.x;
-    const int64_t base = row * a.pitch;
-    constexpr int V = DT == DT_F32 ? 4 : 8;
-    const bool wide = (((uintptr_t)a.x & 15) == 0) && (a.pitch % V == 0);
-    float top = 0.0f;
-    auto see = [&](float v) {
-        v = fabsf(v);
-        top = v > top || v != v ? v : top;      // a NaN stays
-    };
-    auto load = [&](int c, float (&v)[16]) {    // 16 columns from c on
-        if (wide && c + 16 <= a.cols) {
-            if constexpr (DT == DT_F32) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float4 f = *(const float4*)((const float*)a.x + base + c + 4 * e);
-                    v[4 * e] = f.x, v[4 * e + 1] = f.y, v[4 * e + 2] = f.z, v[4 * e + 3] = f.w;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint4 f = *(const uint4*)((const uint16_t*)a.x + base + c + 8 * e);
-                    const uint32_t u[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[8 * e + 2 * k] = from_bits<DT>((uint16_t)u[k]), v[8 * e + 2 * k + 1] = from_bits<DT>((uint16_t)(u[k] >> 16));
-                }
-            }
+__device__ __forceinline__ void load_chunk(const void* x, int64_t base, int64_t c, int cols, float (&v)[Chunk<DT>::N]) {
+    constexpr int NV = Chunk<DT>::N;
+    if (c + NV <= cols) {
+        if constexpr (DT == DT_F32) {
+            __builtin_memcpy(v, (const float*)x + base + c, 16);
         } else {
+            uint32_t u[4];
+            __builtin_memcpy(u, (const uint16_t*)x + base + c, 16);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = c + e < a.cols ? load_scalar<DT>(a.x, base + c + e) : 0.0f;
+            for (int k = 0; k < 4; ++k) v[2 * k] = from_bits<DT>((uint16_t)u[k]), v[2 * k + 1] = from_bits<DT>((uint16_t)(u[k] >> 16));
         }
-    };
-    float v[16];
-    for (int c = threadIdx.x * 16; c < a.cols; c += 4096) {
-        load(c, v);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) see(v[e]);
+        for (int e = 0; e < NV; ++e) v[e] = c + e < cols ? load_scalar<DT>(x, base + c + e) : 0.0f;
+    }
+}
+// The largest magnitude, as bits: unsigned order puts infinities and NaN above every number.
+__device__ __forceinline__ uint32_t larger(uint32_t top, float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+    return u > top ? u : top;
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+struct Range {
+    float top, inv;      // largest magnitude; 127 / top, or 0 where that has no use (zero, not finite, next to the smallest numbers)
+    __device__ __forceinline__ explicit Range(uint32_t bits) : top(__builtin_bit_cast(float, bits)), inv(top >= 1e-30f && top < INFINITY ? 127.0f / top : 0.0f) {}
+    __device__ __forceinline__ float scale() const { return top < INFINITY ? top / 127.0f : NAN; }     // NaN for NaN too
+};
+
+// The nearest whole numbers of the real quotients 127 v / top, ties to even, four to a word. Adding 1.5 * 2^23 in the multiply-add leaves
+// the whole number in the low bits. The product is off by less than 127 * 2^-23 (the reciprocal's rounding), so only where the
+// remainder comes within 2e-5 of a half does a division in 64 bits (127 v is exact there) decide.
+template <int NV>
+__device__ __forceinline__ void quantize_chunk(const float (&v)[NV], const Range& g, uint32_t (&u)[NV / 4]) {
+    constexpr float MAGIC = 12582912.0f;
+    uint32_t b[NV];
+    float far = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+        const float t = __builtin_fmaf(v[e], g.inv, MAGIC);
+        far = fmaxf(far, fabsf(__builtin_fmaf(v[e], g.inv, MAGIC - t)));
+        b[e] = __builtin_bit_cast(uint32_t, t);
+    }
+    if (far >= 0.49998f || g.inv == 0.0f) {
+#pragma unroll
+        for (int e = 0; e < NV; ++e) b[e] = g.top < INFINITY && g.top > 0.0f ? (uint32_t)(int)rint(127.0 * (double)v[e] / (double)g.top) : 0u;
     }
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) see(__shfl_xor(top, o));
+    for (int w = 0; w < NV / 4; ++w)
+        u[w] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * w + 3], b[4 * w + 2], 0x0c0c0400u), __builtin_amdgcn_perm(b[4 * w + 1], b[4 * w], 0x0c0c0400u), 0x05040100u);
+}
+
+// One workgroup per row; HELD chunks per thread stay in registers between the maximum and the quotients, a longer row is read again
+// (from L2). Bound by memory: 8192 x 8192 bfloat16 in @Q us.
+template <int DT, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void k_quantize(QuantArgs a) {
+    constexpr int NV = Chunk<DT>::N;
+    __shared__ uint32_t tops[THREADS / 64];
+    const int64_t row = blockIdx.x, base = row * a.pitch;
+    uint32_t top = 0;
+    float v[HELD][NV];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) load_chunk<DT>(a.x, base, (h * THREADS + threadIdx.x) * NV, a.cols, v[h]);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int e = 0; e < NV; ++e) top = larger(top, v[h][e]);
+    for (int64_t c = (int64_t)(HELD * THREADS + threadIdx.x) * NV; c < a.cols; c += THREADS * NV) {
+        float u[NV];
+        load_chunk<DT>(a.x, base, c, a.cols, u);
+#pragma unroll
+        for (int e = 0; e < NV; ++e) top = larger(top, u[e]);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, o));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) see(tops[w]);
-    const bool finite = top < INFINITY;          // false for NaN
-    if (threadIdx.x == 0) a.scale[row] = finite ? top / 127.0f : NAN;
-    const float inv = top >= 1e-30f ? 127.0f / top : 0.0f;
-    const int64_t q_cols = a.q_pitch / 16 * 16;
-    const bool whole = (((uintptr_t)a.q | (uintptr_t)a.q_pitch) & 15) == 0;
-    for (int c = threadIdx.x * 16; c < a.cols; c += 4096) {
-        load(c, v);
-        int8_t q[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float y = v[e] * inv, n = rintf(y);
-            int r = (int)n;
-            if (!(fabsf(y - n) < 0.4999f) || inv == 0.0f) r = finite && top > 0.0f ? (int)rint(127.0 * (double)v[e] / (double)top) : 0;
-            q[e] = (int8_t)r;
+    for (int w = 0; w < THREADS / 64; ++w) top = larger(top, tops[w]);
+    const Range range(top);
+    if (threadIdx.x == 0) a.scale[row] = range.scale();
+    const bool whole = (((uintptr_t)a.q | (uintptr_t)a.q_pitch) & (NV - 1)) == 0;
+    auto store = [&](int64_t c, const float (&f)[NV]) {
+        uint32_t u[NV / 4];
+        quantize_chunk(f, range, u);
+        int8_t* o = a.q + row * a.q_pitch + c;
+        if (whole && c + NV <= a.pad) {
+            __builtin_memcpy(__builtin_assume_aligned(o, NV), u, NV);
+        } else {
+            for (int e = 0; e < NV; ++e)
+                if (c + e < a.pad) o[e] = (int8_t)(u[e >> 2] >> (8 * (e & 3)));
         }
-        if (whole && c + 16 <= q_cols) *(uint4*)(a.q + row * a.q_pitch + c) = *(const uint4*)q;
-        else
-            for (int e = 0; e < 16; ++e)
-                if (c + e < a.cols) a.q[row * a.q_pitch + c + e] = q[e];
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int64_t c = (h * THREADS + threadIdx.x) * NV;
+        if (c < a.pad) store(c, v[h]);
+    }
+    for (int64_t c = (int64_t)(HELD * THREADS + threadIdx.x) * NV; c < a.pad; c += THREADS * NV) {
+        float u[NV];
+        load_chunk<DT>(a.x, base, c, a.cols, u);
+        store(c, u);
     }
 }
 
@@ -162,14 +201,21 @@ template <class T, int DT>
 __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
     __shared__ __align__(16) char lds[T::LDS];
     const int tiles = a.tiles_p * a.tiles_q;
-    const int piece = blockIdx.x / tiles;
-    int tp, tq;
-    mm_place(blockIdx.x - piece * tiles, a.tiles_p, a.tiles_q, tp, tq);
+    int piece = 0, tp, tq;
+    if (a.splits == 1) {
+        mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
+    } else {        // a piece of k on one XCD (ids go round the 8 of them): its tiles read the same strips through one L2
+        const int at = blockIdx.x >> 3;
+        piece = (blockIdx.x & 7) + 8 * (at / tiles);
+        tp = at % tiles % a.tiles_p;
+        tq = at % tiles / a.tiles_p;
+        if (piece >= a.splits) return;
+    }
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
     const int steps = (a.kbytes + 127) >> 7, first = piece * a.per, last = first + a.per < steps ? first + a.per : steps;
     mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, first, last, false, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     if (a.splits > 1) {
         i32x4* o = a.part + (((int64_t)piece * tiles + tp * a.tiles_q + tq) * (T::FP * T::FQ)) * T::THREADS + threadIdx.x;
 #pragma unroll
@@ -185,20 +231,36 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
         sx[j] = a.s.x[n < a.s.tokens ? n : a.s.tokens - 1];
     }
     f32x4 v[T::FP][T::FQ];
+#ifdef __HIP_DEVICE_COMPILE__
+    const int ml = wp * T::TP + (lane >> 4) * 4;
+    const int64_t here = a.s.channels - p0;
+    float b[T::FP][4];
+    auto load = [&](auto type) {
+        constexpr int BT = decltype(type)::value;
+        const AxisView bias((const char*)a.s.bias + p0 * (BT == DT_F32 ? 4 : 2), here * (BT == DT_F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) b[i][r] = bias.one<BT>(ml + i * 16 + r);
+    };
+    if (!a.s.bias) {
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) b[i][r] = 0.0f;
+    } else if (a.s.bias_dtype == DT_F32) load(std::integral_constant<int, DT_F32>{});
+    else if (a.s.bias_dtype == DT_BF16) load(std::integral_constant<int, DT_BF16>{});
+    else load(std::integral_constant<int, DT_F16>{});
+    const AxisView ws(a.s.w + p0, here);
 #pragma unroll
     for (int i = 0; i < T::FP; ++i) {
-        float w[4], b[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4 + r, c = m < a.s.channels ? m : a.s.channels - 1;
-            w[r] = a.s.w[c];
-            b[r] = bias_at(a.s, c);
-        }
+        const f32x4 w = ws.four(ml + i * 16);
 #pragma unroll
         for (int j = 0; j < T::FQ; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[i][j][r] = (float)acc[i][j][r] * sx[j] * w[r] + b[r];
+            for (int r = 0; r < 4; ++r) v[i][j][r] = (float)acc[i][j][r] * sx[j] * w[r] + b[i][r];
     }
+#endif
     if constexpr (DT == DT_F32) {       // 16 bytes per lane already
 #pragma unroll
         for (int j = 0; j < T::FQ; ++j) {
@@ -231,15 +293,17 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_join(TileArgs a) {
     const int tiles = a.tiles_p * a.tiles_q, tile = blockIdx.x / (T::FP * T::FQ), f = blockIdx.x % (T::FP * T::FQ);
     const int tp = tile / a.tiles_q, tq = tile % a.tiles_q, i = f / T::FQ, j = f % T::FQ;
     i32x4 sum = {};
+#pragma unroll 8
     for (int p = 0; p < a.splits; ++p) sum += a.part[(((int64_t)p * tiles + tile) * (T::FP * T::FQ) + f) * T::THREADS + threadIdx.x];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
+    const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     finish4<DT>(a.s, (int64_t)tq * T::BQ + wq * T::TQ + j * 16 + (lane & 15), (int64_t)tp * T::BP + wp * T::TP + i * 16 + (lane >> 4) * 4, sum);
 }
 
 struct FewArgs {
-    const int8_t *w, *x;
-    int64_t w_pitch, x_pitch;
-    int32_t cols;
+    const int8_t* w;
+    const void* x;          // int8 rows, or the floating ones (DX)
+    int64_t w_pitch, x_pitch;   // elements
+    int32_t cols, share;
     Scales s;
 };
 
@@ -256,45 +320,130 @@ __device__ __forceinline__ i32x4 bytes16(const int8_t* row, int k, int cols) {
     return v;
 }
 
-// Up to 16 * MT tokens: a workgroup takes 16 channels, its waves take k in turns of 64 bytes, straight from memory to the matrix
-// instruction's registers (lane: channel lane & 15, 16 bytes of k). Nothing is read twice but the tokens.
-template <int DT, int MT>
+// Up to 16 * MT tokens, for which the weights' bytes are what counts. A workgroup is 16 waves; `share` of them take the same 16 channels
+// and go through k in turns of 64 bytes, straight from memory to the matrix instruction's registers (lane: channel or token lane & 15,
+// 16 bytes of k), U turns' loads before the first product. Rows may start anywhere. Channels and tokens behind the last one repeat it
+// and are not written.
+// Floating tokens (DX, one to FUSED_TOKENS of them) are quantised by every workgroup for itself, into LDS, while its first weights
+// are on the way: one launch, with the values and the sums of two. One token, 4096 -> 16384: @F us against 17.5 us.
+constexpr int FUSED_TOKENS = 4, FUSED_BYTES = 32768, DT_I8 = AZ_DT_I8;
+template <int DT, int DX, int MT>
 __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
+    constexpr bool FUSED = DX != DT_I8;
+    constexpr int U = MT == 1 ? 8 : 2;
     __shared__ i32x4 joint[16][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t m0 = (int64_t)blockIdx.x * 16;
+    __shared__ __align__(16) int8_t q[FUSED ? FUSED_BYTES : 16];
+    __shared__ uint32_t tops[FUSED_TOKENS][16];
+    __shared__ float scales[FUSED_TOKENS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, turn = wave % a.share;
+    const int64_t m0 = ((int64_t)blockIdx.x * (16 / a.share) + wave / a.share) * 16;
     const int64_t m = m0 + (lane & 15) < a.s.channels ? m0 + (lane & 15) : a.s.channels - 1;
-    const int8_t* wr = a.w + m * a.w_pitch;
+    const int8_t* const wr = a.w + m * a.w_pitch;
+    const int step = a.share * 64, own = (lane >> 4) * 16, pitch = (a.cols + 63) / 64 * 64;
+    // 16 bytes at k of a row, in one load without a branch: where the row ends before they do its last 16, for which the weights become
+    // zero; the bytes of a last piece that is not whole come by themselves after the loop
+    const bool vector = a.cols >= 16;
+    auto bytes = [&](const int8_t* row, int k) {
+        i32x4 v;
+        __builtin_memcpy(&v, row + (k + 16 <= a.cols ? k : a.cols - 16), 16);
+        return v;
+    };
+    int k0 = turn * 64;
+    i32x4 w[U];
+    auto weights = [&] {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * step + own;
+            w[u] = bytes(wr, k);
+            if (k + 16 > a.cols) w[u] = i32x4{0, 0, 0, 0};
+        }
+    };
+    if (vector && k0 < a.cols) weights();
+    if constexpr (FUSED) {
+        constexpr int NV = Chunk<DX>::N;
+        for (int n = 0; n < a.s.tokens; ++n) {
+            uint32_t top = 0;
+            for (int c = threadIdx.x * NV; c < a.cols; c += 1024 * NV) {
+                float v[NV];
+                load_chunk<DX>(a.x, n * a.x_pitch, c, a.cols, v);
+#pragma unroll
+                for (int e = 0; e < NV; ++e) top = larger(top, v[e]);
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, o));
+            if (lane == 0) tops[n][wave] = top;
+        }
+        __syncthreads();
+        for (int n = 0; n < a.s.tokens; ++n) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) top = larger(top, tops[n][v]);
+            const Range range(top);
+            if (threadIdx.x == 0) scales[n] = range.scale();
+            for (int c = threadIdx.x * NV; c < pitch; c += 1024 * NV) {
+                float v[NV];
+                uint32_t u[NV / 4];
+                load_chunk<DX>(a.x, n * a.x_pitch, c, a.cols, v);
+                quantize_chunk(v, range, u);
+                __builtin_memcpy(__builtin_assume_aligned(q + n * pitch + c, NV), u, NV);
+            }
+        }
+        __syncthreads();
+    }
+    const int8_t* xr[MT];
     i32x4 acc[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = i32x4{};
-    for (int k0 = wave * 64; k0 < a.cols; k0 += waves * 64) {
-        const int k = k0 + (lane >> 4) * 16;
-        const i32x4 w = bytes16(wr, k, a.cols);
+    for (int t = 0; t < MT; ++t) {
+        const int n = t * 16 + (lane & 15), in = n < a.s.tokens ? n : a.s.tokens - 1;
+        xr[t] = FUSED ? q + in * pitch : (const int8_t*)a.x + in * a.x_pitch;
+        acc[t] = i32x4{};
+    }
+    for (; vector && k0 < a.cols; k0 += U * step) {
+        i32x4 x[U][MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int n = t * 16 + (lane & 15);
-            const i32x4 x = n < a.s.tokens ? bytes16(a.x + n * a.x_pitch, k, a.cols) : i32x4{};
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc[t], 0, 0, 0);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int k = k0 + u * step + own;
+                if constexpr (FUSED) x[u][t] = *(const i32x4*)(xr[t] + (k < pitch ? k : 0));
+                else x[u][t] = bytes(xr[t], k);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u][t], acc[t], 0, 0, 0);
+        if (k0 + U * step < a.cols) {
+            k0 += U * step;
+            weights();
+            k0 -= U * step;
         }
+    }
+    const int rest = a.cols / 64 * 64 + own;         // where a piece that is not whole could be
+    if ((a.cols & 15) && turn == a.cols / 64 % a.share) {
+        const i32x4 v = rest + 16 > a.cols ? bytes16(wr, rest, a.cols) : i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, FUSED ? *(const i32x4*)(xr[t] + (rest < pitch ? rest : 0)) : bytes16(xr[t], rest, a.cols), acc[t], 0, 0, 0);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) joint[wave][t][lane] = acc[t];
     __syncthreads();
-    for (int t = wave; t < MT; t += waves) {
+    Scales s = a.s;
+    if (FUSED) s.x = scales;
+    for (int t = turn; t < MT; t += a.share) {
         i32x4 sum = {};
-        for (int v = 0; v < waves; ++v) sum += joint[v][t][lane];
-        finish4<DT>(a.s, t * 16 + (lane & 15), m0 + (lane >> 4) * 4, sum);
+        for (int v = 0; v < a.share; ++v) sum += joint[wave - turn + v][t][lane];
+        finish4<DT>(s, t * 16 + (lane & 15), m0 + (lane >> 4) * 4, sum);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-typedef MmTile<256, 256, 2, 4, MM_I8> Big;
-typedef MmTile<128, 128, 2, 2, MM_I8> Mid;
-typedef MmTile<64, 64, 2, 2, MM_I8> Small;
+typedef MmTile<256, 256, 2, 4, 2, MM_I8> Big;
+typedef MmTile<128, 128, 2, 2, 2, MM_I8> Mid;
+typedef MmTile<64, 64, 2, 2, 4, MM_I8> Small;
 
 struct Plan {
-    bool few, align_w, align_x;
+    bool few, fused, align_w, align_x;
     int edge = 64, splits = 1, per = 0;
     int64_t kpitch;
     int64_t q = -1, scale = -1, w = -1, x = -1, part = -1, bytes = 0;
@@ -309,6 +458,8 @@ Plan plan_of(const az_int8_args& a) {
     Plan p;
     p.kpitch = round_up(a.features, 16);
     p.few = a.tokens <= 64;
+    p.fused = a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
+    if (p.fused) return p;
     if (a.x_dtype != AZ_DT_I8) {
         p.q = p.take(a.tokens * p.kpitch);
         p.scale = p.take(a.tokens * 4);
@@ -323,8 +474,8 @@ Plan plan_of(const az_int8_args& a) {
     p.edge = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
     const int steps = (int)((p.kpitch + 127) / 128);
     p.per = steps;
-    if (p.edge == 64) {      // split k until there are two workgroups per compute unit, with at least 4 steps each
-        int64_t s = 512 / tiles(64);
+    if (p.edge == 64) {      // split k until there is a workgroup per compute unit, with at least 4 steps each
+        int64_t s = 256 / tiles(64);
         if (s > steps / 4) s = steps / 4;
         if (s > 1) {
             p.per = (int)((steps + s - 1) / s);
@@ -355,34 +506,58 @@ int launched(const char* what) {
     return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
+// 256 threads hold rows of up to 32 KB, 1024 of up to 128 KB (256 x 23104 float32: @V us, with 256 threads and a second read 14.9 us).
+template <int DT>
+void quantize_as(const QuantArgs& q, hipStream_t st) {
+    const dim3 grid((unsigned)q.rows);
+    const int64_t bytes = (int64_t)q.cols * (DT == DT_F32 ? 4 : 2);
+    if (bytes <= 8192) hipLaunchKernelGGL((k_quantize<DT, 256, 2>), grid, dim3(256), 0, st, q);
+    else if (bytes <= 16384) hipLaunchKernelGGL((k_quantize<DT, 256, 4>), grid, dim3(256), 0, st, q);
+    else if (bytes <= 32768) hipLaunchKernelGGL((k_quantize<DT, 256, 8>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((k_quantize<DT, 1024, 8>), grid, dim3(1024), 0, st, q);
+}
 void quantize(int dtype, const QuantArgs& q, hipStream_t st) {
-    const dim3 grid((unsigned)q.rows), block(256);
-    if (dtype == AZ_DT_F32) hipLaunchKernelGGL((k_quantize<DT_F32>), grid, block, 0, st, q);
-    else if (dtype == AZ_DT_BF16) hipLaunchKernelGGL((k_quantize<DT_BF16>), grid, block, 0, st, q);
-    else hipLaunchKernelGGL((k_quantize<DT_F16>), grid, block, 0, st, q);
+    if (dtype == AZ_DT_F32) quantize_as<DT_F32>(q, st);
+    else if (dtype == AZ_DT_BF16) quantize_as<DT_BF16>(q, st);
+    else quantize_as<DT_F16>(q, st);
 }
 
 template <class T, int DT>
 void run_tiles(const TileArgs& t, hipStream_t st) {
-    const unsigned tiles = (unsigned)(t.tiles_p * t.tiles_q);
-    hipLaunchKernelGGL((k_int8_tile<T, DT>), dim3(tiles * t.splits), dim3(T::THREADS), 0, st, t);
-    if (t.splits > 1) hipLaunchKernelGGL((k_int8_join<T, DT>), dim3(tiles * T::FP * T::FQ), dim3(T::THREADS), 0, st, t);
+    const int rounds = t.splits > 1 ? (t.splits + 7) / 8 * 8 : 1;
+    hipLaunchKernelGGL((k_int8_tile<T, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * rounds)), dim3(T::THREADS), 0, st, t);
+}
+
+// Up to 64 tokens. The waves of a workgroup that share 16 channels are as few as leave a workgroup per compute unit: the join is
+// then smallest.
+template <int DT, int DX>
+int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, hipStream_t st) {
+    const int64_t groups = (a.channels + 15) / 16;
+    int share = 16;
+    while (share > 1 && groups * share / 16 >= 512) share /= 2;
+    const FewArgs f{(const int8_t*)a.weight, x, a.weight_pitch, x_pitch, (int)a.features, share, s};
+    const dim3 grid((unsigned)((groups * share + 15) / 16)), block(1024);
+    if constexpr (DX != DT_I8) {
+        hipLaunchKernelGGL((k_int8_few<DT, DX, 1>), grid, block, 0, st, f);
+    } else {
+        if (a.tokens <= 16) hipLaunchKernelGGL((k_int8_few<DT, DX, 1>), grid, block, 0, st, f);
+        else if (a.tokens <= 32) hipLaunchKernelGGL((k_int8_few<DT, DX, 2>), grid, block, 0, st, f);
+        else if (a.tokens <= 48) hipLaunchKernelGGL((k_int8_few<DT, DX, 3>), grid, block, 0, st, f);
+        else hipLaunchKernelGGL((k_int8_few<DT, DX, 4>), grid, block, 0, st, f);
+    }
+    return launched("k_int8_few");
+}
+
+template <int DT>
+int fused(const az_int8_args& a, const Scales& s, hipStream_t st) {
+    if (a.x_dtype == AZ_DT_F32) return few<DT, DT_F32>(a, a.x, a.x_pitch, s, st);
+    if (a.x_dtype == AZ_DT_BF16) return few<DT, DT_BF16>(a, a.x, a.x_pitch, s, st);
+    return few<DT, DT_F16>(a, a.x, a.x_pitch, s, st);
 }
 
 template <int DT>
 int product(const az_int8_args& a, const Plan& p, const int8_t* x, int64_t x_pitch, const Scales& s, char* ws, hipStream_t st) {
-    if (p.few) {
-        // waves of a workgroup share its 16 channels' k: as many as it takes to have 8 per compute unit, 16 at most
-        const int64_t groups = (a.channels + 15) / 16;
-        int waves = 4;
-        while (waves < 16 && groups * waves < 2048 && waves * 64 < a.features) waves *= 2;
-        const FewArgs f{(const int8_t*)a.weight, x, a.weight_pitch, x_pitch, (int)a.features, s};
-        const dim3 grid((unsigned)groups), block(waves * 64);
-        if (a.tokens <= 16) hipLaunchKernelGGL((k_int8_few<DT, 1>), grid, block, 0, st, f);
-        else if (a.tokens <= 32) hipLaunchKernelGGL((k_int8_few<DT, 2>), grid, block, 0, st, f);
-        else hipLaunchKernelGGL((k_int8_few<DT, 4>), grid, block, 0, st, f);
-        return launched("k_int8_few");
-    }
+    if (p.few) return few<DT, DT_I8>(a, x, x_pitch, s, st);
     const int8_t* w = (const int8_t*)a.weight;
     int64_t w_pitch = a.weight_pitch;
     auto align = [&](const int8_t* src, int64_t pitch, int64_t rows, int64_t at) {
@@ -411,6 +586,8 @@ int product(const az_int8_args& a, const Plan& p, const int8_t* x, int64_t x_pit
     if (p.edge == 256) run_tiles<Big, DT>(t, st);
     else if (p.edge == 128) run_tiles<Mid, DT>(t, st);
     else run_tiles<Small, DT>(t, st);
+    if (t.splits > 1)
+        hipLaunchKernelGGL((k_int8_join<Small, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * Small::FP * Small::FQ)), dim3(Small::THREADS), 0, st, t);
     return launched("k_int8_tile");
 }
 
@@ -426,7 +603,7 @@ extern "C" int az_quantize_rows(const void* x, int32_t dtype, int64_t rows, int6
     if (pitch < cols || q_pitch < cols) return fail(AZ_ERR_ARG, "a row stride is smaller than the row");
     if (rows == 0) return AZ_OK;
     if (!x || !q || !scale) return fail(AZ_ERR_ARG, "null argument");
-    quantize(dtype, QuantArgs{x, pitch, (int)cols, rows, q, q_pitch, scale}, (hipStream_t)stream);
+    quantize(dtype, QuantArgs{x, pitch, (int)cols, rows, q, q_pitch, cols, scale}, (hipStream_t)stream);
     return launched("k_quantize");
 }
 
@@ -444,10 +621,15 @@ extern "C" int az_int8_linear(const az_int8_args* args, void* workspace, int64_t
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     Scales s{a.x_scale, a.weight_scale, a.bias, a.bias_dtype, a.y, (int)a.tokens, (int)a.channels};
+    if (p.fused) {
+        if (a.y_dtype == AZ_DT_F32) return fused<DT_F32>(a, s, st);
+        if (a.y_dtype == AZ_DT_BF16) return fused<DT_BF16>(a, s, st);
+        return fused<DT_F16>(a, s, st);
+    }
     const int8_t* x = (const int8_t*)a.x;
     int64_t x_pitch = a.x_pitch;
     if (a.x_dtype != AZ_DT_I8) {
-        quantize(a.x_dtype, QuantArgs{a.x, a.x_pitch, (int)a.features, a.tokens, (int8_t*)(ws + p.q), p.kpitch, (float*)(ws + p.scale)}, st);
+        quantize(a.x_dtype, QuantArgs{a.x, a.x_pitch, (int)a.features, a.tokens, (int8_t*)(ws + p.q), p.kpitch, p.kpitch, (float*)(ws + p.scale)}, st);
         if (const int rc = launched("k_quantize")) return rc;
         x = (const int8_t*)(ws + p.q);
         x_pitch = p.kpitch;

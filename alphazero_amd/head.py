@@ -28,8 +28,9 @@ def _need(ok: bool, what: str):
 def _on_gpu(name: str, x: torch.Tensor, *others):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise N.NativeError(f"alphazero_amd.head.{name} needs tensors on a GPU (no CPU fallback)")
+    dev = x.device
     for t in others:
-        if t is not None and t.device != x.device:
+        if t is not None and t.device != dev:
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
 
 
@@ -54,8 +55,11 @@ def _device(device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object around it: 0.1 for 2 us
+
+
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _scratch(size: int, device) -> torch.Tensor:
@@ -76,7 +80,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         rows, dev = x.shape[0], x.device
         shape = (rows,) if reduction == "none" else ()
         out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
-        kept = torch.empty(4 * rows + 2, dtype=torch.float32, device=dev)
+        kept = torch.empty(4 * rows + 4, dtype=torch.float32, device=dev)
         L = N.lib()
         with _device(dev):
             ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 0), "az_linear_ce_workspace"), dev)
@@ -231,6 +235,34 @@ def int8_linear(x, qweight, weight_scale, bias=None, *, x_scale=None, out_dtype=
     x's dtype (float32 for int8 x) or out_dtype. Rows of qweight that start at multiples of 16 bytes are read in place. There is no
     gradient."""
     _on_gpu("int8_linear", x, qweight, weight_scale, bias, x_scale)
+    shape, (channels, features) = x.shape, qweight.shape if qweight.dim() == 2 else (0, 0)
+    whole = x.dtype == torch.int8
+    if not (qweight.dtype == torch.int8 and channels >= 1 and 1 <= features <= 131071 and x.dim() >= 1 and shape[-1] == features
+            and (whole or x.dtype in _DTYPES) and weight_scale.dtype == torch.float32 and weight_scale.shape == (channels,)
+            and (bias is None or (bias.dtype in _DTYPES and bias.shape == (channels,))) and whole == (x_scale is not None)
+            and (x_scale is None or (x_scale.dtype == torch.float32 and x_scale.shape == shape[:-1])) and (out_dtype is None or out_dtype in _DTYPES)):
+        _int8_refuse(x, qweight, weight_scale, bias, x_scale, out_dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+        raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with detached tensors")
+    out_dtype = out_dtype or (torch.float32 if whole else x.dtype)
+    dev = x.device
+    y = torch.empty((*shape[:-1], channels), dtype=out_dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    x2, w = _rows(x), _rows(qweight)
+    scale, wscale = None if x_scale is None else x_scale.reshape(-1).contiguous(), weight_scale.contiguous()
+    b = None if bias is None else bias.contiguous()
+    a = N.AzInt8Args(x2.data_ptr(), w.data_ptr(), _ptr(scale), wscale.data_ptr(), _ptr(b), y.data_ptr(), x2.shape[0], features, channels, _pitch(x2),
+                     _pitch(w), N.AZ_DT_I8 if whole else _DTYPES[x.dtype], 0 if b is None else _DTYPES[b.dtype], _DTYPES[out_dtype])
+    L = N.lib()
+    with _device(dev):
+        size = N.check(L.az_int8_workspace(C.byref(a)), "az_int8_workspace")
+        ws = _scratch(size, dev) if size else None
+        N.check(L.az_int8_linear(C.byref(a), _ptr(ws), size, _stream(dev)), "az_int8_linear")
+    return y
+
+
+def _int8_refuse(x, qweight, weight_scale, bias, x_scale, out_dtype):
     _need(x.dtype in _DTYPES or x.dtype == torch.int8, f"x is float32, bfloat16, float16 or int8, not {x.dtype}")
     _need(qweight.dtype == torch.int8 and qweight.dim() == 2, "qweight is an int8 matrix")
     _need(x.dim() >= 1 and x.shape[-1] == qweight.shape[1], f"x {tuple(x.shape)} and qweight {tuple(qweight.shape)} do not fit")
@@ -239,27 +271,7 @@ def int8_linear(x, qweight, weight_scale, bias=None, *, x_scale=None, out_dtype=
     _need(bias is None or (bias.dtype in _DTYPES and tuple(bias.shape) == (qweight.shape[0],)), "bias is one floating value per channel")
     _need((x_scale is not None) == (x.dtype == torch.int8), "x_scale comes with an int8 x, and only with it")
     _need(x_scale is None or (x_scale.dtype == torch.float32 and x_scale.shape == x.shape[:-1]), "x_scale is one float32 per row of x")
-    _need(out_dtype is None or out_dtype in _DTYPES, f"out_dtype is float32, bfloat16 or float16, not {out_dtype}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
-        raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with detached tensors")
-    out_dtype = out_dtype or (torch.float32 if x.dtype == torch.int8 else x.dtype)
-    dev, channels = x.device, qweight.shape[0]
-    y = torch.empty((*x.shape[:-1], channels), dtype=out_dtype, device=dev)
-    if y.numel() == 0:
-        return y
-    x2, w = _rows(x), _rows(qweight)
-    scale, wscale = None if x_scale is None else x_scale.reshape(-1).contiguous(), weight_scale.contiguous()
-    b = None if bias is None else bias.contiguous()
-    a = N.AzInt8Args(x=x2.data_ptr(), weight=w.data_ptr(), x_scale=_ptr(scale), weight_scale=wscale.data_ptr(), bias=_ptr(b), y=y.data_ptr(),
-                     tokens=x2.shape[0], features=x2.shape[1], channels=channels, x_pitch=_pitch(x2), weight_pitch=_pitch(w),
-                     x_dtype=N.AZ_DT_I8 if x.dtype == torch.int8 else _DTYPES[x.dtype], bias_dtype=_DTYPES[b.dtype] if b is not None else 0,
-                     y_dtype=_DTYPES[out_dtype])
-    L = N.lib()
-    with _device(dev):
-        size = N.check(L.az_int8_workspace(C.byref(a)), "az_int8_workspace")
-        ws = _scratch(size, dev) if size else None
-        N.check(L.az_int8_linear(C.byref(a), _ptr(ws), size, _stream(dev)), "az_int8_linear")
-    return y
+    raise ValueError(f"out_dtype is float32, bfloat16 or float16, not {out_dtype}")
 
 
 class Int8Linear(nn.Module):

@@ -363,7 +363,7 @@ typedef struct {
 /* Bytes of scratch memory of a forward (backward = 0) or backward call, or a negative az_status. */
 int64_t az_linear_ce_workspace(const az_linear_ce_args* args, int32_t backward);
 
-/* kept: float [4 * rows + 2], for the backward call. loss, ce, ent: the loss, its cross entropy and the softmax' entropy, one
+/* kept: float [4 * rows + 4], for the backward call. loss, ce, ent: the loss, its cross entropy and the softmax' entropy, one
  * float each (mean or sum over the rows that count), or [rows] with AZ_REDUCE_NONE; ce and ent may be NULL. */
 int az_linear_ce_forward(const az_linear_ce_args* args, float* kept, float* loss, float* ce, float* ent, void* workspace,
                          int64_t workspace_bytes, void* stream);

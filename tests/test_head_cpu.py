@@ -113,7 +113,7 @@ def test_c_entry_points_refuse():
     assert L.az_quantize_rows(256, 0, 4, 8, 8, 256, 7, 256, None) == N.AZ_ERR_ARG
     assert L.az_quantize_rows(None, 0, 4, 8, 8, 256, 8, 256, None) == N.AZ_ERR_ARG
     assert L.az_quantize_rows(None, 0, 0, 8, 8, None, 8, None, None) == N.AZ_OK
-    good = dict(x=256, weight=512, x_scale=None, weight_scale=768, bias=None, y=1024, tokens=2, features=16, channels=4, x_pitch=16, weight_pitch=16,
+    good = dict(x=256, weight=512, x_scale=None, weight_scale=768, bias=None, y=1024, tokens=8, features=16, channels=4, x_pitch=16, weight_pitch=16,
                 x_dtype=N.AZ_DT_F32, bias_dtype=0, y_dtype=N.AZ_DT_F32)
     size = L.az_int8_workspace(C.byref(N.AzInt8Args(**good)))
     assert size > 0
