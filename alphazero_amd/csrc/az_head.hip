@@ -378,7 +378,8 @@ struct JoinArgs {
     float *ref, *inv, *mean, *tsum, *scalars;   // kept for the backward pass: reference, 1 / l, s / l, sum pi
     float *ce, *ent, *tabs;                     // per row
     float *loss, *out_ce, *out_ent;          // results, per row or one; the last two may be null
-    const float *un_x, *un_w;                // float32: what each row, each class was divided by; or null
+    const float *un_x, *un_w;                // float32: what operands were divided by, by row and class or by workgroup; or null
+    int32_t count_x, count_w;
 };
 
 __device__ __forceinline__ Part part_at(const JoinArgs& a, int64_t at) {
@@ -458,9 +459,9 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
     }
     float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides all rows by it
     if (a.un_x) {
-        for (int n = threadIdx.x; n < a.t.rows; n += 1024) ux = fmaxf(ux, a.un_x[n]);
+        for (int n = threadIdx.x; n < a.count_x; n += 1024) ux = fmaxf(ux, a.un_x[n]);
 #pragma unroll 8
-        for (int m = threadIdx.x; m < a.t.classes; m += 1024) uw = fmaxf(uw, a.un_w[m]);
+        for (int m = threadIdx.x; m < a.count_w; m += 1024) uw = fmaxf(uw, a.un_w[m]);
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             ux = fmaxf(ux, __shfl_xor(ux, o));
@@ -820,6 +821,12 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_out(OutArgs a, OutArgs b, Bia
     else bias_block<DT>(c, (int64_t)(id - blocks_a - blocks_b) * T::THREADS + threadIdx.x);
 }
 
+}  // namespace
+}  // namespace az
+#include "az_head_few.cuh"
+namespace az {
+namespace {
+
 // ------------------------------------------------------------------------------------------------ host side
 // float32 goes as planes of float16. Four stages for the small tile: its workgroups wait for memory more than they compute (eight gain
 // nothing for few tiles and cost a resident workgroup for many: 4096 x 722 -> 362 20.5 against 14.8 us).
@@ -842,6 +849,8 @@ int tile_edge(int64_t p, int64_t q) {
 }
 
 struct Layout {       // of the workspace, and the pieces of the classes
+    bool few = false;   // the kernels of az_head_few.cuh
+    int grid = 0, chunks = 0, chunk = 0;      // of those: workgroups; chunks of the classes, classes of a chunk
     bool split, pack;   // float32; operands copied into rows of whole 16 bytes
     int planes;         // 16-bit planes of an operand
     int64_t kpitch;     // bytes of an operand's row as the tile loop reads it (when packed)
@@ -849,7 +858,7 @@ struct Layout {       // of the workspace, and the pieces of the classes
     int pieces;
     int64_t bytes = 0;
     int64_t xp = -1, wp = -1, ux = -1, uw = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1;                     // forward
-    int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1, px = -1, pw = -1;                 // backward
+    int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1, px = -1, pw = -1, fg = -1;                 // backward
     int64_t take(int64_t n) {
         const int64_t at = bytes;
         bytes += round_up(n, 256);
@@ -868,8 +877,38 @@ void operand_layout(const az_linear_ce_args& a, Layout& l) {
 
 int forward_edge(const az_linear_ce_args& a) { return tile_edge(a.classes, a.rows); }
 
+// Waves of a workgroup that split the features of the same classes: each keeps eight turns of loads.
+int few_share(const az_linear_ce_args& a) {
+    const int64_t turns = a.features / (a.dtype == AZ_DT_F32 ? 16 : 32);
+    int share = 1;
+    while (share < 16 && share * 16 <= turns) share *= 2;
+    return share;
+}
+// Workgroups of the streaming kernel: two per compute unit, each with a stretch of classes.
+int few_grid(const az_linear_ce_args& a) {
+    const int64_t groups = (a.classes + 16 / few_share(a) * FEW_CLASSES - 1) / (16 / few_share(a) * FEW_CLASSES);
+    return (int)(groups < 512 ? groups : 512);
+}
+
 Layout forward_layout(const az_linear_ce_args& a) {
     Layout l;
+    if (a.rows <= FEW_ROWS) {
+        l.few = true;
+        l.grid = few_grid(a);
+        l.part = l.take(a.rows * l.grid * 16);
+        l.ce = l.take(a.rows * 8);
+        if (a.target_dense) {
+            l.tpart = l.take(a.rows * l.grid * 8);
+            l.tabs = l.take(a.rows * 4);
+        } else {
+            l.zt = l.take(a.rows * 4);
+        }
+        if (a.dtype == AZ_DT_F32) {
+            l.ux = l.take(l.grid * 4);
+            l.uw = l.take(l.grid * 4);
+        }
+        return l;
+    }
     operand_layout(a, l);
     // a packed piece of the weight stays below 512 MB
     int64_t piece = a.classes;
@@ -928,6 +967,19 @@ OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
 
 Layout backward_layout(const az_linear_ce_args& a) {
     Layout l;
+    if (a.rows <= FEW_GRAD_ROWS) {
+        l.few = true;
+        l.grid = few_grid(a);
+        l.fg = l.take(a.classes * 16 * 4);
+        // chunks of the classes: about 1024 workgroups, but not below 32 classes, where the sums of dx would weigh more than the weights
+        const int64_t wide = (a.features + 1023) / 1024;
+        int64_t chunks = 1024 / wide < 1 ? 1 : 1024 / wide;
+        if (chunks > (a.classes + 31) / 32) chunks = (a.classes + 31) / 32;
+        l.chunk = (int)((a.classes + chunks - 1) / chunks);
+        l.chunks = (int)((a.classes + l.chunk - 1) / l.chunk);
+        l.sum = l.take((int64_t)l.chunks * a.rows * a.features * 4);
+        return l;
+    }
     operand_layout(a, l);
     const int64_t np = round_up(a.rows, 64);
     // G and its transpose of a piece stay at about 1 GB: then the sums of dx that travel between pieces cost a few per cent
@@ -1023,10 +1075,40 @@ void launch_grad(const GradArgs& s, bool dense, bool ent, hipStream_t st) {
     else hipLaunchKernelGGL((k_ce_grad<T, DT, false, false>), grid, block, 0, st, s);
 }
 
+FewArgs few_args(const az_linear_ce_args& a) {
+    FewArgs f{};
+    f.w = a.weight;
+    f.x = a.x;
+    f.bias = a.bias;
+    f.w_pitch = a.weight_pitch;
+    f.x_pitch = a.x_pitch;
+    f.cols = (int)a.features;
+    f.share = few_share(a);
+    f.t = rows_of(a);
+    return f;
+}
+
 struct Kept {      // what the forward pass leaves for the backward one
     float *ref, *inv, *mean, *tsum, *scalars;
     Kept(float* p, int64_t rows) : ref(p), inv(p + rows), mean(p + 2 * rows), tsum(p + 3 * rows), scalars(p + 4 * rows) {}     // 4 of them
 };
+
+template <int DT>
+int join(const az_linear_ce_args& a, const Layout& l, const StatArgs& s, float* kept, float* loss, float* ce, float* ent, char* ws, hipStream_t st) {
+    const Kept k(kept, a.rows);
+    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
+                     a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent,
+                     l.ux >= 0 ? (float*)(ws + l.ux) : nullptr, l.uw >= 0 ? (float*)(ws + l.uw) : nullptr,
+                     l.few ? l.grid : (int)a.rows, l.few ? l.grid : (int)a.classes};
+    if (a.rows <= 512 && s.tiles <= 32) {
+        hipLaunchKernelGGL(k_ce_join_reduce, dim3(1), dim3(1024), 0, st, j);
+    } else {
+        const int per = s.tiles > 32 ? 4 : 64;
+        hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((a.rows + per - 1) / per)), dim3(256), 0, st, j);
+        hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, j);
+    }
+    return launched("k_ce_join");
+}
 
 template <int DT>
 int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, float* ent, char* ws, hipStream_t st) {
@@ -1034,6 +1116,23 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
     const int edge = forward_edge(a);
     StatArgs s{};
     s.t = rows_of(a);
+    if (l.few) {
+        FewArgs f = few_args(a);
+        s.part = f.part = (f32x4*)(ws + l.part);
+        s.tpart = f.tpart = a.target_dense ? (float*)(ws + l.tpart) : nullptr;
+        s.zt = f.zt = a.target_dense ? nullptr : (float*)(ws + l.zt);
+        s.tiles = l.grid;
+        if (DT == DT_F32) {
+            f.un_x = (float*)(ws + l.ux);
+            f.un_w = (float*)(ws + l.uw);
+        }
+        const dim3 grid((unsigned)l.grid), block(1024);
+        if (a.rows <= 16) hipLaunchKernelGGL((k_ce_few<DT, 1, false>), grid, block, 0, st, f);
+        else if (a.rows <= 32) hipLaunchKernelGGL((k_ce_few<DT, 2, false>), grid, block, 0, st, f);
+        else hipLaunchKernelGGL((k_ce_few<DT, 4, false>), grid, block, 0, st, f);
+        if (const int rc = launched("k_ce_few")) return rc;
+        return join<DT>(a, l, s, kept, loss, ce, ent, ws, st);
+    }
     s.bias = a.bias;
     s.un_x = l.split ? (float*)(ws + l.ux) : nullptr;
     s.un_step = 1;
@@ -1070,23 +1169,36 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
         else launch_stats<typename Tiles<DT>::Small, DT>(s, d, e, st);
         if (const int rc = launched("k_ce_stats")) return rc;
     }
-    const Kept k(kept, a.rows);
-    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
-                     a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent,
-                     l.split ? (float*)(ws + l.ux) : nullptr, l.split ? (float*)(ws + l.uw) : nullptr};
-    if (a.rows <= 512 && s.tiles <= 32) {
-        hipLaunchKernelGGL(k_ce_join_reduce, dim3(1), dim3(1024), 0, st, j);
-    } else {
-        const int per = s.tiles > 32 ? 4 : 64;
-        hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((a.rows + per - 1) / per)), dim3(256), 0, st, j);
-        hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, j);
-    }
-    return launched("k_ce_join");
+    return join<DT>(a, l, s, kept, loss, ce, ent, ws, st);
 }
 
 template <int DT>
 int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, void* gx, void* gw, void* gb, char* ws, hipStream_t st) {
     const Layout l = backward_layout(a);
+    if (l.few) {
+        FewArgs f = few_args(a);
+        f.ref = kept.ref;
+        f.inv = kept.inv;
+        f.mean = kept.mean;
+        f.tsum = kept.tsum;
+        f.grad = grad;
+        f.scalars = kept.scalars;
+        f.each = a.reduction == AZ_REDUCE_NONE;
+        f.mean_of = a.reduction == AZ_REDUCE_MEAN;
+        f.g = (float*)(ws + l.fg);
+        hipLaunchKernelGGL((k_ce_few<DT, 1, true>), dim3((unsigned)l.grid), dim3(1024), 0, st, f);
+        if (const int rc = launched("k_ce_few")) return rc;
+        const FewOutArgs o{a.weight, a.x, a.weight_pitch, a.x_pitch, (int)a.features, l.chunk, f.t, f.g, gx ? (float*)(ws + l.sum) : nullptr, gw, gb};
+        const dim3 grid((unsigned)((a.features + 1023) / 1024), (unsigned)l.chunks), block(256);
+        if (a.rows <= 1) hipLaunchKernelGGL((k_ce_few_out<DT, 1>), grid, block, 0, st, o);
+        else if (a.rows <= 2) hipLaunchKernelGGL((k_ce_few_out<DT, 2>), grid, block, 0, st, o);
+        else if (a.rows <= 4) hipLaunchKernelGGL((k_ce_few_out<DT, 4>), grid, block, 0, st, o);
+        else if (a.rows <= 8) hipLaunchKernelGGL((k_ce_few_out<DT, 8>), grid, block, 0, st, o);
+        else hipLaunchKernelGGL((k_ce_few_out<DT, 16>), grid, block, 0, st, o);
+        const int64_t size = a.rows * a.features;
+        if (gx) hipLaunchKernelGGL((k_ce_few_join<DT>), dim3((unsigned)((size + 255) / 256)), dim3(256), 0, st, o.part, l.chunks, size, gx);
+        return launched("k_ce_few_out");
+    }
     const int esize = l.split ? 4 : 2;
     const int64_t np = round_up(a.rows, 64), vp = round_up(l.piece, 64);
     const bool each = a.reduction == AZ_REDUCE_NONE;

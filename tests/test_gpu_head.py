@@ -56,7 +56,9 @@ def _check(x, w, b, t, c=0.0, reduction="mean", grad=None, ignore=-100):
     return got
 
 
-SIZES = [(1, 1, 1), (1, 8, 2), (3, 5, 7), (64, 64, 64), (65, 72, 130), (256, 162, 82), (17, 1000, 300), (300, 200, 513), (130, 722, 362)]
+# up to 16 rows, up to 64 and more take other kernels
+SIZES = [(2, 4100, 40), (5, 1111, 1000), (9, 31, 700), (16, 2050, 70), (12, 70, 20000), (33, 257, 600), (48, 96, 3000),
+         (1, 1, 1), (1, 8, 2), (3, 5, 7), (64, 64, 64), (65, 72, 130), (256, 162, 82), (17, 1000, 300), (300, 200, 513), (130, 722, 362)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=ids)
@@ -71,9 +73,10 @@ def test_loss_and_gradients(size, dtype, dense):
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 @pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_entropy_and_reductions(dtype, dense, reduction):
-    x, w, b, t = _inputs(200, 96, 150, dtype, dense, True)
-    g = torch.linspace(-3, 5, 200, device="cuda") if reduction == "none" else torch.tensor(7.0, device="cuda")
+@pytest.mark.parametrize("rows", [11, 40, 200])
+def test_entropy_and_reductions(dtype, dense, reduction, rows):
+    x, w, b, t = _inputs(rows, 96, 150, dtype, dense, True)
+    g = torch.linspace(-3, 5, rows, device="cuda") if reduction == "none" else torch.tensor(7.0, device="cuda")
     _check(x, w, b, t, c=0.05, reduction=reduction, grad=g)
 
 
@@ -117,9 +120,11 @@ def test_gradient_by_differences():
         assert abs(float(want - have)) <= 2.0 ** -18 * float(size) + 1e-7
 
 
+@pytest.mark.parametrize("rows", [9, 50, 70])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-def test_rows_that_do_not_count_may_hold_anything(dtype):
-    x, w, b, t = _inputs(70, 40, 90, dtype, False, True)
+def test_rows_that_do_not_count_may_hold_anything(dtype, rows):
+    x, w, b, t = _inputs(rows, 40, 90, dtype, False, True)
+    t[torch.arange(1, 8, 3)] = -100
     out = (t == -100).nonzero()[:, 0]
     assert len(out) >= 3
     x[out[0]], x[out[1]], x[out[2], 3] = float("nan"), float("inf"), -float("inf")
@@ -147,8 +152,9 @@ def test_other_ignore_index_and_last_row():
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 @pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
-def test_classes_that_cannot_be(dtype, dense):
-    x, w, b, t = _inputs(50, 24, 200, dtype, dense, True)
+@pytest.mark.parametrize("rows", [13, 50, 90])
+def test_classes_that_cannot_be(dtype, dense, rows):
+    x, w, b, t = _inputs(rows, 24, 200, dtype, dense, True)
     shut = torch.arange(200, device="cuda") % 3 == 0
     shut[64:192] = True                                  # whole tiles of them
     b[shut] = -float("inf")
@@ -166,9 +172,10 @@ def test_classes_that_cannot_be(dtype, dense):
     assert ((loss - total * math.log(200)).abs()[live] <= 8 * 2.0 ** -23 * 6).all()
 
 
-def test_row_without_a_softmax():
-    x, w, b, t = _inputs(5, 8, 12, F32, False, True)
-    t[:] = torch.tensor([1, 2, 3, 4, -100], device="cuda")
+@pytest.mark.parametrize("rows", [5, 30, 100])
+def test_row_without_a_softmax(rows):
+    x, w, b, t = _inputs(rows, 8, 12, F32, False, True)
+    t[:5] = torch.tensor([1, 2, 3, 4, -100], device="cuda")
     b[:] = -float("inf")
     loss = _run(x, w, b, t, reduction="none")[0]
     assert torch.isnan(loss[:4]).all() and float(loss[4]) == 0.0
@@ -178,39 +185,41 @@ def test_row_without_a_softmax():
     assert float(loss[2]) == float("inf") and torch.isfinite(loss[:2]).all()
 
 
-def test_index_outside_the_classes():
-    x, w, b, t = _inputs(40, 16, 30, BF16, False, True)
+@pytest.mark.parametrize("rows", [10, 40, 80])
+def test_index_outside_the_classes(rows):
+    x, w, b, t = _inputs(rows, 16, 30, BF16, False, True)
     for wrong in (30, -1, 1 << 40, -(1 << 62)):
         u = t.clone()
         u[3] = wrong
-        rows = _run(x, w, b, u, reduction="none")[0]
-        assert math.isnan(float(rows[3])) and torch.isfinite(rows[torch.arange(40) != 3]).all()
+        each = _run(x, w, b, u, reduction="none")[0]
+        assert math.isnan(float(each[3])) and torch.isfinite(each[torch.arange(rows) != 3]).all()
         loss, _, _, gx, gw, gb = _run(x, w, b, u)
         assert math.isnan(float(loss)) and torch.isnan(gx[3]).all() and torch.isnan(gw).any() and torch.isnan(gb).all()
 
 
+@pytest.mark.parametrize("rows", [12, 60, 80])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-def test_layouts(dtype):
+def test_layouts(dtype, rows):
     head = _head()
-    x, w, b, t = _inputs(60, 40, 70, dtype, True, True)
+    x, w, b, t = _inputs(rows, 40, 70, dtype, True, True)
     want = _run(x, w, b, t, entropy_coeff=0.01)
-    big = torch.full((80, 64), float("nan"), device="cuda", dtype=dtype)
+    big = torch.full((rows + 20, 64), float("nan"), device="cuda", dtype=dtype)
     wide = torch.full((90, 56), float("nan"), device="cuda", dtype=dtype)
-    tt = torch.full((60, 99), float("nan"), device="cuda")
+    tt = torch.full((rows, 99), float("nan"), device="cuda")
     for dr, dc in ((0, 0), (3, 8), (5, 1)):              # aligned rows of a larger matrix, and rows that start anywhere
-        big[dr:dr + 60, dc:dc + 40] = x
+        big[dr:dr + rows, dc:dc + 40] = x
         wide[dr:dr + 70, dc:dc + 40] = w
         tt[:, dc:dc + 70] = t
-        got = _run_views(big[dr:dr + 60, dc:dc + 40], wide[dr:dr + 70, dc:dc + 40], b, tt[:, dc:dc + 70])
+        got = _run_views(big[dr:dr + rows, dc:dc + 40], wide[dr:dr + 70, dc:dc + 40], b, tt[:, dc:dc + 70])
         for a, v in zip(want, got):
             assert torch.equal(a, v)
     xt = x.t().contiguous().t()                          # columns first
     assert torch.equal(head.linear_cross_entropy(xt, w, t, b, entropy_coeff=0.01), want[0])
-    x3 = x.reshape(3, 20, 40)
-    assert torch.equal(head.linear_cross_entropy(x3, w, t.reshape(3, 20, 70), b, entropy_coeff=0.01), want[0])
-    rows = head.linear_cross_entropy(x3, w, t.reshape(3, 20, 70), b, reduction="none")
-    assert rows.shape == (3, 20)
-    one = x[:1].expand(60, 40)                           # a row many times: stride 0
+    x3 = x.reshape(2, rows // 2, 40)
+    assert torch.equal(head.linear_cross_entropy(x3, w, t.reshape(2, rows // 2, 70), b, entropy_coeff=0.01), want[0])
+    each = head.linear_cross_entropy(x3, w, t.reshape(2, rows // 2, 70), b, reduction="none")
+    assert each.shape == (2, rows // 2)
+    one = x[:1].expand(rows, 40)                           # a row many times: stride 0
     assert torch.equal(head.linear_cross_entropy(one, w, t, b), head.linear_cross_entropy(one.contiguous(), w, t, b))
 
 
