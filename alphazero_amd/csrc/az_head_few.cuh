@@ -1,4 +1,4 @@
-// The loss of a linear layer for few rows (up to 64; with gradient up to 16): what counts is how often the weight goes through memory.
+// The loss of a linear layer for few rows (up to 16, float32 forward up to 32): what counts is how often the weight goes through memory.
 //
 // Forward: the weight streams once, from memory to the matrix instructions' registers, with no copy and no LDS in between; rows may
 // start anywhere. float32 uses the float32 matrix instruction (0.16 PFLOP/s, which is more than the memory feeds with 16 rows).
@@ -10,7 +10,7 @@
 namespace az {
 namespace {
 
-constexpr int FEW_ROWS = 64, FEW_GRAD_ROWS = 16, FEW_CLASSES = 32;   // classes of a wave: two 16-class fragments for each one of x
+constexpr int FEW_GRAD_ROWS = 16, FEW_CLASSES = 32;   // classes of a wave: two 16-class fragments for each one of x
 
 struct FewArgs {
     const void *w, *x, *bias;
@@ -280,79 +280,104 @@ struct FewOutArgs {
     void *gw, *gb;
 };
 
-// Four neighbours of a row from element c on (they may start anywhere); zero behind the last column.
-template <int DT>
-__device__ __forceinline__ void load4(const void* p, int64_t row, int c, int cols, float (&v)[4]) {
-    if (c + 4 <= cols) {
-        if constexpr (DT == DT_F32) {
-            __builtin_memcpy(v, (const float*)p + row + c, 16);
+// Four neighbours of a row from element c on (they may start anywhere), as they are; zero behind the last column.
+template <int DT> struct Four {
+    uint32_t u[DT == DT_F32 ? 4 : 2];
+    __device__ __forceinline__ void load(const void* p, int64_t row, int c, int cols) {
+        if (c + 4 <= cols) {
+            __builtin_memcpy(u, (const char*)p + (row + c) * FewType<DT>::SIZE, sizeof(u));
         } else {
-            uint16_t h[4];
-            __builtin_memcpy(h, (const uint16_t*)p + row + c, 8);
+            float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = from_bits<DT>(h[e]);
+            for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? load_scalar<DT>(p, row + c + e) : 0.0f;
+            put(v);
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? load_scalar<DT>(p, row + c + e) : 0.0f;
     }
-}
+    __device__ __forceinline__ void put(const float (&v)[4]) {
+        if constexpr (DT == DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = __builtin_bit_cast(uint32_t, v[e]);
+        } else {
+            const uint2 h = pack4<DT>(v[0], v[1], v[2], v[3]);
+            u[0] = h.x, u[1] = h.y;
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (DT == DT_F32) return __builtin_bit_cast(float, u[e]);
+        else return from_bits<DT>((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+    }
+    __device__ __forceinline__ void store(void* p, int64_t row, int c, int cols) const {
+        if (c + 4 <= cols) {
+            __builtin_memcpy((char*)p + (row + c) * FewType<DT>::SIZE, u, sizeof(u));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) {
+                    if constexpr (DT == DT_F32) ((uint32_t*)p)[row + c + e] = u[e];
+                    else ((uint16_t*)p)[row + c + e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+                }
+        }
+    }
+};
 
-// dx and dW of up to NB rows: a thread owns four features, holds x and dx of them in registers and goes through its classes; G comes
-// through scalar registers. 2 NB multiply-adds for each weight read and gradient written: with 16 rows about what the memory allows.
+// dx and dW of up to NB rows: a thread owns four features, holds x and dx of them in registers and goes through its classes, the next
+// eight weights on their way while eight are used; G comes from LDS. 2 NB multiply-adds for each weight read and gradient written: with
+// 16 rows about what the memory allows.
 template <int DT, int NB>
 __global__ __launch_bounds__(256) void k_ce_few_out(FewOutArgs a) {
+    constexpr int U = 8, BLOCK = 64;
+    __shared__ __align__(16) float g[BLOCK][16];
     const int d = (blockIdx.x * 256 + threadIdx.x) * 4;
     const int64_t c0 = (int64_t)blockIdx.y * a.chunk, c1 = c0 + a.chunk < a.t.classes ? c0 + a.chunk : a.t.classes;
-    float x[NB][4], acc[NB][4];
+    Four<DT> x[NB];
+    float acc[NB][4];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const bool in = n < a.t.rows && !(a.t.index && a.t.index[n < a.t.rows ? n : 0] == a.t.ignore);
-        if (in) load4<DT>(a.x, n * a.x_pitch, d, a.cols, x[n]);
+        if (in) x[n].load(a.x, n * a.x_pitch, d, a.cols);
+        else x[n].put({0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (!in) x[n][e] = 0.0f;
-            acc[n][e] = 0.0f;
-        }
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
     }
-    constexpr int U = 4;
-    for (int64_t c = c0; c < c1; c += U) {
-        float w[U][4];
+    Four<DT> w[U], next[U];
+    auto weights = [&](Four<DT>(&v)[U], int64_t c) {      // classes behind the last one repeat it and are not used
 #pragma unroll
-        for (int u = 0; u < U; ++u) load4<DT>(a.w, (c + u < c1 ? c + u : c1 - 1) * a.w_pitch, d, a.cols, w[u]);
+        for (int u = 0; u < U; ++u) v[u].load(a.w, (c + u < c1 ? c + u : c1 - 1) * a.w_pitch, d, a.cols);
+    };
+    weights(w, c0);
+    for (int64_t b0 = c0; b0 < c1; b0 += BLOCK) {
+        __syncthreads();
+        {
+            const int64_t c = b0 + (threadIdx.x >> 2);
+            if (c < c1) *(f32x4*)&g[threadIdx.x >> 2][(threadIdx.x & 3) * 4] = *(const f32x4*)(a.g + c * 16 + (threadIdx.x & 3) * 4);
+        }
+        __syncthreads();
+        for (int64_t c = b0; c < b0 + BLOCK && c < c1; c += U) {
+            weights(next, c + U);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (c + u >= c1) break;
-            const float* g = a.g + (c + u) * 16;
-            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < U; ++u) {
+                if (c + u >= c1) break;
+                const float* gu = g[c - b0 + u];
+                float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+                for (int n = 0; n < NB; ++n) {
+                    const float gn = gu[n];
+                    sum += gn;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[n][e] = __builtin_fmaf(g[n], w[u][e], acc[n][e]);
-                    o[e] = __builtin_fmaf(g[n], x[n][e], o[e]);
-                }
-            if (a.gw) {
-                const int64_t at = (c + u) * a.cols + d;
-                if (d + 4 <= a.cols) {
-                    if constexpr (DT == DT_F32) {
-                        __builtin_memcpy((float*)a.gw + at, o, 16);
-                    } else {
-                        const uint2 h = pack4<DT>(o[0], o[1], o[2], o[3]);
-                        __builtin_memcpy((uint16_t*)a.gw + at, &h, 8);
+                    for (int e = 0; e < 4; ++e) {
+                        acc[n][e] = __builtin_fmaf(gn, w[u].get(e), acc[n][e]);
+                        o[e] = __builtin_fmaf(gn, x[n].get(e), o[e]);
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < a.cols) store_scalar<DT>(a.gw, at + e, o[e]);
                 }
+                if (a.gw) {
+                    Four<DT> v;
+                    v.put(o);
+                    v.store(a.gw, (c + u) * a.cols, d, a.cols);
+                }
+                if (a.gb && d == 0) store_scalar<DT>(a.gb, c + u, sum);
             }
-            if (a.gb && d == 0) {
-                float s = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NB; ++n) s += g[n];
-                store_scalar<DT>(a.gb, c + u, s);
-            }
+            for (int u = 0; u < U; ++u) w[u] = next[u];
         }
     }
     if (a.part)
