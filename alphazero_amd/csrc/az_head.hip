@@ -455,7 +455,7 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
         ++count;
         ce += a.ce[n];
         h += a.ent[n];
-        if (a.t.dense) top = fmaxf(top, a.tabs[n]);
+        if (a.t.dense && a.tabs[n] < INFINITY) top = fmaxf(top, a.tabs[n]);     // a row of infinite weights spoils itself only
     }
     float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides all rows by it
     if (a.un_x) {
@@ -866,12 +866,12 @@ struct Layout {       // of the workspace, and the pieces of the classes
     }
 };
 
-bool aligned(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p & 15) == 0 && (pitch & 7) == 0 && (cols & 7) == 0; }
+bool in_place(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p & 15) == 0 && (pitch & 7) == 0 && (cols & 7) == 0 && pitch * 2 <= MM_MAX_PITCH; }
 
 void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.split = a.dtype == AZ_DT_F32;
     l.planes = l.split ? 2 : 1;
-    l.pack = l.split || !aligned(a.x, a.x_pitch, a.features) || !aligned(a.weight, a.weight_pitch, a.features);
+    l.pack = l.split || !in_place(a.x, a.x_pitch, a.features) || !in_place(a.weight, a.weight_pitch, a.features);
     l.kpitch = round_up(a.features, 8) * 2;
 }
 
@@ -1032,8 +1032,6 @@ int check_args(const az_linear_ce_args* a) {
     if (!a->x || !a->weight || !a->target) return fail(AZ_ERR_ARG, "null argument");
     if (a->x_pitch < a->features || a->weight_pitch < a->features || (a->target_dense && a->target_pitch < a->classes))
         return fail(AZ_ERR_ARG, "a row stride is smaller than the row");
-    const Layout l = [&] { Layout t; operand_layout(*a, t); return t; }();
-    if (!l.pack && (a->x_pitch * 2 > MM_MAX_PITCH || a->weight_pitch * 2 > MM_MAX_PITCH)) return fail(AZ_ERR_ARG, "a row stride is too large");
     if (a->reduction < AZ_REDUCE_NONE || a->reduction > AZ_REDUCE_SUM) return fail(AZ_ERR_ARG, "reduction is none, mean or sum");
     return AZ_OK;
 }

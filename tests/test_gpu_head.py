@@ -223,9 +223,35 @@ def test_layouts(dtype, rows):
     assert torch.equal(head.linear_cross_entropy(one, w, t, b), head.linear_cross_entropy(one.contiguous(), w, t, b))
 
 
-def _run_views(x, w, b, t):
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+def test_rows_far_apart(dtype):
+    """Rows of a very wide matrix (beyond what the tiles address in place), and features that start past 2^31 bytes of a tensor."""
+    x, w, b, t = _inputs(70, 64, 300, dtype, False, True)
+    want = _run(x, w, b, t)
+    far = torch.zeros((300, 4_200_008), device="cuda", dtype=dtype)
+    far[:, 4_200_000 - 64:4_200_000] = w
+    got = _run_views(x, far[:, 4_200_000 - 64:4_200_000], b, t, 0.0)
+    for a, v in zip(want, got):
+        assert torch.equal(a, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [8, 80])
+def test_a_row_of_infinite_weights_spoils_itself_only(dtype, rows):
+    x, w, b, t = _inputs(rows, 32, 50, dtype, True, False)
+    bad = t.clone()
+    bad[3, 7] = float("inf")
+    good, got = _run(x, w, None, t, reduction="sum"), _run(x, w, None, bad, reduction="sum")
+    keep = torch.arange(rows) != 3
+    assert torch.equal(got[3][keep], good[3][keep]) and not torch.isfinite(got[3][3]).any()
+    big = t.clone()
+    big[3] *= 1e4                                        # weights of very different sums
+    _check(x, w, None, big, reduction="sum")
+
+
+def _run_views(x, w, b, t, c=0.01):
     x, w, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True), b.detach().clone().requires_grad_(True)
-    loss, ce, ent = _head().linear_cross_entropy(x, w, t, b, entropy_coeff=0.01, parts=True)
+    loss, ce, ent = _head().linear_cross_entropy(x, w, t, b, entropy_coeff=c, parts=True)
     gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
     return loss.detach(), ce, ent, gx, gw, gb
 
