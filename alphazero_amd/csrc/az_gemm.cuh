@@ -238,9 +238,9 @@ __device__ __forceinline__ void mm_stage_turned(char* lds, F bits) {   // image 
         }
     }
 }
-// An image of ROWS x COLS to dst: rows and bytes beyond `rows` / `bytes` are left out; whole = dst rows start at multiples of 16.
+// An image of ROWS x COLS to dst: rows and bytes beyond `rows` / `bytes` are left out. Rows may start anywhere.
 template <class T, int ROWS, int COLS>
-__device__ __forceinline__ void mm_unstage(const char* lds, char* dst, int64_t pitch, int64_t rows, int64_t bytes, bool whole) {
+__device__ __forceinline__ void mm_unstage(const char* lds, char* dst, int64_t pitch, int64_t rows, int64_t bytes) {
     constexpr int C = COLS / 8;
 #pragma unroll
     for (int k = 0; k < ROWS * C / T::THREADS; ++k) {
@@ -248,8 +248,8 @@ __device__ __forceinline__ void mm_unstage(const char* lds, char* dst, int64_t p
         if (r >= rows || c * 16 >= bytes) continue;
         const uint4 v = *(const uint4*)(lds + r * (COLS * 2) + ((c ^ (r & (C - 1))) * 16));
         char* o = dst + r * pitch + c * 16;
-        if (whole && c * 16 + 16 <= bytes) {
-            *(uint4*)o = v;
+        if (c * 16 + 16 <= bytes) {
+            __builtin_memcpy(o, &v, 16);
         } else {
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll

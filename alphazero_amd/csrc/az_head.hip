@@ -593,7 +593,6 @@ struct GradArgs {
 template <class T, int DT, bool DENSE, bool ENT>
 __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
     __shared__ __align__(16) char lds[T::LDS];
-    constexpr int NP = DT == DT_F32 ? 2 : 1;
     int tp, tq;
     mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
@@ -678,34 +677,34 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
         }
         __syncthreads();
     }
-    auto bits = [&](int i, int j, int plane, float by) {
-        const f32x4 v = acc[i][j] * by;
-        if constexpr (DT == DT_F32) {
-            uint16_t h[4], m[4];
+    auto emit = [&](auto which) {
+        constexpr int P = decltype(which)::value;
+        auto bits = [&](int i, int j, float by) {
+            float v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) split2(v[r], h[r], m[r]);
-            const uint2 a = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
-            const uint2 b = make_uint2((uint32_t)m[0] | (uint32_t)m[1] << 16, (uint32_t)m[2] | (uint32_t)m[3] << 16);
-            return plane ? b : a;
-        } else {
-            return pack4<DT>(v[0], v[1], v[2], v[3]);
-        }
-    };
-#pragma unroll 1
-    for (int p = 0; p < NP; ++p) {
-        if constexpr (NP > 1) mm_opaque<T>(acc);       // the planes are made one after another: both would not fit the registers
+            for (int r = 0; r < 4; ++r) {
+                v[r] = acc[i][j][r] * by;
+                if constexpr (P == 1) v[r] = (v[r] - (float)(_Float16)v[r]) * 2048.0f;      // G is finite in float16: hold_scale
+            }
+            return pack4<DT == DT_BF16 ? DT_BF16 : DT_F16>(v[0], v[1], v[2], v[3]);
+        };
         if (a.g) {
-            mm_stage<T>(lds, [&](int i, int j) { return bits(i, j, p, 1.0f); });
+            mm_stage<T>(lds, [&](int i, int j) { return bits(i, j, 1.0f); });
             __syncthreads();
-            mm_unstage<T, T::BQ, T::BP>(lds, a.g + p * a.g_plane + q0 * a.g_pitch + p0 * 2, a.g_pitch, a.t.rows - q0, a.g_pitch - p0 * 2, true);
+            mm_unstage<T, T::BQ, T::BP>(lds, a.g + P * a.g_plane + q0 * a.g_pitch + p0 * 2, a.g_pitch, a.t.rows - q0, a.g_pitch - p0 * 2);
             __syncthreads();
         }
         if (a.gt) {
-            mm_stage_turned<T>(lds, [&](int i, int j) { return bits(i, j, p, share[j]); });
+            mm_stage_turned<T>(lds, [&](int i, int j) { return bits(i, j, share[j]); });
             __syncthreads();
-            mm_unstage<T, T::BP, T::BQ>(lds, a.gt + p * a.gt_plane + p0 * a.gt_pitch + q0 * 2, a.gt_pitch, a.w.rows - p0, a.gt_pitch - q0 * 2, true);
+            mm_unstage<T, T::BP, T::BQ>(lds, a.gt + P * a.gt_plane + p0 * a.gt_pitch + q0 * 2, a.gt_pitch, a.w.rows - p0, a.gt_pitch - q0 * 2);
             __syncthreads();
         }
+    };
+    emit(std::integral_constant<int, 0>{});
+    if constexpr (DT == DT_F32) {
+        mm_opaque<T>(acc);       // the planes are made one after another: both would not fit the registers
+        emit(std::integral_constant<int, 1>{});
     }
 }
 
@@ -743,11 +742,13 @@ __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
         for (int i = 0; i < T::FP; ++i) {
             const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
             const int64_t at = n * width + m;
-            if (row && (width & 3) == 0) {
-                if (m < width) {
-                    if (!first) acc[i][j] += *(const f32x4*)(sum + at);
-                    if (!last) *(f32x4*)(sum + at) = acc[i][j];
+            if (row && m + 4 <= width) {        // four together, wherever a row starts
+                if (!first) {
+                    f32x4 before;
+                    __builtin_memcpy(&before, sum + at, 16);
+                    acc[i][j] += before;
                 }
+                if (!last) __builtin_memcpy(sum + at, &acc[i][j], 16);
             } else if (row) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -761,8 +762,8 @@ __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
             if constexpr (DT == DT_F32) {       // 16 bytes per lane already
                 if (last && row) {
                     float* o = (float*)a.out + at;
-                    if ((width & 3) == 0) {
-                        if (m < width) *(f32x4*)o = acc[i][j];
+                    if (m + 4 <= width) {
+                        __builtin_memcpy(o, &acc[i][j], 16);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
@@ -776,7 +777,7 @@ __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
         if (!last) return;
         mm_stage<T>(lds, [&](int i, int j) { return pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]); });
         __syncthreads();
-        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.out + (q0 * width + p0) * 2, width * 2, a.q.rows - q0, (width - p0) * 2, (width & 7) == 0);
+        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.out + (q0 * width + p0) * 2, width * 2, a.q.rows - q0, (width - p0) * 2);
     }
 }
 
@@ -840,12 +841,28 @@ template <> struct Tiles<DT_BF16> : TilesOf<MM_BF16> {};
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// Tile edge for a product with p x q results: the largest whose tiles give every compute unit work.
-int tile_edge(int64_t p, int64_t q) {
-    auto tiles = [&](int64_t e) { return ((p + e - 1) / e) * ((q + e - 1) / e); };
-    if (tiles(256) >= 192) return 256;
-    if (tiles(128) >= 192) return 128;
-    return 64;
+// What a product takes, in microseconds, from what the tiles were measured to take: a step (64 of k) of a 256 tile 1.5 on its compute
+// unit, of a 128 tile 0.55 (two of them on a unit at a time), of a 64 tile 0.4; and what a tile takes beside its steps (first loads,
+// results), 8, 3 and 1.5.
+struct TileCost {
+    int edge;
+    double step, rest;
+};
+constexpr TileCost TILE_COSTS[3] = {{256, 1.5, 8.0}, {128, 0.55, 3.0}, {64, 0.4, 1.5}};
+
+// Tile edge for p x q results of sums over `steps` steps: rounds of tiles over the compute units, times a tile.
+int tile_edge(int64_t p, int64_t q, int64_t steps) {
+    int best = 256;
+    double least = 1e300;
+    for (const TileCost& c : TILE_COSTS) {
+        const int64_t tiles = ((p + c.edge - 1) / c.edge) * ((q + c.edge - 1) / c.edge);
+        const double t = (double)((tiles + 255) / 256) * (steps * c.step + c.rest);
+        if (t < least) {
+            least = t;
+            best = c.edge;
+        }
+    }
+    return best;
 }
 
 struct Layout {       // of the workspace, and the pieces of the classes
@@ -875,7 +892,8 @@ void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.kpitch = round_up(a.features, 8) * 2;
 }
 
-int forward_edge(const az_linear_ce_args& a) { return tile_edge(a.classes, a.rows); }
+int64_t logit_steps(const az_linear_ce_args& a) { return (a.features + 63) / 64 * (a.dtype == AZ_DT_F32 ? MM_SEGMENTS : 1); }
+int forward_edge(const az_linear_ce_args& a) { return tile_edge(a.classes, a.rows, logit_steps(a)); }
 
 // Waves of a workgroup that split the features of the same classes: each keeps eight turns of loads, unless more splitting makes a
 // workgroup for every half compute unit.
@@ -942,9 +960,10 @@ Layout forward_layout(const az_linear_ce_args& a) {
     return l;
 }
 
-// How dx = G W and dW = G^T x of a piece of nv classes go over the chip: one tile size for both, and the longer walk split where the
-// walks are so long, or so few, that the chip would wait for the last ones. A workgroup's walk is at most half of what a compute unit
-// does in all, but not below 8 steps, where fetching the first stage costs as much as the products.
+// How dx = G W and dW = G^T x of a piece of nv classes go over the chip: one tile size for both, and walks over k split where they are so
+// long, or so few, that the chip would wait for the last ones. A workgroup's walk is at most half of what a compute unit does in all,
+// but not below 8 steps, where fetching the first stage costs as much as the products. Split walks write and read their sums once
+// more. The tile with the least time is taken.
 struct OutPlan {
     int edge;
     struct Job {
@@ -952,23 +971,36 @@ struct OutPlan {
     } x, w;
 };
 OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
-    OutPlan o;
-    o.edge = tile_edge(a.features, a.rows + nv);
+    OutPlan best{};
+    double least = 1e300;
     const int walks = l.split ? MM_SEGMENTS : 1;
     const int64_t steps_x = round_up(nv, 64) / 64 * walks, steps_w = round_up(a.rows, 64) / 64 * walks;
-    auto tiles = [&](int64_t n) { return (int)((n + o.edge - 1) / o.edge); };
-    o.x = {tiles(a.features), tiles(a.rows), 1, (int)steps_x};
-    o.w = {tiles(a.features), tiles(nv), 1, (int)steps_w};
-    const int64_t total = steps_x * o.x.tiles_p * o.x.tiles_q + steps_w * o.w.tiles_p * o.w.tiles_q;
-    const int64_t cap = total / 512 > 8 ? total / 512 : 8;
-    auto split = [&](OutPlan::Job& j, int64_t steps) {
-        if (steps <= 2 * cap) return;
-        j.per = (int)cap;
-        j.splits = (int)((steps + cap - 1) / cap);
-    };
-    split(o.x, steps_x);
-    split(o.w, steps_w);
-    return o;
+    for (const TileCost& c : TILE_COSTS) {
+        OutPlan o;
+        o.edge = c.edge;
+        auto tiles = [&](int64_t n) { return (int)((n + o.edge - 1) / o.edge); };
+        o.x = {tiles(a.features), tiles(a.rows), 1, (int)steps_x};
+        o.w = {tiles(a.features), tiles(nv), 1, (int)steps_w};
+        const int64_t total = steps_x * o.x.tiles_p * o.x.tiles_q + steps_w * o.w.tiles_p * o.w.tiles_q;
+        const int64_t cap = total / 512 > 8 ? total / 512 : 8;
+        double sums = 0.0;
+        auto split = [&](OutPlan::Job& j, int64_t steps, int64_t results) {
+            if (steps <= 2 * cap) return;
+            j.per = (int)cap;
+            j.splits = (int)((steps + cap - 1) / cap);
+            sums += j.splits * (double)results * 8.0;
+        };
+        split(o.x, steps_x, a.rows * a.features);
+        split(o.w, steps_w, nv * a.features);
+        const int64_t items = (int64_t)o.x.tiles_p * o.x.tiles_q * o.x.splits + (int64_t)o.w.tiles_p * o.w.tiles_q * o.w.splits;
+        const int64_t longest = o.x.per > o.w.per ? o.x.per : o.w.per, mean = total / 256 + 1;
+        const double t = (mean > longest ? mean : longest) * c.step + (double)((items + 255) / 256) * c.rest + (sums > 0.0 ? 5.0 + sums / 4.5e6 : 0.0);
+        if (t < least) {
+            least = t;
+            best = o;
+        }
+    }
+    return best;
 }
 
 Layout backward_layout(const az_linear_ce_args& a) {
@@ -1254,7 +1286,7 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         s.g_plane = a.rows * vpi * 2;
         s.v0 = (int)v0;
         s.db_pitch = nv;
-        const int edge = tile_edge(nv, a.rows);
+        const int edge = tile_edge(nv, a.rows, logit_steps(a));
         s.tiles_p = (int)((nv + edge - 1) / edge);
         s.tiles_q = (int)((a.rows + edge - 1) / edge);
         const bool d = a.target_dense, e = a.entropy_coeff != 0.0f;

@@ -270,8 +270,8 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
             for (int i = 0; i < T::FP; ++i) {
                 const int64_t m = p0 + wp * T::TP + i * 16 + (lane >> 4) * 4;
                 float* o = (float*)a.s.y + n * a.s.channels + m;
-                if ((a.s.channels & 3) == 0) {
-                    if (m < a.s.channels) *(f32x4*)o = v[i][j];
+                if (m + 4 <= a.s.channels) {
+                    __builtin_memcpy(o, &v[i][j], 16);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -282,8 +282,7 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
     } else {
         mm_stage<T>(lds, [&](int i, int j) { return pack4<DT>(v[i][j][0], v[i][j][1], v[i][j][2], v[i][j][3]); });
         __syncthreads();
-        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.s.y + (q0 * a.s.channels + p0) * 2, (int64_t)a.s.channels * 2, a.s.tokens - q0, (a.s.channels - p0) * 2,
-                                    (a.s.channels & 7) == 0);
+        mm_unstage<T, T::BQ, T::BP>(lds, (char*)a.s.y + (q0 * a.s.channels + p0) * 2, (int64_t)a.s.channels * 2, a.s.tokens - q0, (a.s.channels - p0) * 2);
     }
 }
 
@@ -327,18 +326,24 @@ __device__ __forceinline__ i32x4 bytes16(const int8_t* row, int k, int cols) {
 // Floating tokens (DX, one to FUSED_TOKENS of them) are quantised by every workgroup for itself, into LDS, while its first weights
 // are on the way: one launch, with the values and the sums of two. One token, 4096 -> 16384: @F us against 17.5 us.
 constexpr int FUSED_TOKENS = 4, FUSED_BYTES = 32768, DT_I8 = AZ_DT_I8;
+// Channels of a wave in fragments of 16: two for each token fragment read from memory, as long as the sums fit.
+constexpr int few_fragments(bool fused, int mt) { return !fused && mt <= 2 ? 2 : 1; }
 template <int DT, int DX, int MT>
 __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
     constexpr bool FUSED = DX != DT_I8;
-    constexpr int U = MT == 1 ? 8 : 2;
-    __shared__ i32x4 joint[16][MT][64];
+    constexpr int CT = few_fragments(FUSED, MT), U = MT == 1 ? (CT == 1 ? 8 : 4) : 2;
+    __shared__ i32x4 joint[16][CT][MT][64];
     __shared__ __align__(16) int8_t q[FUSED ? FUSED_BYTES : 16];
     __shared__ uint32_t tops[FUSED_TOKENS][16];
     __shared__ float scales[FUSED_TOKENS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, turn = wave % a.share;
-    const int64_t m0 = ((int64_t)blockIdx.x * (16 / a.share) + wave / a.share) * 16;
-    const int64_t m = m0 + (lane & 15) < a.s.channels ? m0 + (lane & 15) : a.s.channels - 1;
-    const int8_t* const wr = a.w + m * a.w_pitch;
+    const int64_t m0 = ((int64_t)blockIdx.x * (16 / a.share) + wave / a.share) * (16 * CT);
+    const int8_t* wr[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+        const int64_t m = m0 + i * 16 + (lane & 15);
+        wr[i] = a.w + (m < a.s.channels ? m : a.s.channels - 1) * a.w_pitch;
+    }
     const int step = a.share * 64, own = (lane >> 4) * 16, pitch = (a.cols + 63) / 64 * 64;
     // 16 bytes at k of a row, in one load without a branch: where the row ends before they do its last 16, for which the weights become
     // zero; the bytes of a last piece that is not whole come by themselves after the loop
@@ -349,13 +354,16 @@ __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
         return v;
     };
     int k0 = turn * 64;
-    i32x4 w[U];
+    i32x4 w[U][CT];
     auto weights = [&] {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * step + own;
-            w[u] = bytes(wr, k);
-            if (k + 16 > a.cols) w[u] = i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                w[u][i] = bytes(wr[i], k);
+                if (k + 16 > a.cols) w[u][i] = i32x4{0, 0, 0, 0};
+            }
         }
     };
     if (vector && k0 < a.cols) weights();
@@ -391,12 +399,13 @@ __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
         __syncthreads();
     }
     const int8_t* xr[MT];
-    i32x4 acc[MT];
+    i32x4 acc[CT][MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int n = t * 16 + (lane & 15), in = n < a.s.tokens ? n : a.s.tokens - 1;
         xr[t] = FUSED ? q + in * pitch : (const int8_t*)a.x + in * a.x_pitch;
-        acc[t] = i32x4{};
+#pragma unroll
+        for (int i = 0; i < CT; ++i) acc[i][t] = i32x4{};
     }
     for (; vector && k0 < a.cols; k0 += U * step) {
         i32x4 x[U][MT];
@@ -411,7 +420,9 @@ __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u][t], acc[t], 0, 0, 0);
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], x[u][t], acc[i][t], 0, 0, 0);
         if (k0 + U * step < a.cols) {
             k0 += U * step;
             weights();
@@ -420,20 +431,28 @@ __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
     }
     const int rest = a.cols / 64 * 64 + own;         // where a piece that is not whole could be
     if ((a.cols & 15) && turn == a.cols / 64 % a.share) {
-        const i32x4 v = rest + 16 > a.cols ? bytes16(wr, rest, a.cols) : i32x4{0, 0, 0, 0};
+        i32x4 x[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, FUSED ? *(const i32x4*)(xr[t] + (rest < pitch ? rest : 0)) : bytes16(xr[t], rest, a.cols), acc[t], 0, 0, 0);
+        for (int t = 0; t < MT; ++t) x[t] = FUSED ? *(const i32x4*)(xr[t] + (rest < pitch ? rest : 0)) : bytes16(xr[t], rest, a.cols);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const i32x4 v = rest + 16 > a.cols ? bytes16(wr[i], rest, a.cols) : i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, x[t], acc[i][t], 0, 0, 0);
+        }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) joint[wave][t][lane] = acc[t];
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) joint[wave][i][t][lane] = acc[i][t];
     __syncthreads();
     Scales s = a.s;
     if (FUSED) s.x = scales;
-    for (int t = turn; t < MT; t += a.share) {
+    for (int f = turn; f < CT * MT; f += a.share) {
+        const int i = f / MT, t = f % MT;
         i32x4 sum = {};
-        for (int v = 0; v < a.share; ++v) sum += joint[wave - turn + v][t][lane];
-        finish4<DT>(s, t * 16 + (lane & 15), m0 + (lane >> 4) * 4, sum);
+        for (int v = 0; v < a.share; ++v) sum += joint[wave - turn + v][i][t][lane];
+        finish4<DT>(s, t * 16 + (lane & 15), m0 + i * 16 + (lane >> 4) * 4, sum);
     }
 }
 
@@ -532,18 +551,19 @@ void run_tiles(const TileArgs& t, hipStream_t st) {
 // then smallest.
 template <int DT, int DX>
 int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, hipStream_t st) {
-    const int64_t groups = (a.channels + 15) / 16;
-    int share = 16;
-    while (share > 1 && groups * share / 16 >= 512) share /= 2;
-    const FewArgs f{(const int8_t*)a.weight, x, a.weight_pitch, x_pitch, (int)a.features, share, s};
-    const dim3 grid((unsigned)((groups * share + 15) / 16)), block(1024);
-    if constexpr (DX != DT_I8) {
-        hipLaunchKernelGGL((k_int8_few<DT, DX, 1>), grid, block, 0, st, f);
-    } else {
-        if (a.tokens <= 16) hipLaunchKernelGGL((k_int8_few<DT, DX, 1>), grid, block, 0, st, f);
-        else if (a.tokens <= 32) hipLaunchKernelGGL((k_int8_few<DT, DX, 2>), grid, block, 0, st, f);
-        else if (a.tokens <= 48) hipLaunchKernelGGL((k_int8_few<DT, DX, 3>), grid, block, 0, st, f);
-        else hipLaunchKernelGGL((k_int8_few<DT, DX, 4>), grid, block, 0, st, f);
+    auto run = [&](auto tokens) {
+        constexpr int MT = decltype(tokens)::value, WIDE = 16 * few_fragments(DX != DT_I8, MT);
+        const int64_t groups = (a.channels + WIDE - 1) / WIDE;
+        int share = 16;
+        while (share > 1 && groups * share / 16 >= 512) share /= 2;
+        const FewArgs f{(const int8_t*)a.weight, x, a.weight_pitch, x_pitch, (int)a.features, share, s};
+        hipLaunchKernelGGL((k_int8_few<DT, DX, MT>), dim3((unsigned)((groups * share + 15) / 16)), dim3(1024), 0, st, f);
+    };
+    if (DX != DT_I8 || a.tokens <= 16) run(std::integral_constant<int, 1>{});
+    else if constexpr (DX == DT_I8) {
+        if (a.tokens <= 32) run(std::integral_constant<int, 2>{});
+        else if (a.tokens <= 48) run(std::integral_constant<int, 3>{});
+        else run(std::integral_constant<int, 4>{});
     }
     return launched("k_int8_few");
 }
