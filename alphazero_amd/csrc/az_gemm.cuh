@@ -288,4 +288,29 @@ __device__ __forceinline__ void mm_place(int id, int tiles_p, int tiles_q, int& 
     tq = in / width;
 }
 
+// ---- host: which tile -----------------------------------------------------------------------------------------------------
+// What the tiles were measured to take, in microseconds: a step (128 bytes of k), and a tile beside its steps (first loads, results), with as
+// many of them on a compute unit at a time as its LDS holds. 4096 x 722 -> 362 float16 dense: 64 tiles 14.8 (logits) and 17.1 us (G), 128
+// tiles 22.1 and 32.4; 7955 x 3877 -> 829: 128 tiles 79; 809 x 437 -> 20359: 256 tiles 37 and 54, 128 tiles 37 and 48.
+struct MmTileCost {
+    int edge, at_once;
+    double step, rest;
+};
+constexpr MmTileCost MM_TILE_COSTS[3] = {{256, 1, 1.5, 8.0}, {128, 2, 1.1, 6.0}, {64, 2, 0.8, 4.0}};
+
+// Tile edge for p x q results of sums over `steps` steps: rounds of tiles over the compute units, times a tile.
+inline int mm_tile_edge(int64_t p, int64_t q, int64_t steps) {
+    int best = 256;
+    double least = 1e300;
+    for (const MmTileCost& c : MM_TILE_COSTS) {
+        const int64_t tiles = ((p + c.edge - 1) / c.edge) * ((q + c.edge - 1) / c.edge), round = 256 * c.at_once;
+        const double t = (double)((tiles + round - 1) / round) * (steps * c.step + c.rest);
+        if (t < least) {
+            least = t;
+            best = c.edge;
+        }
+    }
+    return best;
+}
+
 }  // namespace az

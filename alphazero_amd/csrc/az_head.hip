@@ -841,30 +841,6 @@ template <> struct Tiles<DT_BF16> : TilesOf<MM_BF16> {};
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// What a product takes, in microseconds, from what the tiles were measured to take: a step (64 of k) of a 256 tile 1.5 on its compute
-// unit, of a 128 tile 0.55 (two of them on a unit at a time), of a 64 tile 0.4; and what a tile takes beside its steps (first loads,
-// results), 8, 3 and 1.5.
-struct TileCost {
-    int edge;
-    double step, rest;
-};
-constexpr TileCost TILE_COSTS[3] = {{256, 1.5, 8.0}, {128, 0.55, 3.0}, {64, 0.4, 1.5}};
-
-// Tile edge for p x q results of sums over `steps` steps: rounds of tiles over the compute units, times a tile.
-int tile_edge(int64_t p, int64_t q, int64_t steps) {
-    int best = 256;
-    double least = 1e300;
-    for (const TileCost& c : TILE_COSTS) {
-        const int64_t tiles = ((p + c.edge - 1) / c.edge) * ((q + c.edge - 1) / c.edge);
-        const double t = (double)((tiles + 255) / 256) * (steps * c.step + c.rest);
-        if (t < least) {
-            least = t;
-            best = c.edge;
-        }
-    }
-    return best;
-}
-
 struct Layout {       // of the workspace, and the pieces of the classes
     bool few = false;   // the kernels of az_head_few.cuh
     int grid = 0, chunks = 0, chunk = 0;      // of those: workgroups; chunks of the classes, classes of a chunk
@@ -893,7 +869,7 @@ void operand_layout(const az_linear_ce_args& a, Layout& l) {
 }
 
 int64_t logit_steps(const az_linear_ce_args& a) { return (a.features + 63) / 64 * (a.dtype == AZ_DT_F32 ? MM_SEGMENTS : 1); }
-int forward_edge(const az_linear_ce_args& a) { return tile_edge(a.classes, a.rows, logit_steps(a)); }
+int forward_edge(const az_linear_ce_args& a) { return mm_tile_edge(a.classes, a.rows, logit_steps(a)); }
 
 // Waves of a workgroup that split the features of the same classes: each keeps eight turns of loads, unless more splitting makes a
 // workgroup for every half compute unit.
@@ -975,7 +951,7 @@ OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
     double least = 1e300;
     const int walks = l.split ? MM_SEGMENTS : 1;
     const int64_t steps_x = round_up(nv, 64) / 64 * walks, steps_w = round_up(a.rows, 64) / 64 * walks;
-    for (const TileCost& c : TILE_COSTS) {
+    for (const MmTileCost& c : MM_TILE_COSTS) {
         OutPlan o;
         o.edge = c.edge;
         auto tiles = [&](int64_t n) { return (int)((n + o.edge - 1) / o.edge); };
@@ -993,8 +969,9 @@ OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
         split(o.x, steps_x, a.rows * a.features);
         split(o.w, steps_w, nv * a.features);
         const int64_t items = (int64_t)o.x.tiles_p * o.x.tiles_q * o.x.splits + (int64_t)o.w.tiles_p * o.w.tiles_q * o.w.splits;
-        const int64_t longest = o.x.per > o.w.per ? o.x.per : o.w.per, mean = total / 256 + 1;
-        const double t = (mean > longest ? mean : longest) * c.step + (double)((items + 255) / 256) * c.rest + (sums > 0.0 ? 5.0 + sums / 4.5e6 : 0.0);
+        const int64_t longest = o.x.per > o.w.per ? o.x.per : o.w.per;
+        const double all = (total * c.step + items * c.rest) / (256 * c.at_once), one = longest * c.step + c.rest;
+        const double t = (all > one ? all : one) + (sums > 0.0 ? 5.0 + sums / 4.5e6 : 0.0);
         if (t < least) {
             least = t;
             best = o;
@@ -1286,7 +1263,7 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         s.g_plane = a.rows * vpi * 2;
         s.v0 = (int)v0;
         s.db_pitch = nv;
-        const int edge = tile_edge(nv, a.rows, logit_steps(a));
+        const int edge = mm_tile_edge(nv, a.rows, logit_steps(a));
         s.tiles_p = (int)((nv + edge - 1) / edge);
         s.tiles_q = (int)((a.rows + edge - 1) / edge);
         const bool d = a.target_dense, e = a.entropy_coeff != 0.0f;
