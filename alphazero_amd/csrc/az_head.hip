@@ -544,11 +544,12 @@ __device__ __forceinline__ float hold_scale(const float* scalars) {
 }
 
 // Largest |gradient| of the rows, for one gradient per row.
-__global__ __launch_bounds__(1024) void k_ce_largest(const float* grad, int rows, float* out) {
+__global__ __launch_bounds__(1024) void k_ce_largest(const float* grad, Rows t, float* out) {
     __shared__ float tops[16];
     float top = 0.0f;
     auto see = [&](float g) { top = g > top || g != g ? g : top; };      // a NaN stays
-    for (int n = threadIdx.x; n < rows; n += 1024) see(fabsf(grad[n]));
+    for (int n = threadIdx.x; n < t.rows; n += 1024)
+        if (!(t.index && t.index[n] == t.ignore)) see(fabsf(grad[n]));      // the gradient of a row that does not count may be anything
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) see(__shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
@@ -563,6 +564,8 @@ struct Factor {
     const float *grad, *scalars, *largest;   // largest: one gradient per row
     int32_t mean, half;                      // half: G is held times hold_scale
     const float* un;                         // float32: what the other operand was divided by, or null
+    const int64_t* index;                    // rows that do not count get 0, whatever their gradient
+    int64_t ignore;
 };
 __device__ __forceinline__ float factor_all(const Factor& f) {            // dW, db, and dx with one factor
     float v = f.largest ? *f.largest : f.grad[0];
@@ -571,6 +574,7 @@ __device__ __forceinline__ float factor_all(const Factor& f) {            // dW,
     return f.half ? v / hold_scale(f.scalars) : v;
 }
 __device__ __forceinline__ float factor_row(const Factor& f, int64_t n) {  // dx with one factor per row
+    if (f.index && f.index[n] == f.ignore) return 0.0f;
     const float v = f.un ? f.grad[n] * *f.un : f.grad[n];
     return f.half ? v / hold_scale(f.scalars) : v;
 }
@@ -621,7 +625,7 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
             if constexpr (DENSE) total = a.tsum[n];
             else target = a.t.index[n];
             counts = DENSE || target != a.t.ignore;
-            if (a.f.largest) share[j] = *a.f.largest > 0.0f || *a.f.largest != *a.f.largest ? a.f.grad[n] / *a.f.largest : 0.0f;
+            if (a.f.largest) share[j] = counts && (*a.f.largest > 0.0f || *a.f.largest != *a.f.largest) ? a.f.grad[n] / *a.f.largest : 0.0f;
             if (!DENSE && (target < 0 || target >= a.t.classes)) f = NAN;
         }
         const Reference at(ref);
@@ -1227,8 +1231,9 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     const int64_t np = round_up(a.rows, 64), vp = round_up(l.piece, 64);
     const bool each = a.reduction == AZ_REDUCE_NONE;
     const float *un_x = l.split ? kept.scalars + 2 : nullptr, *un_w = l.split ? kept.scalars + 3 : nullptr;
-    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT != DT_BF16, nullptr};
-    if (each) hipLaunchKernelGGL(k_ce_largest, dim3(1), dim3(1024), 0, st, grad, (int)a.rows, (float*)(ws + l.largest));
+    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT != DT_BF16, nullptr, a.target_dense ? nullptr : (const int64_t*)a.target,
+                   a.ignore_index};
+    if (each) hipLaunchKernelGGL(k_ce_largest, dim3(1), dim3(1024), 0, st, grad, rows_of(a), (float*)(ws + l.largest));
     GradArgs s{};
     s.t = rows_of(a);
     s.bias = a.bias;

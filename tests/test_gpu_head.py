@@ -130,8 +130,14 @@ def test_rows_that_do_not_count_may_hold_anything(dtype, rows):
     x[out[0]], x[out[1]], x[out[2], 3] = float("nan"), float("inf"), -float("inf")
     got = _check(x, w, b, t, c=0.01)
     assert (got[3][out] == 0).all()
-    none = _run(x, w, b, t, reduction="none")
-    assert (none[0][out] == 0).all()
+    g = torch.linspace(0.5, 1.5, rows, device="cuda")
+    g[out] = float("nan")                                # nor may their gradients matter
+    none = _run(x, w, b, t, g, reduction="none")
+    assert (none[0][out] == 0).all() and (none[3][out] == 0).all()
+    assert all(torch.isfinite(v).all() for v in none[3:])
+    g[out] = 0.0
+    for a, v in zip(none, _run(x, w, b, t, g, reduction="none")):
+        assert torch.equal(a, v)
 
 
 def test_no_row_counts():
