@@ -6,7 +6,6 @@ They take GPU tensors of float32, bfloat16 or float16 and run on the current str
 fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -16,7 +15,6 @@ from torch.autograd.function import once_differentiable
 from . import _native as N
 
 _DTYPES = {torch.float32: N.AZ_DT_F32, torch.bfloat16: N.AZ_DT_BF16, torch.float16: N.AZ_DT_F16}
-_HERE = contextlib.nullcontext()
 _REDUCE = {"none": N.AZ_REDUCE_NONE, "mean": N.AZ_REDUCE_MEAN, "sum": N.AZ_REDUCE_SUM}
 
 
@@ -50,16 +48,22 @@ def _pitch(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
-def _device(device):
-    """The device made current for native calls; nothing to do where it already is."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object around it: 0.1 for 2 us
+# torch.cuda.current_device and current_stream without their checks and objects: 0.1 instead of 0.5 to 3 us of host time each
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream(device) -> int:
     return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _native(device, name: str, *args) -> int:
+    """A call of the library with `device` as the current one."""
+    fn = getattr(N.lib(), name)
+    if _current_device() == device.index:
+        return N.check(fn(*args), name)
+    with torch.cuda.device(device):
+        return N.check(fn(*args), name)
 
 
 def _scratch(size: int, device) -> torch.Tensor:
@@ -81,11 +85,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         shape = (rows,) if reduction == "none" else ()
         out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
         kept = torch.empty(4 * rows + 4, dtype=torch.float32, device=dev)
-        L = N.lib()
-        with _device(dev):
-            ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 0), "az_linear_ce_workspace"), dev)
-            N.check(L.az_linear_ce_forward(C.byref(a), kept.data_ptr(), out[0].data_ptr(), out[1].data_ptr() if parts else None,
-                                           out[2].data_ptr() if parts else None, ws.data_ptr(), ws.numel(), _stream(dev)), "az_linear_ce_forward")
+        r = C.byref(a)
+        size = N.check(N.lib().az_linear_ce_workspace(r, 0), "az_linear_ce_workspace")
+        ws = _scratch(size, dev)
+        _native(dev, "az_linear_ce_forward", r, kept.data_ptr(), out[0].data_ptr(), out[1].data_ptr() if parts else None,
+                out[2].data_ptr() if parts else None, ws.data_ptr(), size, _stream(dev))
         ctx.save_for_backward(x, weight, bias, target, kept)
         ctx.args = (ignore_index, reduction, entropy_coeff)
         if parts:
@@ -106,11 +110,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
         gb = torch.empty(bias.shape, dtype=x.dtype, device=dev) if bias is not None and need_b else None
-        L = N.lib()
-        with _device(dev):
-            ws = _scratch(N.check(L.az_linear_ce_workspace(C.byref(a), 1), "az_linear_ce_workspace"), dev)
-            N.check(L.az_linear_ce_backward(C.byref(a), kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), ws.numel(),
-                                            _stream(dev)), "az_linear_ce_backward")
+        r = C.byref(a)
+        size = N.check(N.lib().az_linear_ce_workspace(r, 1), "az_linear_ce_workspace")
+        ws = _scratch(size, dev)
+        _native(dev, "az_linear_ce_backward", r, kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), size, _stream(dev))
         return gx, gw, gb, None, None, None, None, None
 
 
@@ -176,10 +179,10 @@ class _Dropout(torch.autograd.Function):
 
 
 def _dropout(x, residual, seed_tensor, threshold, seed, offset):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _device(x.device):
-        N.check(N.lib().az_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], threshold, seed,
-                                   _ptr(seed_tensor), offset, _stream(x.device)), "az_dropout")
+    y = torch.empty_like(x)      # contiguous, as x is here
+    dev = x.device
+    _native(dev, "az_dropout", x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], threshold, seed, _ptr(seed_tensor), offset,
+            _stream(dev))
     return y
 
 
@@ -221,9 +224,8 @@ def quantize_rows(x):
     x2 = _rows(x.detach())
     q = torch.empty(x2.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
-    with _device(x.device):
-        N.check(N.lib().az_quantize_rows(x2.data_ptr(), _DTYPES[x.dtype], x2.shape[0], x2.shape[1], _pitch(x2), q.data_ptr(), q.shape[1],
-                                         scale.data_ptr(), _stream(x.device)), "az_quantize_rows")
+    _native(x.device, "az_quantize_rows", x2.data_ptr(), _DTYPES[x.dtype], x2.shape[0], x2.shape[1], _pitch(x2), q.data_ptr(), q.shape[1],
+            scale.data_ptr(), _stream(x.device))
     return q.reshape(x.shape), scale.reshape(x.shape[:-1])
 
 
@@ -242,7 +244,8 @@ def int8_linear(x, qweight, weight_scale, bias=None, *, x_scale=None, out_dtype=
             and (bias is None or (bias.dtype in _DTYPES and bias.shape == (channels,))) and whole == (x_scale is not None)
             and (x_scale is None or (x_scale.dtype == torch.float32 and x_scale.shape == shape[:-1])) and (out_dtype is None or out_dtype in _DTYPES)):
         _int8_refuse(x, qweight, weight_scale, bias, x_scale, out_dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (x_scale is not None and x_scale.requires_grad)):
         raise ValueError("int8_linear has no gradient: call it under torch.no_grad() or with detached tensors")
     out_dtype = out_dtype or (torch.float32 if whole else x.dtype)
     dev = x.device
@@ -254,11 +257,10 @@ def int8_linear(x, qweight, weight_scale, bias=None, *, x_scale=None, out_dtype=
     b = None if bias is None else bias.contiguous()
     a = N.AzInt8Args(x2.data_ptr(), w.data_ptr(), _ptr(scale), wscale.data_ptr(), _ptr(b), y.data_ptr(), x2.shape[0], features, channels, _pitch(x2),
                      _pitch(w), N.AZ_DT_I8 if whole else _DTYPES[x.dtype], 0 if b is None else _DTYPES[b.dtype], _DTYPES[out_dtype])
-    L = N.lib()
-    with _device(dev):
-        size = N.check(L.az_int8_workspace(C.byref(a)), "az_int8_workspace")
-        ws = _scratch(size, dev) if size else None
-        N.check(L.az_int8_linear(C.byref(a), _ptr(ws), size, _stream(dev)), "az_int8_linear")
+    r = C.byref(a)
+    size = N.check(N.lib().az_int8_workspace(r), "az_int8_workspace")
+    ws = _scratch(size, dev) if size else None
+    _native(dev, "az_int8_linear", r, _ptr(ws), size, _stream(dev))
     return y
 
 
