@@ -6,8 +6,8 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = ["az_engine.hip", "az_net.hip", "az_net_mfma.hip", "az_net_layers.hip", "az_replay.hip", "az_head.hip", "az_dropout.hip", "az_int8.hip", "az_hostrng.cpp"]
-HDR = ["az_board.cuh", "az_net.h", "az_mfma_gemm.cuh", "az_lane.cuh", "az_gemm.cuh", "az_head_few.cuh", "az_types.cuh", "../../include/azamd.h"]
+SRC = ["az_engine.hip", "az_net.hip", "az_net_mfma.hip", "az_net_layers.hip", "az_replay.hip", "az_head_f32.hip", "az_head_bf16.hip", "az_head_f16.hip", "az_head.hip", "az_dropout.hip", "az_int8.hip", "az_hostrng.cpp"]
+HDR = ["az_board.cuh", "az_net.h", "az_mfma_gemm.cuh", "az_lane.cuh", "az_gemm.cuh", "az_head.cuh", "az_head_few.cuh", "az_types.cuh", "../../include/azamd.h"]
 # -ffp-contract=off: the search kernels must round every float64 product and sum separately.
 # -packed-fp32-ops: no packed float32 instructions, some forms of which have given wrong results now and then. The host pass does not
 # know the feature and says so; that is harmless.

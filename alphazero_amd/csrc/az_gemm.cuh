@@ -1,4 +1,4 @@
-// Tile loop of the matrix products of the head operators (az_head.hip, az_int8.hip): C[p][q] = sum_k P[p][k] * Q[q][k], both
+// Tile loop of the matrix products of the head operators (az_head.cuh, az_int8.hip): C[p][q] = sum_k P[p][k] * Q[q][k], both
 // operands with k contiguous, 16-bit floats or 8-bit integers, accumulated in 32 bits.
 //
 // A workgroup owns BP x BQ results and walks k in steps of 128 bytes (64 16-bit or 128 8-bit values). A step's BP + BQ rows of

@@ -5,7 +5,7 @@
 // 1 x 4096 -> 131072 bfloat16: 200 us (5.3 TB/s); 5 x 3765 -> 52111 float32: 200 us (3.9 TB/s).
 // Backward: the logits are made again the same way and become G [classes][16] in float32; then one pass reads the weight, adds G W
 // to dx in registers and writes dW = G^T x. That is three reads of the weight in all and one write of its gradient.
-// Included by az_head.hip.
+// Included by az_head.cuh.
 #pragma once
 
 namespace az {
