@@ -85,11 +85,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         shape = (rows,) if reduction == "none" else ()
         out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
         kept = torch.empty(4 * rows + 4, dtype=torch.float32, device=dev)
-        r = C.byref(a)
-        size = N.check(N.lib().az_linear_ce_workspace(r, 0), "az_linear_ce_workspace")
-        ws = _scratch(size, dev)
-        _native(dev, "az_linear_ce_forward", r, kept.data_ptr(), out[0].data_ptr(), out[1].data_ptr() if parts else None,
-                out[2].data_ptr() if parts else None, ws.data_ptr(), size, _stream(dev))
+        if rows:
+            r = C.byref(a)
+            size = N.check(N.lib().az_linear_ce_workspace(r, 0), "az_linear_ce_workspace")
+            ws = _scratch(size, dev)
+            _native(dev, "az_linear_ce_forward", r, kept.data_ptr(), out[0].data_ptr(), out[1].data_ptr() if parts else None,
+                    out[2].data_ptr() if parts else None, ws.data_ptr(), size, _stream(dev))
+        else:       # an empty sum, a mean of nothing
+            for o in out:
+                o.fill_(float("nan") if reduction == "mean" else 0.0)
         ctx.save_for_backward(x, weight, bias, target, kept)
         ctx.args = (ignore_index, reduction, entropy_coeff)
         if parts:
@@ -110,6 +114,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
         gb = torch.empty(bias.shape, dtype=x.dtype, device=dev) if bias is not None and need_b else None
+        if not x.shape[0]:
+            for g in (gw, gb):
+                if g is not None:
+                    g.zero_()
+            return gx, gw, gb, None, None, None, None, None
         r = C.byref(a)
         size = N.check(N.lib().az_linear_ce_workspace(r, 1), "az_linear_ce_workspace")
         ws = _scratch(size, dev)
@@ -150,10 +159,6 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
         _need(target.shape == lead, f"target {tuple(target.shape)} does not fit {tuple(lead)}")
         target = target.reshape(-1).contiguous()
     x2 = _rows(x)
-    if x2.shape[0] == 0:      # no rows: an empty sum, a mean of nothing
-        zero = (x2.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
-        one = x2.new_zeros(lead, dtype=torch.float32) + zero if reduction == "none" else zero / 0 if reduction == "mean" else zero
-        return (one, one.detach(), one.detach()) if parts else one
     out = _LinearCrossEntropy.apply(x2, _rows(weight), bias if bias is None else bias.contiguous(), target, int(ignore_index), reduction,
                                     float(entropy_coeff), bool(parts))
     if reduction == "none" and len(lead) != 1:

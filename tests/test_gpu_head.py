@@ -310,6 +310,25 @@ def test_no_rows():
     assert head.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_no_rows_look_at_no_weights(reduction, dense):
+    """Without rows the weights have no part in the result, whatever they hold: infinities, or values whose sum leaves float16."""
+    head = _head()
+    for fill in (float("inf"), 65504.0):
+        x = torch.empty(0, 9, dtype=F16, device="cuda", requires_grad=True)
+        w = torch.full((50, 9), fill, dtype=F16, device="cuda", requires_grad=True)
+        b = torch.full((50,), fill, dtype=F16, device="cuda", requires_grad=True)
+        t = torch.empty(0, 50, device="cuda") if dense else torch.empty(0, dtype=torch.int64, device="cuda")
+        loss, ce, ent = head.linear_cross_entropy(x, w, t, b, reduction=reduction, parts=True)
+        for v in (loss, ce, ent):
+            assert v.shape == ((0,) if reduction == "none" else ()) and v.dtype == F32
+            assert torch.isnan(v).all() if reduction == "mean" else not v.any()
+        assert not ce.requires_grad
+        loss.sum().backward()
+        assert x.grad.shape == (0, 9) and not w.grad.any() and not b.grad.any()
+
+
 # ------------------------------------------------------------------------------------------------ dropout
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 @pytest.mark.parametrize("count", [1, 7, 8, 9, 255, 2048, 2049, 100003])
