@@ -48,6 +48,7 @@ struct DropArgs {
     uint64_t seed, offset;
     uint32_t threshold;
     float scale;
+    int64_t first;              // group of the launch's first thread
 };
 
 template <int DT>
@@ -65,7 +66,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
 
 template <int DT, bool RES, bool WIDE>
 __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
-    const int64_t group = (int64_t)blockIdx.x * 256 + threadIdx.x, i = group * 8;
+    const int64_t group = a.first + (int64_t)blockIdx.x * 256 + threadIdx.x, i = group * 8;
     if (i >= a.count) return;
     uint32_t w[4];
     const bool whole = WIDE && i + 8 <= a.count;
@@ -98,15 +99,20 @@ __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
 }
 
 template <int DT>
-void launch(const DropArgs& a, hipStream_t st) {
+void launch(DropArgs a, hipStream_t st) {
     const bool wide = (((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.residual) & 15) == 0;
-    const dim3 grid((unsigned)((a.count + 2047) / 2048)), block(256);
-    if (a.residual) {
-        if (wide) hipLaunchKernelGGL((k_dropout<DT, true, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_dropout<DT, true, false>), grid, block, 0, st, a);
-    } else {
-        if (wide) hipLaunchKernelGGL((k_dropout<DT, false, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_dropout<DT, false, false>), grid, block, 0, st, a);
+    constexpr int64_t MOST = int64_t(1) << 34;      // elements of a launch, which holds fewer than 2^32 threads
+    for (int64_t i = 0; i < a.count; i += MOST) {
+        a.first = i / 8;
+        const int64_t n = a.count - i < MOST ? a.count - i : MOST;
+        const dim3 grid((unsigned)((n + 2047) / 2048)), block(256);
+        if (a.residual) {
+            if (wide) hipLaunchKernelGGL((k_dropout<DT, true, true>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((k_dropout<DT, true, false>), grid, block, 0, st, a);
+        } else {
+            if (wide) hipLaunchKernelGGL((k_dropout<DT, false, true>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((k_dropout<DT, false, false>), grid, block, 0, st, a);
+        }
     }
 }
 
@@ -122,7 +128,7 @@ extern "C" int az_dropout(const void* x, const void* residual, void* y, int64_t 
     if (count < 0 || count > (int64_t(1) << 40)) return fail(AZ_ERR_ARG, "count is 0..2^40");
     if (count == 0) return AZ_OK;
     if (!x || !y) return fail(AZ_ERR_ARG, "null argument");
-    const DropArgs a{x, residual, y, count, seed_dev, seed, offset, (uint32_t)threshold, threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f};
+    const DropArgs a{x, residual, y, count, seed_dev, seed, offset, (uint32_t)threshold, threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f, 0};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == AZ_DT_F32) launch<DT_F32>(a, st);
     else if (dtype == AZ_DT_BF16) launch<DT_BF16>(a, st);

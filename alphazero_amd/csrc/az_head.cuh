@@ -928,13 +928,16 @@ Layout forward_layout(const az_linear_ce_args& a) {
         return l;
     }
     operand_layout(a, l);
-    // a packed piece of the weight stays below 512 MB
-    int64_t piece = a.classes;
-    if (l.pack_w) piece = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
+    const int64_t edge = forward_edge(a), tiles = (a.classes + edge - 1) / edge;
+    // A launch holds fewer than 2^32 threads, a tile 512 at most; a packed piece of the weight stays below 512 MB. Pieces start at tiles.
+    int64_t piece = (int64_t(1) << 22) / ((a.rows + edge - 1) / edge) * edge;
+    if (l.pack_w) {
+        const int64_t w = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
+        if (w < piece) piece = w;
+    }
     l.piece = piece < 256 ? 256 : piece;
     if (l.piece > a.classes) l.piece = a.classes;
     l.pieces = (int)((a.classes + l.piece - 1) / l.piece);
-    const int64_t edge = forward_edge(a), tiles = (a.classes + edge - 1) / edge;
     if (l.pack_x) l.xp = l.take(a.rows * l.kpitch * l.planes);
     if (l.pack_w) l.wp = l.take(l.piece * l.kpitch * l.planes);
     if (l.split) {
@@ -1052,6 +1055,7 @@ int check_args(const az_linear_ce_args* a) {
     if (a->rows < 1 || a->features < 1 || a->classes < 1) return fail(AZ_ERR_ARG, "rows, features and classes are at least 1");
     if (a->rows > (1 << 30) || a->classes > (1 << 30)) return fail(AZ_ERR_ARG, "rows and classes are at most 2^30");
     if (a->features * 2 > MM_MAX_PITCH - 16 || a->rows * 2 > MM_MAX_PITCH - 128) return fail(AZ_ERR_ARG, "features and rows are at most 4194000");
+    if (a->rows * a->features > (int64_t(1) << 34)) return fail(AZ_ERR_ARG, "rows times features are at most 2^34");
     if (!a->x || !a->weight || !a->target) return fail(AZ_ERR_ARG, "null argument");
     if (a->x_pitch < a->features || a->weight_pitch < a->features || (a->target_dense && a->target_pitch < a->classes))
         return fail(AZ_ERR_ARG, "a row stride is smaller than the row");

@@ -460,6 +460,8 @@ __global__ __launch_bounds__(1024) void k_int8_few(FewArgs a) {
 typedef MmTile<256, 256, 2, 4, 2, MM_I8> Big;
 typedef MmTile<128, 128, 2, 2, 2, MM_I8> Mid;
 typedef MmTile<64, 64, 2, 2, 4, MM_I8> Small;
+constexpr int MOST_THREADS = Big::THREADS;
+static_assert(Mid::THREADS <= MOST_THREADS && Small::THREADS <= MOST_THREADS, "");
 
 struct Plan {
     bool few, fused, align_w, align_x;
@@ -512,7 +514,7 @@ int check_args(const az_int8_args* a) {
     for (const int32_t d : {a->y_dtype, a->bias ? a->bias_dtype : (int32_t)AZ_DT_F32})
         if (d != AZ_DT_F32 && d != AZ_DT_BF16 && d != AZ_DT_F16) return fail(AZ_ERR_ARG, "the output and the bias are float32, bfloat16 or float16");
     if (a->tokens < 1 || a->features < 1 || a->channels < 1) return fail(AZ_ERR_ARG, "tokens, features and channels are at least 1");
-    if (a->tokens > (1 << 30) || a->channels > (1 << 30)) return fail(AZ_ERR_ARG, "tokens and channels are at most 2^30");
+    if (a->tokens > (1 << 30) || a->channels > (1 << 27)) return fail(AZ_ERR_ARG, "tokens are at most 2^30, channels 2^27");
     if (a->features > 131071) return fail(AZ_ERR_ARG, "features are at most 131071: 2^31 / 128^2 products fill a 32-bit sum");
     if (!a->x || !a->weight || !a->weight_scale || !a->y || (a->x_dtype == AZ_DT_I8 && !a->x_scale)) return fail(AZ_ERR_ARG, "null argument");
     if (a->x_pitch < a->features || a->weight_pitch < a->features) return fail(AZ_ERR_ARG, "a row stride is smaller than the row");
@@ -527,13 +529,25 @@ int launched(const char* what) {
 
 // 256 threads hold rows of up to 32 KB, 1024 of up to 128 KB (256 x 23104 float32: 8.5 us, with 256 threads and a second read 14.9 us).
 template <int DT>
-void quantize_as(const QuantArgs& q, hipStream_t st) {
+void launch_quantize(const QuantArgs& q, hipStream_t st) {
     const dim3 grid((unsigned)q.rows);
     const int64_t bytes = (int64_t)q.cols * (DT == DT_F32 ? 4 : 2);
     if (bytes <= 8192) hipLaunchKernelGGL((k_quantize<DT, 256, 2>), grid, dim3(256), 0, st, q);
     else if (bytes <= 16384) hipLaunchKernelGGL((k_quantize<DT, 256, 4>), grid, dim3(256), 0, st, q);
     else if (bytes <= 32768) hipLaunchKernelGGL((k_quantize<DT, 256, 8>), grid, dim3(256), 0, st, q);
     else hipLaunchKernelGGL((k_quantize<DT, 1024, 8>), grid, dim3(1024), 0, st, q);
+}
+template <int DT>
+void quantize_as(const QuantArgs& q, hipStream_t st) {
+    constexpr int64_t MOST = int64_t(1) << 21;      // rows of a launch, which holds fewer than 2^32 threads
+    for (int64_t r = 0; r < q.rows; r += MOST) {
+        QuantArgs part = q;
+        part.x = (const char*)q.x + r * q.pitch * (DT == DT_F32 ? 4 : 2);
+        part.q += r * q.q_pitch;
+        part.scale += r;
+        part.rows = q.rows - r < MOST ? q.rows - r : MOST;
+        launch_quantize<DT>(part, st);
+    }
 }
 void quantize(int dtype, const QuantArgs& q, hipStream_t st) {
     if (dtype == AZ_DT_F32) quantize_as<DT_F32>(q, st);
@@ -581,7 +595,12 @@ int product(const az_int8_args& a, const Plan& p, const int8_t* x, int64_t x_pit
     const int8_t* w = (const int8_t*)a.weight;
     int64_t w_pitch = a.weight_pitch;
     auto align = [&](const int8_t* src, int64_t pitch, int64_t rows, int64_t at) {
-        hipLaunchKernelGGL(k_align, dim3((unsigned)((rows * (p.kpitch >> 4) + 255) / 256)), dim3(256), 0, st, src, pitch, rows, (int)a.features, (int8_t*)(ws + at), p.kpitch);
+        const int64_t most = (int64_t(1) << 31) / (p.kpitch >> 4);      // rows of a launch, which holds fewer than 2^32 threads
+        for (int64_t r = 0; r < rows; r += most) {
+            const int64_t n = rows - r < most ? rows - r : most;
+            hipLaunchKernelGGL(k_align, dim3((unsigned)((n * (p.kpitch >> 4) + 255) / 256)), dim3(256), 0, st, src + r * pitch, pitch, n, (int)a.features,
+                               (int8_t*)(ws + at) + r * p.kpitch, p.kpitch);
+        }
     };
     if (p.align_w) {
         align(w, w_pitch, a.channels, p.w);
@@ -595,18 +614,25 @@ int product(const az_int8_args& a, const Plan& p, const int8_t* x, int64_t x_pit
     }
     TileArgs t{};
     t.w = MmOperand{(const char*)w, w_pitch, 0, (int)a.channels};
-    t.x = MmOperand{(const char*)x, x_pitch, 0, (int)a.tokens};
     t.s = s;
     t.kbytes = (int)p.kpitch;
     t.tiles_p = (int)((a.channels + p.edge - 1) / p.edge);
-    t.tiles_q = (int)((a.tokens + p.edge - 1) / p.edge);
     t.splits = p.splits;
     t.per = p.per;
     t.part = p.part >= 0 ? (i32x4*)(ws + p.part) : nullptr;
-    if (p.edge == 256) run_tiles<Big, DT>(t, st);
-    else if (p.edge == 128) run_tiles<Mid, DT>(t, st);
-    else run_tiles<Small, DT>(t, st);
-    if (t.splits > 1)
+    const int64_t most = ((int64_t(1) << 31) / MOST_THREADS / t.tiles_p) * p.edge;      // tokens of a launch, which holds fewer than 2^32 threads
+    for (int64_t r = 0; r < a.tokens; r += most) {
+        const int64_t n = a.tokens - r < most ? a.tokens - r : most;
+        t.x = MmOperand{(const char*)x + r * x_pitch, x_pitch, 0, (int)n};
+        t.s.x = s.x + r;
+        t.s.y = (char*)s.y + r * a.channels * (DT == DT_F32 ? 4 : 2);
+        t.s.tokens = (int)n;
+        t.tiles_q = (int)((n + p.edge - 1) / p.edge);
+        if (p.edge == 256) run_tiles<Big, DT>(t, st);
+        else if (p.edge == 128) run_tiles<Mid, DT>(t, st);
+        else run_tiles<Small, DT>(t, st);
+    }
+    if (t.splits > 1)      // few tiles, one launch
         hipLaunchKernelGGL((k_int8_join<Small, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * Small::FP * Small::FQ)), dim3(Small::THREADS), 0, st, t);
     return launched("k_int8_tile");
 }

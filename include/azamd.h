@@ -353,7 +353,7 @@ typedef struct {
     const void* weight;       /* [classes, features] of dtype */
     const void* bias;         /* [classes] of dtype, or NULL */
     const void* target;       /* int64 [rows], or float [rows, classes] with target_dense */
-    int64_t rows, features, classes;            /* at least 1; rows, classes <= 2^30, rows, features <= 4194000 */
+    int64_t rows, features, classes;            /* at least 1; classes <= 2^30, rows, features <= 4194000, rows * features <= 2^34 */
     int64_t x_pitch, weight_pitch, target_pitch;
     int64_t ignore_index;
     int32_t dtype;            /* AZ_DT_F32 / BF16 / F16 */
@@ -395,7 +395,7 @@ typedef struct {
     const float* weight_scale;  /* [channels] */
     const void* bias;         /* [channels] of bias_dtype, or NULL */
     void* y;                  /* [tokens, channels] of y_dtype, contiguous, 16-byte aligned */
-    int64_t tokens, features, channels;     /* at least 1; features <= 131071 */
+    int64_t tokens, features, channels;     /* at least 1; features <= 131071, tokens <= 2^30, channels <= 2^27 */
     int64_t x_pitch, weight_pitch;
     int32_t x_dtype, bias_dtype, y_dtype;
 } az_int8_args;

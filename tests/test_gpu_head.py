@@ -725,3 +725,73 @@ def test_int8_weights_beyond_4_gigabytes(tokens):
     y = head.int8_linear(x, w, ws)
     for i in (0, 262_144, 524_288, channels - 500):
         _int8_check(x, w[i:i + 500], ws[i:i + 500], None, y[:, i:i + 500], q, s)
+
+
+# ------------------------------------------------------------------------------------------------ more than one launch holds
+def test_dropout_of_more_than_one_launch():
+    """2^35 + 12345 elements in place: more threads than a launch holds."""
+    from alphazero_amd import _native as N
+    n, seed, offset, threshold = (1 << 35) + 12_345, 5, 3, 40_000
+    x = torch.ones(n, dtype=BF16, device="cuda")
+    N.check(N.lib().az_dropout(x.data_ptr(), None, x.data_ptr(), n, N.AZ_DT_BF16, threshold, seed, None, offset, torch.cuda.current_stream().cuda_stream),
+            "az_dropout")
+    scale = torch.tensor(65536.0 / (65536 - threshold), dtype=BF16)
+    for at in (0, (1 << 34) - 4096, (1 << 35) - 4096, n - 8000 - n % 8):
+        end = min(n, at + 8192)
+        c = np.arange(at // 8, (end + 7) // 8, dtype=np.uint64)
+        words = np.stack(R.philox_block((c & np.uint64(0xFFFFFFFF), c >> np.uint64(32), np.full_like(c, offset), np.zeros_like(c)), (seed, 0)), 1)
+        bits = np.stack((words & np.uint64(0xFFFF), words >> np.uint64(16)), 2).reshape(-1)[:end - at]
+        want = torch.where(torch.from_numpy(bits >= threshold), scale, torch.zeros((), dtype=BF16))
+        assert torch.equal(x[at:end].cpu(), want), at
+
+
+def test_quantize_rows_of_more_than_one_launch():
+    rows = (1 << 24) + 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((rows, 8), generator=g, device="cuda").to(BF16)
+    q, scale = _head().quantize_rows(x)
+    for i in range(0, rows, 1 << 22):
+        v = x[i:i + (1 << 22)].double()
+        top = v.abs().amax(1)
+        assert torch.equal(scale[i:i + (1 << 22)], (top / 127).float())      # torch's float32 division by a number is a product with 1 / 127
+        assert torch.equal(q[i:i + (1 << 22)].double(), torch.round(127 * v / top[:, None]))      # 127 v is exact; ties to even
+
+
+def test_int8_tokens_of_more_than_one_launch():
+    tokens, feats, channels = (1 << 28) + 77, 16, 3
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randint(-127, 128, (tokens, feats), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (channels, feats), generator=g, device="cuda", dtype=torch.int8)
+    xs = torch.rand(tokens, generator=g, device="cuda") + 0.5
+    ws = torch.tensor([1.0, 0.5, 2.0], device="cuda")
+    y = _head().int8_linear(x, w, ws, x_scale=xs)
+    for i in list(range(0, tokens, 1 << 24)):
+        sums = x[i:i + (1 << 24)].float() @ w.float().t()        # whole numbers below 2^24: exact
+        assert torch.equal(y[i:i + (1 << 24)], sums * xs[i:i + (1 << 24), None] * ws), i      # powers of two: one rounding
+
+
+def test_int8_weights_copied_in_more_than_one_launch():
+    channels, feats, tokens = (1 << 18) + 3, 131_057, 65
+    w = torch.empty((channels, feats), dtype=torch.int8, device="cuda")
+    w.random_(-127, 128, generator=torch.Generator(device="cuda").manual_seed(3))
+    x = torch.randint(-127, 128, (tokens, feats), device="cuda", dtype=torch.int8)
+    y = _head().int8_linear(x, w, torch.ones(channels, device="cuda"), x_scale=torch.ones(tokens, device="cuda"))
+    for i in (0, 131_072, channels - 259):
+        want = x.double() @ w[i:i + 259].double().t()
+        assert torch.equal(y[:, i:i + 259], want.float()), i
+
+
+def test_loss_of_more_tiles_than_one_launch():
+    """20000 x 13.6 million logits: more tiles than a launch holds."""
+    rows, feats, classes = 20_000, 8, 13_600_003
+    x, w = _large((rows, feats), 5, 1.5), _large((classes, feats), 6)
+    t = torch.randint(classes, (rows,), device="cuda")
+    t[0], t[1], t[-1] = classes - 1, 0, 13_591_552
+    with torch.no_grad():
+        loss = _head().linear_cross_entropy(x, w, t, reduction="none")
+        at = torch.cat([torch.arange(8, device="cuda"), torch.randint(rows, (48,), device="cuda"), torch.arange(rows - 8, rows, device="cuda")])
+        z = x[at].double() @ w.double().t()
+        want = torch.logsumexp(z, 1) - z[torch.arange(64), t[at]]
+    # logits of up to 60 in float32 and sums of 53125 parts: 60 * 2^-22 + 2^-20 of the loss
+    assert torch.isfinite(loss).all()
+    assert ((loss[at].double() - want).abs() <= 60 * 2.0 ** -22 + 2.0 ** -20 * want.abs()).all()

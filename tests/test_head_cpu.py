@@ -126,6 +126,19 @@ def test_c_entry_points_refuse():
     assert L.az_int8_linear(C.byref(a), None, size, None) == N.AZ_ERR_ARG and L.az_int8_linear(C.byref(a), 256, size - 1, None) == N.AZ_ERR_ARG
 
 
+def test_c_entry_points_refuse_what_no_launch_holds():
+    L = N.lib()
+    good = dict(x=256, weight=512, bias=None, target=768, rows=1 << 20, features=1 << 14, classes=3, x_pitch=1 << 15, weight_pitch=1 << 15, target_pitch=0,
+                ignore_index=-100, dtype=N.AZ_DT_BF16, target_dense=0, reduction=N.AZ_REDUCE_MEAN, entropy_coeff=0.0)
+    assert L.az_linear_ce_workspace(C.byref(N.AzLinearCeArgs(**good)), 0) > 0
+    assert L.az_linear_ce_workspace(C.byref(N.AzLinearCeArgs(**(good | dict(features=(1 << 14) + 1)))), 0) == N.AZ_ERR_ARG
+    good = dict(x=256, weight=512, x_scale=None, weight_scale=768, bias=None, y=1024, tokens=1 << 30, features=16, channels=1 << 27, x_pitch=16,
+                weight_pitch=16, x_dtype=N.AZ_DT_F32, bias_dtype=0, y_dtype=N.AZ_DT_F32)
+    assert L.az_int8_workspace(C.byref(N.AzInt8Args(**good))) > 0
+    for change in (dict(tokens=(1 << 30) + 1), dict(channels=(1 << 27) + 1)):
+        assert L.az_int8_workspace(C.byref(N.AzInt8Args(**(good | change)))) == N.AZ_ERR_ARG, change
+
+
 def test_generator_known_answers():
     """The published known answers of Philox4x32-10 (counters and keys of zeros, of ones, and of the digits of pi)."""
     def words(c, k):
