@@ -89,42 +89,46 @@ __device__ __forceinline__ void quantize_chunk(const float (&v)[NV], const Range
         u[w] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * w + 3], b[4 * w + 2], 0x0c0c0400u), __builtin_amdgcn_perm(b[4 * w + 1], b[4 * w], 0x0c0c0400u), 0x05040100u);
 }
 
-// One workgroup per row; HELD chunks per thread stay in registers between the maximum and the quotients, a longer row is read again
-// (from L2). Bound by memory: 8192 x 8192 bfloat16 in 50 us (4.0 TB/s).
-template <int DT, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS) void k_quantize(QuantArgs a) {
-    constexpr int NV = Chunk<DT>::N;
-    __shared__ uint32_t tops[THREADS / 64];
-    const int64_t row = blockIdx.x, base = row * a.pitch;
+// LANES threads per row (up to 64, or a workgroup), HELD chunks per thread stay in registers between the maximum and the quotients; a longer row is read again (from
+// L2). Up to 64 lanes the maximum needs no barrier. Bound by memory: 8192 x 8192 bfloat16 in 40 us (5.0 TB/s).
+template <int DT, int LANES, int HELD>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_quantize(QuantArgs a) {
+    static_assert(LANES <= 64 || LANES >= 256, "the waves of a row are a workgroup");
+    constexpr int NV = Chunk<DT>::N, THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
+    const int lane = threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES, base = row * a.pitch;
+    if (ROWS > 1 && row >= a.rows) return;
     uint32_t top = 0;
     float v[HELD][NV];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) load_chunk<DT>(a.x, base, (h * THREADS + threadIdx.x) * NV, a.cols, v[h]);
+    for (int h = 0; h < HELD; ++h) load_chunk<DT>(a.x, base, (h * LANES + lane) * NV, a.cols, v[h]);
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
 #pragma unroll
         for (int e = 0; e < NV; ++e) top = larger(top, v[h][e]);
-    for (int64_t c = (int64_t)(HELD * THREADS + threadIdx.x) * NV; c < a.cols; c += THREADS * NV) {
+    for (int64_t c = (int64_t)(HELD * LANES + lane) * NV; c < a.cols; c += LANES * NV) {
         float u[NV];
         load_chunk<DT>(a.x, base, c, a.cols, u);
 #pragma unroll
         for (int e = 0; e < NV; ++e) top = larger(top, u[e]);
     }
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, o));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
+    for (int o = 1; o < (LANES < 64 ? LANES : 64); o *= 2) top = larger(top, (uint32_t)__shfl_xor((int)top, o));
+    if constexpr (LANES > 64) {
+        __shared__ uint32_t tops[LANES / 64];
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) top = larger(top, tops[w]);
+        for (int w = 0; w < LANES / 64; ++w) top = larger(top, tops[w]);
+    }
     const Range range(top);
-    if (threadIdx.x == 0) a.scale[row] = range.scale();
-    const bool whole = (((uintptr_t)a.q | (uintptr_t)a.q_pitch) & (NV - 1)) == 0;
+    if (lane == 0) a.scale[row] = range.scale();
     auto store = [&](int64_t c, const float (&f)[NV]) {
         uint32_t u[NV / 4];
         quantize_chunk(f, range, u);
         int8_t* o = a.q + row * a.q_pitch + c;
-        if (whole && c + NV <= a.pad) {
-            __builtin_memcpy(__builtin_assume_aligned(o, NV), u, NV);
+        if (c + NV <= a.pad) {
+            __builtin_memcpy(o, u, NV);      // may start anywhere
         } else {
             for (int e = 0; e < NV; ++e)
                 if (c + e < a.pad) o[e] = (int8_t)(u[e >> 2] >> (8 * (e & 3)));
@@ -132,10 +136,10 @@ __global__ __launch_bounds__(THREADS) void k_quantize(QuantArgs a) {
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
-        const int64_t c = (h * THREADS + threadIdx.x) * NV;
+        const int64_t c = (h * LANES + lane) * NV;
         if (c < a.pad) store(c, v[h]);
     }
-    for (int64_t c = (int64_t)(HELD * THREADS + threadIdx.x) * NV; c < a.pad; c += THREADS * NV) {
+    for (int64_t c = (int64_t)(HELD * LANES + lane) * NV; c < a.pad; c += LANES * NV) {
         float u[NV];
         load_chunk<DT>(a.x, base, c, a.cols, u);
         store(c, u);
@@ -527,15 +531,30 @@ int launched(const char* what) {
     return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
-// 256 threads hold rows of up to 32 KB, 1024 of up to 128 KB (256 x 23104 float32: 8.5 us, with 256 threads and a second read 14.9 us).
+// Two to eight chunks per lane. From 2048 rows on a short row gets no more lanes than hold it (262144 x 64 bfloat16: 17 us, with 256 lanes
+// 270; 32768 x 2048: 40 against 54); with fewer rows more lanes are the shorter wait (256 x 2048: 3.6 us, with 64 lanes 5.4). 256 lanes
+// hold up to 32 KB, 1024 up to 128 KB (256 x 23104 float32: 8.5 us, with 256 lanes and a second read 14.9).
 template <int DT>
 void launch_quantize(const QuantArgs& q, hipStream_t st) {
-    const dim3 grid((unsigned)q.rows);
     const int64_t bytes = (int64_t)q.cols * (DT == DT_F32 ? 4 : 2);
-    if (bytes <= 8192) hipLaunchKernelGGL((k_quantize<DT, 256, 2>), grid, dim3(256), 0, st, q);
-    else if (bytes <= 16384) hipLaunchKernelGGL((k_quantize<DT, 256, 4>), grid, dim3(256), 0, st, q);
-    else if (bytes <= 32768) hipLaunchKernelGGL((k_quantize<DT, 256, 8>), grid, dim3(256), 0, st, q);
-    else hipLaunchKernelGGL((k_quantize<DT, 1024, 8>), grid, dim3(1024), 0, st, q);
+    auto run = [&](auto lanes, auto held) {
+        constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value, THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
+        hipLaunchKernelGGL((k_quantize<DT, LANES, HELD>), dim3((unsigned)((q.rows + ROWS - 1) / ROWS)), dim3(THREADS), 0, st, q);
+    };
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    const std::integral_constant<int, 256> wide;
+    const bool many = q.rows >= 2048;
+    if (many && bytes <= 256) run(eight, two);
+    else if (many && bytes <= 512) run(std::integral_constant<int, 16>{}, two);
+    else if (many && bytes <= 1024) run(std::integral_constant<int, 32>{}, two);
+    else if (many && bytes <= 2048) run(std::integral_constant<int, 64>{}, two);
+    else if (many && bytes <= 4096) run(std::integral_constant<int, 64>{}, four);
+    else if (bytes <= 8192) run(wide, two);
+    else if (bytes <= 16384) run(wide, four);
+    else if (bytes <= 32768) run(wide, eight);
+    else run(std::integral_constant<int, 1024>{}, eight);
 }
 template <int DT>
 void quantize_as(const QuantArgs& q, hipStream_t st) {

@@ -396,6 +396,25 @@ def test_quantize_rows(dtype, size):
     assert torch.equal(q.cpu(), rq) and torch.equal(s.cpu(), rs)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("size", [(2051, 1), (2048, 63), (2049, 129), (2050, 361), (3001, 513), (2053, 1025), (2047, 2048), (2055, 2047)], ids=ids)
+def test_quantize_many_short_rows(dtype, size):
+    """Rows that share a workgroup, of odd lengths and far apart; a row that is not finite and one of zeros stay their own affair."""
+    rows, cols = size
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    wide = (torch.randn((rows, cols + 3), generator=g, device="cuda") * 3).to(dtype)
+    x = wide[:, 1:cols + 1]
+    x[5], x[7, cols // 2], x[rows - 2, cols - 1] = 0.0, float("nan"), float("-inf")
+    q, scale = _head().quantize_rows(x)
+    v = x.double()
+    top = v.abs().amax(1)
+    good = torch.isfinite(top) & (top > 0)
+    assert torch.equal(scale[good], (top[good] / 127).float()) and scale[5] == 0 and torch.isnan(scale[[7, rows - 2]]).all()
+    assert not q[~good].any()
+    exact = torch.round(127 * v[good] / top[good, None])
+    assert torch.equal(q[good].double(), exact)
+
+
 def test_quantize_rows_near_halves_and_odd_values():
     head = _head()
     g = torch.Generator(device="cuda").manual_seed(2)
