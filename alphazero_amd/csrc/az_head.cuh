@@ -221,6 +221,13 @@ struct Rows {               // what a row's target says
     float entropy;          // c
 };
 
+// The walk over the features in `pieces` of `per` steps; with more than one, k_ce_walk leaves their products in part, [pieces][tiles] of what
+// the lanes of a tile hold.
+struct Walk {
+    int32_t pieces, per;
+    f32x4* part;
+};
+
 struct StatArgs {
     MmOperand w, x;
     Rows t;
@@ -234,13 +241,47 @@ struct StatArgs {
     float* tpart;           // dense: [rows][tiles][2] sum pi, sum |pi|
     float* zt;              // index: [rows] logit of the target
     int32_t tiles_p, tiles_q;
+    Walk walk;
 };
+
+// The small tile's products before anything is done to them, a piece of the features per workgroup: where rows and classes make few
+// tiles, one walk over the features would leave most of the chip idle (forward, 64 x 8192 -> 60 float32: 159 us in one walk, 41 in pieces;
+// 128 x 4096 -> 4096 bfloat16: 36 and 31).
+template <class T, int DT>
+__global__ __launch_bounds__(T::THREADS) void k_ce_walk(MmOperand w, MmOperand x, int kbytes, int tiles_p, int tiles_q, Walk walk) {
+    __shared__ __align__(16) char lds[T::LDS];
+    constexpr bool SPLIT = DT == DT_F32;
+    const int tiles = tiles_p * tiles_q, piece = blockIdx.x / tiles, tile = blockIdx.x % tiles, tp = tile % tiles_p, tq = tile / tiles_p;
+    const int steps = ((kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), begin = piece * walk.per;
+    typename T::acc_t acc[T::FP][T::FQ];
+    mm_tile<T>(w, x, (int64_t)tp * T::BP, (int64_t)tq * T::BQ, kbytes, begin, begin + walk.per < steps ? begin + walk.per : steps, SPLIT, lds, acc);
+    f32x4* const o = walk.part + (int64_t)blockIdx.x * (T::FP * T::FQ * T::THREADS) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < T::FQ; ++j) o[(i * T::FQ + j) * T::THREADS] = acc[i][j];
+}
 
 // The tile's logits in acc.
 template <class T, int DT, class A>
 __device__ __forceinline__ void logits(const A& a, int64_t p0, int64_t q0, char* lds, typename T::acc_t (&acc)[T::FP][T::FQ]) {
     constexpr bool SPLIT = DT == DT_F32;
-    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, ((a.kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), SPLIT, lds, acc);
+    if (T::BP == 64 && a.walk.pieces > 1) {
+        const int64_t tile = T::FP * T::FQ * T::THREADS, all = tile * a.tiles_p * a.tiles_q;
+        const f32x4* const o = a.walk.part + (q0 / T::BQ * a.tiles_p + p0 / T::BP) * tile + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FQ; ++j) acc[i][j] = o[(i * T::FQ + j) * T::THREADS];
+#pragma unroll 4
+        for (int k = 1; k < a.walk.pieces; ++k)
+#pragma unroll
+            for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+                for (int j = 0; j < T::FQ; ++j) acc[i][j] += o[k * all + (i * T::FQ + j) * T::THREADS];
+    } else {
+        mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, ((a.kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), SPLIT, lds, acc);
+    }
 #ifdef __HIP_DEVICE_COMPILE__
     const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     const int ml = wp * T::TP + (lane >> 4) * 4;
@@ -596,6 +637,7 @@ struct GradArgs {
     const float *un_w, *un_x;
     int32_t un_step, v0;
     int32_t tiles_p, tiles_q;
+    Walk walk;
     const float *ref, *inv, *mean, *tsum;
     Factor f;
     char* g;               // [rows][g_pitch] per plane, or null (no dx wanted)
@@ -867,7 +909,7 @@ struct Layout {       // of the workspace, and the pieces of the classes
     int64_t piece;      // classes of a piece
     int pieces;
     int64_t bytes = 0;
-    int64_t xp = -1, wp = -1, ux = -1, uw = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1;                     // forward
+    int64_t xp = -1, wp = -1, ux = -1, uw = -1, part = -1, tpart = -1, zt = -1, ce = -1, tabs = -1, walk = -1;          // forward
     int64_t xt = -1, wt = -1, g = -1, gt = -1, db = -1, sum = -1, largest = -1, px = -1, pw = -1, fg = -1;                 // backward
     int64_t take(int64_t n) {
         const int64_t at = bytes;
@@ -887,7 +929,31 @@ void operand_layout(const az_linear_ce_args& a, Layout& l) {
 }
 
 int64_t logit_steps(const az_linear_ce_args& a) { return (a.features + 63) / 64 * (a.dtype == AZ_DT_F32 ? MM_SEGMENTS : 1); }
-int forward_edge(const az_linear_ce_args& a) { return mm_tile_edge(a.classes, a.rows, logit_steps(a)); }
+
+// Tile edge of the logits of nv classes, and pieces of the walk over the features (small tiles only). In microseconds: a step of a workgroup
+// that has a compute unit for itself takes about half of what it takes two (1024 x 2048 -> 1000 bfloat16, 256 tiles: one walk 28, two
+// pieces 30), joining costs a launch and 16 KB per piece that one workgroup reads. At most 512 workgroups, two on each compute unit, so the sums never take more than 8 MB.
+constexpr int64_t WALK_BYTES = int64_t(512) * 64 * 64 * 4;
+struct LogitPlan {
+    int edge, pieces, per;
+};
+LogitPlan logit_plan(const az_linear_ce_args& a, int64_t nv, int edge = 0) {
+    const int64_t steps = logit_steps(a), tiles = ((nv + 63) / 64) * ((a.rows + 63) / 64);
+    LogitPlan p{edge ? edge : mm_tile_edge(nv, a.rows, steps), 1, (int)steps};
+    if ((edge && edge != 64) || tiles > 256) return p;
+    double least = steps * 0.4 + 4.0;      // of small tiles, which is what few tiles always are
+    if (p.edge != 64) return p;
+    for (int64_t n = 2; n * tiles <= 512 && n * 2 <= steps; ++n) {
+        const int64_t per = (steps + n - 1) / n;
+        const double t = per * (n * tiles <= 256 ? 0.4 : 0.8) + 4.0 + 8.0 + n * 0.25;
+        if (t < least) {
+            least = t;
+            p = {64, (int)((steps + per - 1) / per), (int)per};
+        }
+    }
+    return p;
+}
+int forward_edge(const az_linear_ce_args& a) { return logit_plan(a, a.classes).edge; }
 
 // Waves of a workgroup that split the features of the same classes: each keeps eight turns of loads, unless more splitting makes a
 // workgroup for every half compute unit.
@@ -944,6 +1010,7 @@ Layout forward_layout(const az_linear_ce_args& a) {
         l.ux = l.take(a.rows * 4);
         l.uw = l.take(a.classes * 4);
     }
+    if (edge == 64) l.walk = l.take(WALK_BYTES);
     l.part = l.take(a.rows * tiles * 16);
     l.ce = l.take(a.rows * 8);       // cross entropy, entropy
     if (a.target_dense) {
@@ -1043,6 +1110,7 @@ Layout backward_layout(const az_linear_ce_args& a) {
         if (o.x.splits > 1 && o.x.splits * a.rows * a.features * 4 > nx) nx = o.x.splits * a.rows * a.features * 4;
         if (o.w.splits > 1 && o.w.splits * nv * a.features * 4 > nw) nw = o.w.splits * nv * a.features * 4;
     }
+    l.walk = l.take(WALK_BYTES);
     l.px = l.take(nx);
     l.pw = l.take(nw);
     l.largest = l.take(16);
@@ -1087,6 +1155,16 @@ void pack(PackArgs& a, hipStream_t st) {
     a.end_wt = a.end_x + a.wt.blocks();
     const int64_t n = a.end_wt + a.xt.blocks();
     if (n) hipLaunchKernelGGL((k_pack<DT>), dim3((unsigned)n), dim3(256), 0, st, a);
+}
+
+// The pieces of the walk over the features, where there are more than one.
+template <int DT, class S>
+int walk(const LogitPlan& plan, S& s, char* part, hipStream_t st) {
+    s.walk = {plan.pieces, plan.per, (f32x4*)part};
+    if (plan.pieces == 1) return AZ_OK;
+    typedef typename Tiles<DT>::Small T;
+    hipLaunchKernelGGL((k_ce_walk<T, DT>), dim3((unsigned)(s.tiles_p * s.tiles_q * plan.pieces)), dim3(T::THREADS), 0, st, s.w, s.x, s.kbytes, s.tiles_p, s.tiles_q, s.walk);
+    return launched("k_ce_walk");
 }
 
 template <class T, int DT>
@@ -1205,6 +1283,7 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
         s.tile0 = (int)(v0 / edge);
         s.tiles_p = (int)((nv + edge - 1) / edge);
         const bool d = a.target_dense, e = a.entropy_coeff != 0.0f || ent;
+        if (const int rc = walk<DT>(logit_plan(a, nv, edge), s, ws + l.walk, st)) return rc;
         if (edge == 256) launch_stats<typename Tiles<DT>::Big, DT>(s, d, e, st);
         else if (edge == 128) launch_stats<typename Tiles<DT>::Mid, DT>(s, d, e, st);
         else launch_stats<typename Tiles<DT>::Small, DT>(s, d, e, st);
@@ -1279,10 +1358,12 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         s.g_plane = a.rows * vpi * 2;
         s.v0 = (int)v0;
         s.db_pitch = nv;
-        const int edge = mm_tile_edge(nv, a.rows, logit_steps(a));
+        const LogitPlan logit = logit_plan(a, nv);
+        const int edge = logit.edge;
         s.tiles_p = (int)((nv + edge - 1) / edge);
         s.tiles_q = (int)((a.rows + edge - 1) / edge);
         const bool d = a.target_dense, e = a.entropy_coeff != 0.0f;
+        if (const int rc = walk<DT>(logit, s, ws + l.walk, st)) return rc;
         if (edge == 256) launch_grad<typename Tiles<DT>::Big, DT>(s, d, e, st);
         else if (edge == 128) launch_grad<typename Tiles<DT>::Mid, DT>(s, d, e, st);
         else launch_grad<typename Tiles<DT>::Small, DT>(s, d, e, st);

@@ -80,6 +80,15 @@ def test_entropy_and_reductions(dtype, dense, reduction, rows):
     _check(x, w, b, t, c=0.05, reduction=reduction, grad=g)
 
 
+@pytest.mark.parametrize("size", [(20, 5000, 90), (70, 8200, 60), (33, 4096, 1100), (130, 2999, 70), (257, 1999, 33), (65, 20001, 3)], ids=ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_long_features(size, dtype, dense):
+    """Few rows and classes: the walk over the features is split."""
+    x, w, b, t = _inputs(*size, dtype, dense, size[0] & 1 == 0)
+    _check(x, w, b, t, c=0.01 if size[0] > 100 else 0.0, reduction="sum" if size[0] == 70 else "mean")
+
+
 @pytest.mark.parametrize("size", [(520, 64, 20000), (2048, 128, 3000), (5000, 40, 700)], ids=ids)
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 def test_large_and_middle_tiles(size, dtype):
