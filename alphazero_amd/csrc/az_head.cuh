@@ -969,10 +969,25 @@ int few_grid(const az_linear_ce_args& a) {
     return (int)(groups < 512 ? groups : 512);
 }
 
-// Rows up to which the forward pass streams the weight. Measured with 32000 classes of 2048 features: 16-bit, 24 rows 58 us against the
-// tiles' 39 (rows that start anywhere, which the tiles have copied: 131 against 89); float32, 24 rows 101 against 238, 48 rows, which
-// need more accumulators than the streaming kernel has registers, 246 against 240.
-bool few_forward(const az_linear_ce_args& a) { return a.rows <= (a.dtype == AZ_DT_F32 ? 32 : 16); }
+// Where the kernels of az_head_few.cuh, which stream the weight as it lies, take the place of the tiles. Measured with 1 to 32 rows.
+// Forward, 16 bits: tiles read a weight in place as fast (16 x 4096 -> 4096: 26 us against 31, 16 x 1024 -> 32000: 30 against 52); only
+// copying a large one costs more (16 x 4095 -> 32000: 212 against 185; 16 x 2047 -> 16000: 54 against 68).
+// Forward, float32, where tiles always copy: streaming (16 x 4096 -> 4096: 43 us against 72) unless long features and few classes leave it
+// few workgroups (16 x 8192 -> 60: 59 against 40). 24 rows 101 us against 238 (2048 -> 32000), 48 rows, which need more accumulators
+// than it has registers, 246 against 240.
+bool few_forward(const az_linear_ce_args& a) {
+    if (a.dtype == AZ_DT_F32) return a.rows <= 32 && (a.features <= 1024 || a.features <= 4 * a.classes);
+    return a.rows <= 16 && !in_place(a.weight, a.weight_pitch, a.features) && a.classes * a.features > (int64_t(1) << 26);
+}
+// Backward: streaming saves the turned copies of the weight and G, its sums over the classes grow with the rows. 16 bits: 4096 -> 8000 4 rows 51 us
+// against 88, 16 rows 74 against 89; 4096 -> 1000 4 rows 31 against 28, 16 rows 45 against 28; copied 2047 -> 16000 116 to 147 against
+// 132, 4095 -> 32000 489 against 500. float32: 4096 -> 1000 1 row 35 against 50, 16 rows 56 against 52; 16 x 1024 -> 200 34 against 23.
+bool few_backward(const az_linear_ce_args& a) {
+    const int64_t size = a.classes * a.features;
+    if (a.rows > FEW_GRAD_ROWS || a.features > 16 * a.classes) return false;
+    if (a.dtype == AZ_DT_F32) return size >= a.rows * (3 << 16);
+    return size >= a.rows * (3 << 19) && (size >= int64_t(1) << 25 || in_place(a.weight, a.weight_pitch, a.features));
+}
 
 Layout forward_layout(const az_linear_ce_args& a) {
     Layout l;
@@ -1068,7 +1083,7 @@ OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
 
 Layout backward_layout(const az_linear_ce_args& a) {
     Layout l;
-    if (a.rows <= FEW_GRAD_ROWS) {
+    if (few_backward(a)) {
         l.few = true;
         l.grid = few_grid(a);
         l.fg = l.take(a.classes * 16 * 4);

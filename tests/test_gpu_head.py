@@ -89,6 +89,44 @@ def test_long_features(size, dtype, dense):
     _check(x, w, b, t, c=0.01 if size[0] > 100 else 0.0, reduction="sum" if size[0] == 70 else "mean")
 
 
+# a few rows of a large weight take the kernels that stream it: both passes, only the backward one (16 bits, read in place)
+@pytest.mark.parametrize("size", [(1, 1032, 33000), (2, 1032, 33000), (4, 1032, 33000), (7, 2056, 17000), (16, 1032, 33000), (16, 1025, 66000), (3, 1025, 66001),
+                                  (30, 1025, 66001), (9, 72, 66001)], ids=ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_few_rows_of_a_large_weight(size, dtype, dense):
+    x, w, b, t = _inputs(*size, dtype, dense, size[0] != 4)
+    _check(x, w, b, t, c=0.01 if size[0] in (7, 16) else 0.0, grad=torch.tensor(256.0 if dtype == F16 else 1.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("size", [(13, 1032, 33000), (11, 1025, 66001)], ids=ids)
+def test_few_rows_of_a_large_weight_special_values(dtype, size):
+    rows, feats, classes = size
+    x, w, b, t = _inputs(*size, dtype, False, True)
+    t[4], t[6] = -100, 7
+    shut = torch.arange(classes, device="cuda") % 3 == 0
+    shut[64:4096] = True
+    b[shut] = -float("inf")
+    t = torch.where(t == -100, t, torch.where(shut[t.clamp(min=0)], 1, t))
+    g = torch.linspace(0.5, 2.0, rows, device="cuda")
+    good = _check(x, w, b, t, c=0.05, reduction="none", grad=g)
+    assert not good[5][shut].any() and not good[4][shut].any()
+    y = x.clone()
+    y[4] = float("nan")                                  # a row that does not count holds anything
+    h = g.clone()
+    h[4] = float("inf")
+    for a, v in zip(good, _run(y, w, b, t, h, entropy_coeff=0.05, reduction="none")):
+        assert torch.equal(a, v)
+    for wrong in (classes, -1, 1 << 40):
+        u = t.clone()
+        u[6] = wrong
+        each, _, _, gx, gw, gb = _run(x, w, b, u, g, reduction="none")
+        keep = torch.arange(rows) != 6
+        assert math.isnan(float(each[6])) and torch.isfinite(each[keep]).all()
+        assert torch.isnan(gx[6]).all() and torch.isnan(gw).any() and torch.isnan(gb).any()
+
+
 @pytest.mark.parametrize("size", [(520, 64, 20000), (2048, 128, 3000), (5000, 40, 700)], ids=ids)
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 def test_large_and_middle_tiles(size, dtype):
