@@ -280,13 +280,25 @@ __device__ __forceinline__ void mm_opaque(typename T::acc_t (&acc)[T::FP][T::FQ]
         for (int j = 0; j < T::FQ; ++j) asm volatile("" : "+v"(acc[i][j]));
 }
 
+// Place of a workgroup in a walk over `total` of them: consecutive ids go round the 8 XCDs, so each XCD gets a contiguous stretch.
+__device__ __forceinline__ int mm_stretch(int id, int total) {
+    const int per = total >> 3, rest = total & 7, xcd = id & 7;
+    return xcd * per + (xcd < rest ? xcd : rest) + (id >> 3);
+}
+// Workgroup id -> piece of k and tile, for few tiles whose walk over k is split: a stretch has whole pieces or parts of one, in which the
+// tiles that read the same strip of the longer side follow each other.
+__device__ __forceinline__ void mm_place_piece(int id, int pieces, int tiles_p, int tiles_q, int& piece, int& tp, int& tq) {
+    const int tiles = tiles_p * tiles_q, l = mm_stretch(id, tiles * pieces), t = l % tiles;
+    piece = l / tiles;
+    const bool wide = tiles_p >= tiles_q;
+    tp = wide ? t / tiles_q : t % tiles_p;
+    tq = wide ? t % tiles_q : t / tiles_p;
+}
 // Workgroup id -> tile (p, q): consecutive ids go round the 8 XCDs, so each XCD gets a contiguous stretch of the walk, and the
 // walk goes through groups of 8 p tiles with q outermost inside a group: the 32 tiles that an XCD works on at a time are about
 // 8 x 4, which read 12 operand strips through its L2 instead of 33.
 __device__ __forceinline__ void mm_place(int id, int tiles_p, int tiles_q, int& tp, int& tq) {
-    const int total = tiles_p * tiles_q, per = total >> 3, rest = total & 7;
-    const int xcd = id & 7, at = id >> 3;
-    const int l = xcd * per + (xcd < rest ? xcd : rest) + at;
+    const int l = mm_stretch(id, tiles_p * tiles_q);
     const int group = l / (8 * tiles_q), in = l - group * 8 * tiles_q;
     const int width = tiles_p - group * 8 < 8 ? tiles_p - group * 8 : 8;
     tp = group * 8 + in % width;

@@ -251,11 +251,12 @@ template <class T, int DT>
 __global__ __launch_bounds__(T::THREADS) void k_ce_walk(MmOperand w, MmOperand x, int kbytes, int tiles_p, int tiles_q, Walk walk) {
     __shared__ __align__(16) char lds[T::LDS];
     constexpr bool SPLIT = DT == DT_F32;
-    const int tiles = tiles_p * tiles_q, piece = blockIdx.x / tiles, tile = blockIdx.x % tiles, tp = tile % tiles_p, tq = tile / tiles_p;
+    int piece, tp, tq;
+    mm_place_piece(blockIdx.x, walk.pieces, tiles_p, tiles_q, piece, tp, tq);
     const int steps = ((kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), begin = piece * walk.per;
     typename T::acc_t acc[T::FP][T::FQ];
     mm_tile<T>(w, x, (int64_t)tp * T::BP, (int64_t)tq * T::BQ, kbytes, begin, begin + walk.per < steps ? begin + walk.per : steps, SPLIT, lds, acc);
-    f32x4* const o = walk.part + (int64_t)blockIdx.x * (T::FP * T::FQ * T::THREADS) + threadIdx.x;
+    f32x4* const o = walk.part + (((int64_t)piece * tiles_q + tq) * tiles_p + tp) * (T::FP * T::FQ * T::THREADS) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < T::FP; ++i)
 #pragma unroll

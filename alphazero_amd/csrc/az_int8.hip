@@ -208,12 +208,8 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
     int piece = 0, tp, tq;
     if (a.splits == 1) {
         mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
-    } else {        // a piece of k on one XCD (ids go round the 8 of them): its tiles read the same strips through one L2
-        const int at = blockIdx.x >> 3;
-        piece = (blockIdx.x & 7) + 8 * (at / tiles);
-        tp = at % tiles % a.tiles_p;
-        tq = at % tiles / a.tiles_p;
-        if (piece >= a.splits) return;
+    } else {
+        mm_place_piece(blockIdx.x, a.splits, a.tiles_p, a.tiles_q, piece, tp, tq);
     }
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
@@ -329,7 +325,7 @@ __device__ __forceinline__ i32x4 bytes16(const int8_t* row, int k, int cols) {
 // and are not written.
 // Floating tokens (DX, one to FUSED_TOKENS of them) are quantised by every workgroup for itself, into LDS, while its first weights
 // are on the way: one launch, with the values and the sums of two. One token, 4096 -> 16384: 14.3 us against 17.5 us.
-constexpr int FUSED_TOKENS = 4, FUSED_BYTES = 32768, DT_I8 = AZ_DT_I8;
+constexpr int FEW_TOKENS = 48, FUSED_TOKENS = 2, FUSED_BYTES = 32768, DT_I8 = AZ_DT_I8;
 // Channels of a wave in fragments of 16: two for each token fragment read from memory, as long as the sums fit.
 constexpr int few_fragments(bool fused, int mt) { return !fused && mt <= 2 ? 2 : 1; }
 template <int DT, int DX, int MT>
@@ -482,16 +478,25 @@ struct Plan {
 Plan plan_of(const az_int8_args& a) {
     Plan p;
     p.kpitch = round_up(a.features, 16);
-    p.few = a.tokens <= 64;
-    p.fused = a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
+    auto crooked = [&](const void* q, int64_t pitch) { return (((uintptr_t)q | (uintptr_t)pitch) & 15) != 0 || (a.features & 15) != 0 || pitch > MM_MAX_PITCH; };
+    const bool copy = crooked(a.weight, a.weight_pitch);
+    // Where the kernel for few tokens takes the place of the tiles. From 16384 channels on the tiles fill the chip in one walk (one int8 token,
+    // 1024 -> 32000: 8.3 us against 13.6; 4096 -> 32000: 23.6 against 27). Below, they join pieces of k in a second launch (16 x 4096 ->
+    // 4096: 11.4 against 9.2, 16 x 4096 -> 8000 13.1 against 9.6, 48 x 1024 -> 4096 8.7 against 7.5), which pays with more tokens and with
+    // longer walks (32 x 4096 -> 1024 8.7 against 10.7, 16 x 8192 -> 1024 10 against 14, 64 x 4096 -> 32000 24.8 against 76). A weight that the
+    // tiles have to copy: 4 x 4095 -> 4096 22 against 24, 32 x 4095 -> 4096 23 against 36. One or two floating tokens are quantised in
+    // the same launch, also for more channels where a row is long (1 x 14336 -> 4096 bfloat16: 17 us against 23, 1 x 4096 -> 16384 14.3 against
+    // 16.3, 1 x 1024 -> 32000 16.7 against 11.7; four tokens 14336 -> 4096 29 against 25).
+    const bool small = a.channels < 16384;
+    p.few = small && a.features <= 4096 && a.tokens <= (copy ? 4 : a.features <= 2048 ? FEW_TOKENS : 16);
+    p.fused = (small || a.channels <= 4 * a.features) && a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
     if (p.fused) return p;
     if (a.x_dtype != AZ_DT_I8) {
         p.q = p.take(a.tokens * p.kpitch);
         p.scale = p.take(a.tokens * 4);
     }
     if (p.few) return p;
-    auto crooked = [&](const void* q, int64_t pitch) { return (((uintptr_t)q | (uintptr_t)pitch) & 15) != 0 || (a.features & 15) != 0 || pitch > MM_MAX_PITCH; };
-    p.align_w = crooked(a.weight, a.weight_pitch);
+    p.align_w = copy;
     p.align_x = a.x_dtype == AZ_DT_I8 && crooked(a.x, a.x_pitch);
     if (p.align_w) p.w = p.take(a.channels * p.kpitch);
     if (p.align_x) p.x = p.take(a.tokens * p.kpitch);
@@ -499,8 +504,9 @@ Plan plan_of(const az_int8_args& a) {
     const int steps = (int)((p.kpitch + 127) / 128);
     p.edge = mm_tile_edge(a.channels, a.tokens, steps);
     p.per = steps;
-    if (p.edge == 64) {      // split k until there is a workgroup per compute unit, with at least 4 steps each
-        int64_t s = 256 / tiles(64);
+    if (p.edge == 64) {      // split k until there is a workgroup per compute unit with at least 4 steps, or two with 24 (128 x 14336 -> 4096: 22 us, one: 25)
+        int64_t s = 512 / tiles(64);
+        if (s * 24 > steps) s = 256 / tiles(64);
         if (s > steps / 4) s = steps / 4;
         if (s > 1) {
             p.per = (int)((steps + s - 1) / s);
@@ -576,11 +582,10 @@ void quantize(int dtype, const QuantArgs& q, hipStream_t st) {
 
 template <class T, int DT>
 void run_tiles(const TileArgs& t, hipStream_t st) {
-    const int rounds = t.splits > 1 ? (t.splits + 7) / 8 * 8 : 1;
-    hipLaunchKernelGGL((k_int8_tile<T, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * rounds)), dim3(T::THREADS), 0, st, t);
+    hipLaunchKernelGGL((k_int8_tile<T, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * t.splits)), dim3(T::THREADS), 0, st, t);
 }
 
-// Up to 64 tokens. The waves of a workgroup that share 16 channels are as few as leave a workgroup per compute unit: the join is
+// Up to FEW_TOKENS tokens. The waves of a workgroup that share 16 channels are as few as leave a workgroup per compute unit: the join is
 // then smallest.
 template <int DT, int DX>
 int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, hipStream_t st) {
@@ -595,8 +600,7 @@ int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, 
     if (DX != DT_I8 || a.tokens <= 16) run(std::integral_constant<int, 1>{});
     else if constexpr (DX == DT_I8) {
         if (a.tokens <= 32) run(std::integral_constant<int, 2>{});
-        else if (a.tokens <= 48) run(std::integral_constant<int, 3>{});
-        else run(std::integral_constant<int, 4>{});
+        else run(std::integral_constant<int, 3>{});
     }
     return launched("k_int8_few");
 }

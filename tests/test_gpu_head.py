@@ -489,7 +489,10 @@ def _int8_check(x, qw, ws, b, y, q, s):
 
 
 INT8 = [(1, 1, 1), (1, 64, 16), (1, 4096, 1024), (5, 100, 33), (16, 130, 50), (17, 2000, 83), (33, 77, 300), (64, 512, 128), (65, 64, 64), (70, 1000, 90),
-        (256, 3000, 256), (300, 129, 517), (1024, 200, 2500), (2304, 256, 5632)]
+        (256, 3000, 256), (300, 129, 517), (1024, 200, 2500), (2304, 256, 5632),
+        # few tokens of aligned weights, of crooked ones, of many channels; walks over the features in pieces
+        (3, 256, 100), (9, 1024, 500), (16, 4096, 333), (20, 2048, 31), (40, 2048, 100), (48, 512, 128), (49, 512, 128), (2, 4095, 300), (4, 131, 50), (1, 128, 16500),
+        (3, 130, 16400), (20, 8208, 70), (64, 23104, 256), (90, 14336, 1000), (200, 5000, 65)]
 
 
 @pytest.mark.parametrize("size", INT8, ids=ids)
