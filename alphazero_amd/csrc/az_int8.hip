@@ -537,9 +537,10 @@ int launched(const char* what) {
     return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
-// Two to eight chunks per lane. From 2048 rows on a short row gets no more lanes than hold it (262144 x 64 bfloat16: 17 us, with 256 lanes
-// 270; 32768 x 2048: 40 against 54); with fewer rows more lanes are the shorter wait (256 x 2048: 3.6 us, with 64 lanes 5.4). 256 lanes
-// hold up to 32 KB, 1024 up to 128 KB (256 x 23104 float32: 8.5 us, with 256 lanes and a second read 14.9).
+// Two to four chunks per lane: more hold fewer rows in flight. From 2048 rows on a short row gets no more lanes than hold it (262144 x 64
+// bfloat16: 17 us, with 256 lanes 270; 32768 x 2048: 40 against 54); with fewer rows more lanes are the shorter wait (256 x 2048: 3.6 us, with
+// 64 lanes 5.4). Long rows: 1024 x 23104 bfloat16 21 us with 1024 lanes of three chunks, 33 with eight; 1024 x 14336 float32 14 with four,
+// 21 with eight. What does not fit is read twice (1024 x 23104 float32: 22 us with four of six chunks held, 26 with all).
 template <int DT>
 void launch_quantize(const QuantArgs& q, hipStream_t st) {
     const int64_t bytes = (int64_t)q.cols * (DT == DT_F32 ? 4 : 2);
@@ -549,18 +550,20 @@ void launch_quantize(const QuantArgs& q, hipStream_t st) {
     };
     const std::integral_constant<int, 2> two;
     const std::integral_constant<int, 4> four;
-    const std::integral_constant<int, 8> eight;
-    const std::integral_constant<int, 256> wide;
+    const std::integral_constant<int, 64> wave;
+    const std::integral_constant<int, 256> group;
+    const std::integral_constant<int, 1024> all;
     const bool many = q.rows >= 2048;
-    if (many && bytes <= 256) run(eight, two);
+    if (many && bytes <= 256) run(std::integral_constant<int, 8>{}, two);
     else if (many && bytes <= 512) run(std::integral_constant<int, 16>{}, two);
     else if (many && bytes <= 1024) run(std::integral_constant<int, 32>{}, two);
-    else if (many && bytes <= 2048) run(std::integral_constant<int, 64>{}, two);
-    else if (many && bytes <= 4096) run(std::integral_constant<int, 64>{}, four);
-    else if (bytes <= 8192) run(wide, two);
-    else if (bytes <= 16384) run(wide, four);
-    else if (bytes <= 32768) run(wide, eight);
-    else run(std::integral_constant<int, 1024>{}, eight);
+    else if (many && bytes <= 2048) run(wave, two);
+    else if (many && bytes <= 4096) run(wave, four);
+    else if (bytes <= 8192) run(group, two);
+    else if (bytes <= 16384) run(group, four);
+    else if (bytes <= 32768) run(std::integral_constant<int, 512>{}, four);
+    else if (bytes <= 49152) run(all, std::integral_constant<int, 3>{});
+    else run(all, four);
 }
 template <int DT>
 void quantize_as(const QuantArgs& q, hipStream_t st) {

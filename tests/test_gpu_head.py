@@ -444,7 +444,8 @@ def test_quantize_rows(dtype, size):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("size", [(2051, 1), (2048, 63), (2049, 129), (2050, 361), (3001, 513), (2053, 1025), (2047, 2048), (2055, 2047)], ids=ids)
+@pytest.mark.parametrize("size", [(2051, 1), (2048, 63), (2049, 129), (2050, 361), (3001, 513), (2053, 1025), (2047, 2048), (2055, 2047),
+                                  (100, 6001), (70, 14333), (60, 23105), (50, 33001), (40, 70003)], ids=ids)
 def test_quantize_many_short_rows(dtype, size):
     """Rows that share a workgroup, of odd lengths and far apart; a row that is not finite and one of zeros stay their own affair."""
     rows, cols = size
