@@ -55,7 +55,10 @@ struct PackJob {
     const float* all;
     const int64_t* target;  // null: every row counts
     int64_t ignore;
-    __host__ __device__ int64_t blocks() const { return own ? (rows + 3) / 4 : (rows * (pitch >> 4) + 255) / 256; }
+    // Lanes of a row that is scaled by itself: as many as it has pieces, up to a wave, or a workgroup from 4096 columns on (forward pass of
+    // 64 x 64 -> 131000: 51 us, with a wave for each row 101; of 64 x 65536 -> 64: 78 against 180).
+    __host__ __device__ int lanes() const { return pitch <= 128 ? 8 : pitch <= 256 ? 16 : pitch <= 512 ? 32 : pitch < 8192 ? 64 : 256; }
+    __host__ __device__ int64_t blocks() const { return own ? (rows + 256 / lanes() - 1) / (256 / lanes()) : (rows * (pitch >> 4) + 255) / 256; }
     __device__ __forceinline__ bool counts(int64_t r) const { return !(target && target[r] == ignore); }
 };
 
@@ -83,7 +86,7 @@ __device__ __forceinline__ void load_planes(const void* src, int64_t at, int lef
 }
 
 template <int DT>
-__device__ __forceinline__ void pack_block(const PackJob& j, int64_t block) {
+__device__ __forceinline__ void pack_block(const PackJob& j, int64_t block, float* tops) {
     constexpr int NP = DT == DT_F32 ? 2 : 1;
     const int pieces = (int)(j.pitch >> 4);
     __align__(16) uint16_t h[2][8];
@@ -92,23 +95,38 @@ __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + piece * 16) = *(const uint4*)h[p];
     };
-    if (DT == DT_F32 && j.own) {       // a wave per row
-        const int64_t r = block * 4 + (threadIdx.x >> 6);
-        const int lane = threadIdx.x & 63;
+    if (DT == DT_F32 && j.own) {
+        const int lanes = j.lanes(), lane = threadIdx.x & (lanes - 1);
+        const int64_t r = block * (256 / lanes) + threadIdx.x / lanes;
         if (r >= j.rows) return;
-        float top = 0.0f;
-        if (j.counts(r))
-            for (int i = lane; i < pieces; i += 64) {
+        const bool counts = j.counts(r);
+        float first[8], top = 0.0f;        // a lane's first piece stays in registers, what a row has beyond comes again from L2
+        load8((const float*)j.src, r * j.src_pitch + lane * 8, counts ? j.cols - lane * 8 : 0, first);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = larger(top, fabsf(first[e]));
+        if (counts)
+            for (int i = lane + lanes; i < pieces; i += lanes) {
                 float v[8];
                 load8((const float*)j.src, r * j.src_pitch + i * 8, j.cols - i * 8, v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = larger(top, fabsf(v[e]));
             }
+        for (int o = 1; o < 64 && o < lanes; o *= 2) top = larger(top, __shfl_xor(top, o));
+        if (lanes == 256) {
+            if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+            __syncthreads();
 #pragma unroll
-        for (int o = 1; o < 64; o *= 2) top = larger(top, __shfl_xor(top, o));
-        const float un = unscale_of(top);
+            for (int w = 0; w < 4; ++w) top = larger(top, tops[w]);
+        }
+        const float un = unscale_of(top), scale = 1.0f / un;
         if (lane == 0) j.own[r] = un;
-        for (int i = lane; i < pieces; i += 64) put(r, i, 1.0f / un);
+        if (lane < pieces) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) split2(first[e] * scale, h[0][e], h[1][e]);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + lane * 16) = *(const uint4*)h[p];
+        }
+        for (int i = lane + lanes; i < pieces; i += lanes) put(r, i, scale);
     } else {
         const int64_t at = block * 256 + threadIdx.x;
         if (at < (int64_t)j.rows * pieces) put(at / pieces, (int)(at % pieces), DT == DT_F32 ? 1.0f / *j.all : 1.0f);
@@ -171,8 +189,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
     __shared__ __align__(16) uint16_t tile[DT == DT_F32 ? 2 : 1][64][66];
     const int64_t id = blockIdx.x;
-    if (id < a.end_w) pack_block<DT>(a.w, id);
-    else if (id < a.end_x) pack_block<DT>(a.x, id - a.end_w);
+    if (id < a.end_w) pack_block<DT>(a.w, id, (float*)tile);
+    else if (id < a.end_x) pack_block<DT>(a.x, id - a.end_w, (float*)tile);
     else if (id < a.end_wt) turn_block<DT>(a.wt, id - a.end_x, tile);
     else turn_block<DT>(a.xt, id - a.end_wt, tile);
 }
@@ -453,9 +471,11 @@ __device__ __forceinline__ void join_row(const JoinArgs& a, int64_t n, int lane)
             v.ref = ref;
         }
     };
+#pragma unroll 4
     for (int i = lane; i < a.tiles; i += LANES) larger(a.part[first + i][0]);
 #pragma unroll
     for (int o = 1; o < LANES; o *= 2) larger(__shfl_xor(v.ref, o));
+#pragma unroll 4
     for (int i = lane; i < a.tiles; i += LANES) {
         join_part(v, part_at(a, first + i));
         if (a.t.dense) ta += a.tpart[2 * (first + i) + 1];
@@ -514,8 +534,12 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
     float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides all rows by it
     if (a.un_x) {
         for (int n = threadIdx.x; n < a.count_x; n += 1024) ux = fmaxf(ux, a.un_x[n]);
-#pragma unroll 8
-        for (int m = threadIdx.x; m < a.count_w; m += 1024) uw = fmaxf(uw, a.un_w[m]);
+#pragma unroll 4
+        for (int m = threadIdx.x; m < a.count_w >> 2; m += 1024) {
+            const f32x4 v = ((const f32x4*)a.un_w)[m];
+            uw = fmaxf(fmaxf(uw, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
+        }
+        if (const int m = (a.count_w & ~3) + threadIdx.x; m < a.count_w) uw = fmaxf(uw, a.un_w[m]);
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             ux = fmaxf(ux, __shfl_xor(ux, o));
@@ -985,7 +1009,7 @@ bool few_forward(const az_linear_ce_args& a) {
 // 132, 4095 -> 32000 489 against 500. float32: 4096 -> 1000 1 row 35 against 50, 16 rows 56 against 52; 16 x 1024 -> 200 34 against 23.
 bool few_backward(const az_linear_ce_args& a) {
     const int64_t size = a.classes * a.features;
-    if (a.rows > FEW_GRAD_ROWS || a.features > 16 * a.classes) return false;
+    if (a.rows > FEW_GRAD_ROWS || a.features > 16 * a.classes || a.features < 256) return false;      // 256 lanes take 4 features each
     if (a.dtype == AZ_DT_F32) return size >= a.rows * (3 << 16);
     return size >= a.rows * (3 << 19) && (size >= int64_t(1) << 25 || in_place(a.weight, a.weight_pitch, a.features));
 }

@@ -1,4 +1,5 @@
-// The loss of a linear layer for few rows (up to 16, float32 forward up to 32): what counts is how often the weight goes through memory.
+// The loss of a linear layer for few rows (up to 16, float32 forward up to 32; few_forward and few_backward say where): what counts is how
+// often the weight goes through memory.
 //
 // Forward: the weight streams once, from memory to the matrix instructions' registers, with no copy and no LDS in between; rows may
 // start anywhere. float32 uses the float32 matrix instruction (0.16 PFLOP/s, which is more than the memory feeds with 16 rows).
