@@ -343,8 +343,8 @@ typedef enum { AZ_DT_F32 = 0, AZ_DT_BF16 = 1, AZ_DT_F16 = 2, AZ_DT_I8 = 3 } az_d
 typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2 } az_reduce;
 
 /* Cross entropy of softmax(x weight^T + bias) against class indices or against rows of target weights, minus entropy_coeff times
- * the softmax' entropy; the logits are never stored. Rows whose index is ignore_index cost nothing, get zero gradients and stay
- * out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
+ * the softmax' entropy; the logits are never stored (up to 8 MB of partial sums of few of them are). Rows whose index is
+ * ignore_index cost nothing, get zero gradients and stay out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
  * -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax and gives NaN. The gradient of the logits is
  * held in 16 bits between the products (two planes for float32), relative to the largest sum of target weights of a row: with float16,
  * rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give NaN with float32. */
