@@ -337,6 +337,25 @@ __device__ __forceinline__ void logits(const A& a, int64_t p0, int64_t q0, char*
 #endif
 }
 
+// A row's target weights for the classes that a lane holds, from class `at` on, `left` of which exist. A tile without the last class (`full`)
+// loads 16 bytes at a time and asks nothing; a question for each of them, held in a scalar register each, made the 256 tile spill
+// (8192 x 1024 -> 4001 float16: forward 114 us, now 99, backward 353,
+// now 305). Rows behind the last one get the last one's, which nobody uses.
+template <class T>
+__device__ __forceinline__ void target_weights(const Rows& t, int64_t n, int64_t at, int left, bool full, f32x4 (&pi)[T::FP]) {
+    const float* const p = t.dense + (n < t.rows ? n : t.rows - 1) * t.dense_pitch + at;
+    asm volatile("" : "+v"(left));        // the questions are not kept from one row of the lane for the next
+    if (full) {
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i) __builtin_memcpy(&pi[i], p + i * 16, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < T::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pi[i][r] = i * 16 + r < left ? p[i * 16 + r] : 0.0f;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <class T, int DT, bool DENSE, bool ENT>
 __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
@@ -382,7 +401,8 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
                         if (hit == i * 16 + r) a.zt[n] = acc[i][j][r];
             }
         }
-        const float* pi = DENSE && n < a.t.rows ? a.t.dense + n * a.t.dense_pitch + a.v0 + p0 + wp * T::TP + (lane >> 4) * 4 : nullptr;
+        f32x4 pi[T::FP];
+        if constexpr (DENSE) target_weights<T>(a.t, n, a.v0 + p0 + wp * T::TP + (lane >> 4) * 4, left, p0 + T::BP <= a.t.classes - a.v0, pi);
 #pragma unroll
         for (int i = 0; i < T::FP; ++i)
 #pragma unroll
@@ -392,7 +412,7 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_stats(StatArgs a) {
                 l += e;
                 if constexpr (ENT) s += e == 0.0f ? 0.0f : e * t;   // 0 * -inf of a class that cannot be
                 if constexpr (DENSE) {
-                    const float v = pi && i * 16 + r < left ? pi[i * 16 + r] : 0.0f;
+                    const float v = pi[i][r];
                     pi_sum += v;
                     pi_abs += fabsf(v);
                     dot += v == 0.0f ? 0.0f : v * t;
@@ -673,8 +693,9 @@ struct GradArgs {
     int64_t db_pitch;
 };
 
+// Two waves to a SIMD: with float32, target weights and entropy the 128 tile would else take one register too many for them.
 template <class T, int DT, bool DENSE, bool ENT>
-__global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
+__global__ __launch_bounds__(T::THREADS, 2) void k_ce_grad(GradArgs a) {
     __shared__ __align__(16) char lds[T::LDS];
     int tp, tq;
     mm_place(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
@@ -705,7 +726,8 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
             if (!DENSE && (target < 0 || target >= a.t.classes)) f = NAN;
         }
         const Reference at(ref);
-        const float* pi = DENSE && row ? a.t.dense + n * a.t.dense_pitch + a.v0 + ml : nullptr;
+        f32x4 pi[T::FP];
+        if constexpr (DENSE) target_weights<T>(a.t, n, a.v0 + ml, left, p0 + T::BP <= a.t.classes - a.v0, pi);
         const float scale = (DENSE ? total * inv : inv) * f, c = a.t.entropy * LN2 * inv * f;
 #pragma unroll
         for (int i = 0; i < T::FP; ++i)
@@ -714,7 +736,7 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_grad(GradArgs a) {
                 const float t = at.t(acc[i][j][r]);
                 const float e = __builtin_amdgcn_exp2f(t);
                 float g = e * scale;
-                if constexpr (DENSE) g -= pi && i * 16 + r < left ? pi[i * 16 + r] * f : 0.0f;
+                if constexpr (DENSE) g -= pi[i][r] * f;
                 if constexpr (ENT) g += e == 0.0f ? 0.0f : c * e * (t - mean);
                 acc[i][j][r] = counts ? g : 0.0f;
             }
