@@ -70,17 +70,16 @@ struct MmTile {
 };
 
 // Planes of segment s of 3: (h, m) (m, h) (h, h).
+// With planes of Q only (P is 16-bit by itself) it is walked twice: m, then h. Planes of bfloat16 keep their exponent, m is not scaled.
 constexpr int MM_SEGMENTS = 3;
-__device__ __forceinline__ int mm_plane_p(int s) { return s == 1; }
-__device__ __forceinline__ int mm_plane_q(int s) { return s == 0; }
 
 // One tile: acc[i][j] = results p = p0 + wp * TP + 16 i + 4 (lane >> 4) + 0..3, q = q0 + wq * TQ + 16 j + (lane & 15), where
 // wave = wp * WQ + wq. kbytes: bytes of k per row (a multiple of 16). k_first / k_last: the 128-byte steps [k_first, k_last) of
-// the walk of ceil(kbytes / 128) steps (three times that many for float32, `split`) that this workgroup takes. All lanes of the workgroup call it; on
+// the walk of ceil(kbytes / 128) steps for each of `segments` (1, 2 or 3) that this workgroup takes. All lanes of the workgroup call it; on
 // return every wave has read its last fragment and passed a barrier, so the LDS may be used for something else.
 template <class T>
 __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, int64_t p0, int64_t q0, int kbytes, int k_first, int k_last,
-                                        bool split, char* lds, typename T::acc_t (&acc)[T::FP][T::FQ]) {
+                                        int segments, char* lds, typename T::acc_t (&acc)[T::FP][T::FQ]) {
 #ifdef __HIP_DEVICE_COMPILE__   // the buffer resource type exists on the device only
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -97,7 +96,7 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     const char* const qbase = Q.base + q0 * Q.pitch;
     // bytes from the tile's first row to the end of the matrix' last row; below zero (an empty tile) reads nothing
     const int64_t pext = ((int64_t)P.rows - p0 - 1) * P.pitch + kbytes, qext = ((int64_t)Q.rows - q0 - 1) * Q.pitch + kbytes;
-    int ks = split ? k_first / ksteps : 0;      // segment and step within it of the next stage to fetch
+    int ks = segments > 1 ? k_first / ksteps : 0;      // segment and step within it of the next stage to fetch
     int kk = k_first - ks * ksteps;
     int left = k_last - k_first;                // stages still to fetch
 
@@ -106,10 +105,8 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
         const int k = kk << 7;
         const char* pb = pbase + k;
         const char* qb = qbase + k;
-        if (split) {
-            pb += mm_plane_p(ks) * P.plane;
-            qb += mm_plane_q(ks) * Q.plane;
-        }
+        if (segments == 3) pb += (ks == 1) * P.plane;
+        if (segments > 1) qb += (ks == 0) * Q.plane;
         const int64_t pn = pext - k, qn = qext - k;
         const bool none = left <= 0;
         const int pr = pn < 0 || none ? 0 : (pn > 0x7fffffff ? 0x7fffffff : (int)pn), qr = qn < 0 || none ? 0 : (qn > 0x7fffffff ? 0x7fffffff : (int)qn);
@@ -177,7 +174,7 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     meet(std::integral_constant<int, T::STAGES - 1>{});
     read(0, sw0, a0, b0);
     int s = 0;
-    const int turn = split ? 2 * ksteps - k_first : -1;      // the step that the (h, h) segment starts with
+    const int turn = segments > 1 ? (segments - 1) * ksteps - k_first : -1;      // the step that the (h, h) segment starts with
     auto lower = [&] {
         if constexpr (T::KIND == MM_F16)
 #pragma unroll
@@ -201,7 +198,7 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
         __builtin_amdgcn_sched_barrier(0);
     }
     meet(std::integral_constant<int, 0>{});
-    if (split && turn >= n) lower();      // a piece of the walk that ends before it
+    if (segments > 1 && turn >= n) lower();      // a piece of the walk that ends before it
 #endif
 }
 

@@ -273,7 +273,7 @@ __global__ __launch_bounds__(T::THREADS) void k_ce_walk(MmOperand w, MmOperand x
     mm_place_piece(blockIdx.x, walk.pieces, tiles_p, tiles_q, piece, tp, tq);
     const int steps = ((kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), begin = piece * walk.per;
     typename T::acc_t acc[T::FP][T::FQ];
-    mm_tile<T>(w, x, (int64_t)tp * T::BP, (int64_t)tq * T::BQ, kbytes, begin, begin + walk.per < steps ? begin + walk.per : steps, SPLIT, lds, acc);
+    mm_tile<T>(w, x, (int64_t)tp * T::BP, (int64_t)tq * T::BQ, kbytes, begin, begin + walk.per < steps ? begin + walk.per : steps, SPLIT ? MM_SEGMENTS : 1, lds, acc);
     f32x4* const o = walk.part + (((int64_t)piece * tiles_q + tq) * tiles_p + tp) * (T::FP * T::FQ * T::THREADS) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < T::FP; ++i)
@@ -299,7 +299,7 @@ __device__ __forceinline__ void logits(const A& a, int64_t p0, int64_t q0, char*
 #pragma unroll
                 for (int j = 0; j < T::FQ; ++j) acc[i][j] += o[k * all + (i * T::FQ + j) * T::THREADS];
     } else {
-        mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, ((a.kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), SPLIT, lds, acc);
+        mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, 0, ((a.kbytes + 127) >> 7) * (SPLIT ? MM_SEGMENTS : 1), SPLIT ? MM_SEGMENTS : 1, lds, acc);
     }
 #ifdef __HIP_DEVICE_COMPILE__
     const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
@@ -685,6 +685,7 @@ struct GradArgs {
     Walk walk;
     const float *ref, *inv, *mean, *tsum;
     Factor f;
+    int32_t two;           // 16 bits: G in two planes
     char* g;               // [rows][g_pitch] per plane, or null (no dx wanted)
     int64_t g_pitch, g_plane;
     char* gt;              // [classes of the piece][gt_pitch] per plane, or null (no dW wanted)
@@ -789,7 +790,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_ce_grad(GradArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 v[r] = acc[i][j][r] * by;
-                if constexpr (P == 1) v[r] = (v[r] - (float)(_Float16)v[r]) * 2048.0f;      // G is finite in float16: hold_scale
+                if constexpr (P == 1 && DT == DT_BF16) v[r] -= (float)(__bf16)v[r];
+                else if constexpr (P == 1) v[r] = (v[r] - (float)(_Float16)v[r]) * 2048.0f;      // G is finite in float16: hold_scale
             }
             return pack4<DT == DT_BF16 ? DT_BF16 : DT_F16>(v[0], v[1], v[2], v[3]);
         };
@@ -807,9 +809,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_ce_grad(GradArgs a) {
         }
     };
     emit(std::integral_constant<int, 0>{});
-    if constexpr (DT == DT_F32) {
-        mm_opaque<T>(acc);       // the planes are made one after another: both would not fit the registers
-        emit(std::integral_constant<int, 1>{});
+    if constexpr (DT == DT_F32 || T::BP < 256) {
+        if (DT == DT_F32 || a.two) {
+            mm_opaque<T>(acc);       // the planes are made one after another: both would not fit the registers
+            emit(std::integral_constant<int, 1>{});
+        }
     }
 }
 
@@ -824,15 +828,16 @@ struct OutArgs {
     Factor f;
 };
 
-template <class T, int DT>
+// SEGMENTS of the walk: three for float32, two for 16 bits with G in two planes.
+template <class T, int DT, int SEGMENTS>
 __device__ __forceinline__ void out_tile(const OutArgs& a, int id, char* lds) {
     const int tiles = a.tiles_p * a.tiles_q, split = id / tiles;
     int tp, tq;
     mm_place(id - split * tiles, a.tiles_p, a.tiles_q, tp, tq);
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
-    const int steps = ((a.kbytes + 127) >> 7) * (DT == DT_F32 ? MM_SEGMENTS : 1), begin = split * a.per;
-    mm_tile<T>(a.p, a.q, p0, q0, a.kbytes, begin, begin + a.per < steps ? begin + a.per : steps, DT == DT_F32, lds, acc);
+    const int steps = ((a.kbytes + 127) >> 7) * SEGMENTS, begin = split * a.per;
+    mm_tile<T>(a.p, a.q, p0, q0, a.kbytes, begin, begin + a.per < steps ? begin + a.per : steps, SEGMENTS, lds, acc);
     const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     const int64_t width = a.p.rows;
     const bool first = a.first || a.splits > 1, last = a.last && a.splits == 1;
@@ -918,12 +923,12 @@ __device__ __forceinline__ void bias_block(const BiasArgs& a, int64_t m) {
 }
 
 // dx, dW and db of a piece in one launch: they share nothing but G, and small ones fill the chip together.
-template <class T, int DT>
+template <class T, int DT, int SEGMENTS>
 __global__ __launch_bounds__(T::THREADS) void k_ce_out(OutArgs a, OutArgs b, BiasArgs c, int blocks_a, int blocks_b) {
     __shared__ __align__(16) char lds[T::LDS];
     const int id = blockIdx.x;
-    if (id < blocks_a) out_tile<T, DT>(a, id, lds);
-    else if (id < blocks_a + blocks_b) out_tile<T, DT>(b, id - blocks_a, lds);
+    if (id < blocks_a) out_tile<T, DT, SEGMENTS>(a, id, lds);
+    else if (id < blocks_a + blocks_b) out_tile<T, DT, SEGMENTS>(b, id - blocks_a, lds);
     else bias_block<DT>(c, (int64_t)(id - blocks_a - blocks_b) * T::THREADS + threadIdx.x);
 }
 
@@ -951,7 +956,8 @@ struct Layout {       // of the workspace, and the pieces of the classes
     int grid = 0, chunks = 0, chunk = 0;      // of those: workgroups; chunks of the classes, classes of a chunk
     bool split;              // float32
     bool pack_w, pack_x;     // operands copied into rows of whole 16 bytes
-    int planes;         // 16-bit planes of an operand
+    int planes, g_planes;         // 16-bit planes of an operand, and of G
+    int edge_most = 256;          // largest tile of the backward pass
     int64_t kpitch;     // bytes of an operand's row as the tile loop reads it (when packed)
     int64_t piece;      // classes of a piece
     int pieces;
@@ -970,6 +976,12 @@ bool in_place(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p
 void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.split = a.dtype == AZ_DT_F32;
     l.planes = l.split ? 2 : 1;
+    // With few rows a handful of values (the targets) are most of G, and the rounding of each to 16 bits shows in the gradients: 1.6 times
+    // the error of their own type's rounding with up to 40 rows, 1.45 with 100, 1.4 and steady beyond. There G takes two planes: 1.0,
+    // for 8 to 20 % of the two passes' time (64 x 4096 -> 4096 bfloat16: 77 us, now 91; 64 x 722 -> 362 34, now 39).
+    const bool two = !l.split && a.rows <= 128;
+    l.g_planes = l.split || two ? 2 : 1;
+    if (two) l.edge_most = 128;
     l.pack_w = l.split || !in_place(a.weight, a.weight_pitch, a.features);
     l.pack_x = l.split || !in_place(a.x, a.x_pitch, a.features);
     l.kpitch = round_up(a.features, 8) * 2;
@@ -1027,13 +1039,13 @@ bool few_forward(const az_linear_ce_args& a) {
     return a.rows <= 16 && !in_place(a.weight, a.weight_pitch, a.features) && a.classes * a.features > (int64_t(1) << 26);
 }
 // Backward: streaming saves the turned copies of the weight and G, its sums over the classes grow with the rows. 16 bits: 4096 -> 8000 4 rows 51 us
-// against 88, 16 rows 74 against 89; 4096 -> 1000 4 rows 31 against 28, 16 rows 45 against 28; copied 2047 -> 16000 116 to 147 against
-// 132, 4095 -> 32000 489 against 500. float32: 4096 -> 1000 1 row 35 against 50, 16 rows 56 against 52; 16 x 1024 -> 200 34 against 23.
+// against 100, 16 rows 74 against 101; 4096 -> 1000 4 rows 31 against 32, 16 rows 45 against 32; copied 2047 -> 16000 116 to 147 against
+// 140, 4095 -> 32000 489 against 540. float32: 4096 -> 1000 1 row 35 against 50, 16 rows 56 against 52; 16 x 1024 -> 200 34 against 23.
 bool few_backward(const az_linear_ce_args& a) {
     const int64_t size = a.classes * a.features;
     if (a.rows > FEW_GRAD_ROWS || a.features > 16 * a.classes || a.features < 256) return false;      // 256 lanes take 4 features each
     if (a.dtype == AZ_DT_F32) return size >= a.rows * (3 << 16);
-    return size >= a.rows * (3 << 19) && (size >= int64_t(1) << 25 || in_place(a.weight, a.weight_pitch, a.features));
+    return size >= a.rows << 20 && (size >= int64_t(1) << 25 || in_place(a.weight, a.weight_pitch, a.features));
 }
 
 Layout forward_layout(const az_linear_ce_args& a) {
@@ -1097,9 +1109,10 @@ struct OutPlan {
 OutPlan out_plan(const az_linear_ce_args& a, const Layout& l, int64_t nv) {
     OutPlan best{};
     double least = 1e300;
-    const int walks = l.split ? MM_SEGMENTS : 1;
+    const int walks = l.split ? MM_SEGMENTS : l.g_planes;
     const int64_t steps_x = round_up(nv, 64) / 64 * walks, steps_w = round_up(a.rows, 64) / 64 * walks;
     for (const MmTileCost& c : MM_TILE_COSTS) {
+        if (c.edge > l.edge_most) continue;
         OutPlan o;
         o.edge = c.edge;
         auto tiles = [&](int64_t n) { return (int)((n + o.edge - 1) / o.edge); };
@@ -1147,7 +1160,7 @@ Layout backward_layout(const az_linear_ce_args& a) {
     operand_layout(a, l);
     const int64_t np = round_up(a.rows, 64);
     // G and its transpose of a piece stay at about 1 GB: then the sums of dx that travel between pieces cost a few per cent
-    int64_t piece = (int64_t(1) << 30) / (np * 4 * l.planes) / 256 * 256;
+    int64_t piece = (int64_t(1) << 30) / (np * 4 * l.g_planes) / 256 * 256;
     if (l.pack_w) {
         const int64_t w = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
         if (w < piece) piece = w;
@@ -1160,8 +1173,8 @@ Layout backward_layout(const az_linear_ce_args& a) {
     if (l.pack_w) l.wp = l.take(l.piece * l.kpitch * l.planes);
     l.xt = l.take(a.features * np * 2 * l.planes);
     l.wt = l.take(a.features * vp * 2 * l.planes);
-    l.g = l.take(a.rows * vp * 2 * l.planes);
-    l.gt = l.take(l.piece * np * 2 * l.planes);
+    l.g = l.take(a.rows * vp * 2 * l.g_planes);
+    l.gt = l.take(l.piece * np * 2 * l.g_planes);
     l.db = l.take((a.rows + 63) / 64 * l.piece * 4);      // the smallest tiles make the most sums
     if (l.pieces > 1) l.sum = l.take(a.rows * a.features * 4);
     // sums of split walks, for the piece that splits most
@@ -1400,6 +1413,7 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     s.mean = kept.mean;
     s.tsum = kept.tsum;
     s.f = f;
+    s.two = !l.split && l.g_planes == 2;
     s.g = gx ? ws + l.g : nullptr;
     s.g_pitch = vp * 2;
     s.g_plane = a.rows * vp * 2;
@@ -1420,7 +1434,8 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         s.g_plane = a.rows * vpi * 2;
         s.v0 = (int)v0;
         s.db_pitch = nv;
-        const LogitPlan logit = logit_plan(a, nv);
+        LogitPlan logit = logit_plan(a, nv);
+        if (logit.edge > l.edge_most) logit.edge = l.edge_most;
         const int edge = logit.edge;
         s.tiles_p = (int)((nv + edge - 1) / edge);
         s.tiles_q = (int)((a.rows + edge - 1) / edge);
@@ -1464,14 +1479,18 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         const bool swap = plan.w.per > plan.x.per;
         const OutArgs &longer = swap ? ow : ox, &second = swap ? ox : ow;
         const int64_t ba = swap ? bw : bx, bs = swap ? bx : bw;
-        auto run = [&](auto tile) {
+        auto run = [&](auto tile, auto segments) {
             typedef decltype(tile) T;
             const int64_t bb = (ob.classes + T::THREADS - 1) / T::THREADS;
-            hipLaunchKernelGGL((k_ce_out<T, DT>), dim3((unsigned)(ba + bs + bb)), dim3(T::THREADS), 0, st, longer, second, ob, (int)ba, (int)bs);
+            hipLaunchKernelGGL((k_ce_out<T, DT, decltype(segments)::value>), dim3((unsigned)(ba + bs + bb)), dim3(T::THREADS), 0, st, longer, second, ob, (int)ba, (int)bs);
         };
-        if (plan.edge == 256) run(typename Tiles<DT>::Big{});
-        else if (plan.edge == 128) run(typename Tiles<DT>::Mid{});
-        else run(typename Tiles<DT>::Small{});
+        const std::integral_constant<int, DT == DT_F32 ? MM_SEGMENTS : 1> usual;
+        const std::integral_constant<int, DT == DT_F32 ? MM_SEGMENTS : 2> two;
+        if (plan.edge == 256) run(typename Tiles<DT>::Big{}, usual);
+        else if (plan.edge == 128 && s.two) run(typename Tiles<DT>::Mid{}, two);
+        else if (plan.edge == 128) run(typename Tiles<DT>::Mid{}, usual);
+        else if (s.two) run(typename Tiles<DT>::Small{}, two);
+        else run(typename Tiles<DT>::Small{}, usual);
         if (const int rc = launched("k_ce_out")) return rc;
         const int64_t jx = bx && ox.splits > 1 ? (a.rows * a.features + 255) / 256 : 0, jw = bw && ow.splits > 1 ? (nv * a.features + 255) / 256 : 0;
         if (jx + jw) hipLaunchKernelGGL((k_ce_out_join<DT>), dim3((unsigned)(jx + jw)), dim3(256), 0, st, ox, ow, jx);

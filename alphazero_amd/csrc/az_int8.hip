@@ -214,7 +214,7 @@ __global__ __launch_bounds__(T::THREADS) void k_int8_tile(TileArgs a) {
     const int64_t p0 = (int64_t)tp * T::BP, q0 = (int64_t)tq * T::BQ;
     typename T::acc_t acc[T::FP][T::FQ];
     const int steps = (a.kbytes + 127) >> 7, first = piece * a.per, last = first + a.per < steps ? first + a.per : steps;
-    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, first, last, false, lds, acc);
+    mm_tile<T>(a.w, a.x, p0, q0, a.kbytes, first, last, 1, lds, acc);
     const int lane = mm_lane_after(), wave = threadIdx.x >> 6, wp = wave / T::WQ, wq = wave % T::WQ;
     if (a.splits > 1) {
         i32x4* o = a.part + (((int64_t)piece * tiles + tp * a.tiles_q + tq) * (T::FP * T::FQ)) * T::THREADS + threadIdx.x;

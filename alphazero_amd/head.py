@@ -138,7 +138,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
 
     An index outside 0..classes-1 that is not ignore_index gives a NaN loss and NaN gradients (the check is on the device, nothing
     waits for it). Everything is accumulated in float32; the gradient of the logits is rounded to the inputs' 16-bit type between the
-    products (float32 inputs keep 24 bits). Scratch memory for the backward pass stays near 1 GB whatever the number of classes."""
+    products with more than 128 rows, and keeps 16 bits or more with fewer (float32 inputs: 22). Scratch memory for the backward pass stays near 1 GB whatever the number of classes."""
     _on_gpu("linear_cross_entropy", x, weight, target, bias)
     _need(reduction in _REDUCE, 'reduction is "none", "mean" or "sum"')
     _need(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1], f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")

@@ -89,6 +89,29 @@ def test_long_features(size, dtype, dense):
     _check(x, w, b, t, c=0.01 if size[0] > 100 else 0.0, reduction="sum" if size[0] == 70 else "mean")
 
 
+@pytest.mark.parametrize("rows", [1, 3, 17, 40, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+@pytest.mark.parametrize("size", [(759, 369), (72, 2000), (4096, 130)], ids=ids)
+def test_gradients_of_few_rows_keep_their_type(size, dtype, dense, rows):
+    """With few rows the gradient of the logits is held in more than 16 bits: what is left is the rounding of the results (half a step) and
+    16 bits or more of each term of their sums, 2^-15 with the float32 sums' own."""
+    x, w, b, t = _inputs(rows, *size, dtype, dense, True)
+    got = _run(x, w, b, t, torch.tensor(64.0, device="cuda"), reduction="sum")
+    z = x.double() @ w.double().t() + b.double()
+    if dense:
+        pi = t.double()
+    else:
+        pi = torch.zeros_like(z)
+        live = t != -100
+        pi[live, t[live]] = 1.0
+    g = 64.0 * (pi.sum(1, keepdim=True) * torch.softmax(z, 1) - pi)
+    size_g = 64.0 * (pi.sum(1, keepdim=True) * torch.softmax(z, 1) + pi)      # of what g is the difference of, for its softmax' float32
+    for name, v, want, terms in (("gx", got[3], g @ w.double(), size_g @ w.double().abs()), ("gw", got[4], g.t() @ x.double(), size_g.t() @ x.double().abs())):
+        half = torch.finfo(dtype).eps / 2
+        R.close(name, v, (want, half * want.abs() + 2.0 ** -15 * terms + R.TINY[dtype]))
+
+
 # a few rows of a large weight take the kernels that stream it: both passes, only the backward one (16 bits, read in place)
 @pytest.mark.parametrize("size", [(1, 1032, 33000), (2, 1032, 33000), (4, 1032, 33000), (7, 2056, 17000), (16, 1032, 33000), (16, 1025, 66000), (3, 1025, 66001),
                                   (30, 1025, 66001), (9, 72, 66001)], ids=ids)
