@@ -1038,14 +1038,15 @@ bool few_forward(const az_linear_ce_args& a) {
     if (a.dtype == AZ_DT_F32) return a.rows <= 32 && (a.features <= 1024 || a.features <= 4 * a.classes);
     return a.rows <= 16 && !in_place(a.weight, a.weight_pitch, a.features) && a.classes * a.features > (int64_t(1) << 26);
 }
-// Backward: streaming saves the turned copies of the weight and G, its sums over the classes grow with the rows. 16 bits: 4096 -> 8000 4 rows 51 us
-// against 100, 16 rows 74 against 101; 4096 -> 1000 4 rows 31 against 32, 16 rows 45 against 32; copied 2047 -> 16000 116 to 147 against
-// 140, 4095 -> 32000 489 against 540. float32: 4096 -> 1000 1 row 35 against 50, 16 rows 56 against 52; 16 x 1024 -> 200 34 against 23.
+// Backward: streaming saves the turned copies of the weight and G, its sums over the classes grow with the rows (streaming against tiles, us).
+// 16 bits: 4096 -> 8000 4 rows 49, 100, 16 rows 71, 100; 2048 -> 4000 8 rows 37, 46, 16 rows 46, 46; 4096 -> 1000 4 rows 30, 38, 16 rows 45, 38;
+// 1024 -> 200 4 rows 23, 19; copied 2047 -> 16000 1 row 114, 142, 16 rows 142, 140. float32: 2048 -> 4000 16 rows 51, 75; 2048 -> 1000
+// 4 rows 29, 40, 16 rows 43, 40; 1024 -> 200 1 row 19, 23, 8 rows 27, 24.
 bool few_backward(const az_linear_ce_args& a) {
     const int64_t size = a.classes * a.features;
     if (a.rows > FEW_GRAD_ROWS || a.features > 16 * a.classes || a.features < 256) return false;      // 256 lanes take 4 features each
     if (a.dtype == AZ_DT_F32) return size >= a.rows * (3 << 16);
-    return size >= a.rows << 20 && (size >= int64_t(1) << 25 || in_place(a.weight, a.weight_pitch, a.features));
+    return size >= a.rows << 19 && (size >= int64_t(1) << 24 || in_place(a.weight, a.weight_pitch, a.features));
 }
 
 Layout forward_layout(const az_linear_ce_args& a) {
