@@ -663,6 +663,44 @@ def test_captured_and_replayed():
             assert torch.equal(a, v) and torch.equal(a, u)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+def test_split_walks_captured_and_at_once(dtype):
+    """Products whose walk is in pieces, in one graph and on two streams at once: each call has its own scratch memory."""
+    head = _head()
+    x, w, b, t = _inputs(70, 6000, 90, dtype, False, True)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    q, ws = head.quantize_rows(w.detach())
+    one = torch.ones((), device="cuda")
+
+    def step():
+        loss = head.linear_cross_entropy(x, w, t, b, entropy_coeff=0.01)
+        gx, gw = torch.autograd.grad(loss, (x, w), one)
+        return loss.detach(), gx, gw, head.int8_linear(x.detach(), q, ws)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(70, 6000, device="cuda") * (k + 1))
+        want = [v.clone() for v in step()]
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            there = step()
+        here = step()
+        torch.cuda.synchronize()
+        for a, v, u, h in zip(want, out, there, here):
+            assert torch.equal(a, v) and torch.equal(a, u) and torch.equal(a, h)
+
+
 # ------------------------------------------------------------------------------------------------ the framework's own callers
 def _net_and_batch(seed=0, n=5, rows=48):
     import stubnets
