@@ -3,13 +3,15 @@ with its gradient (the logits are never stored), dropout from a counter-based ge
 in 8-bit integers with a scale for each token and channel.
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the tensors' device; there is no CPU
-fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two."""
+fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two.
+Derivatives are reverse-mode ones: a dual tensor (torch.autograd.forward_ad) is refused."""
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -30,6 +32,9 @@ def _on_gpu(name: str, x: torch.Tensor, *others):
     for t in others:
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
+    # a dual tensor does not ask for a gradient: without this its tangent would be lost and the derivative read as zero
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, *others)):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _ptr(t):

@@ -1,0 +1,25 @@
+"""Calls of alphazero_amd.head that have to be refused rather than answered wrongly, on stand-ins for GPU tensors."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from alphazero_amd import head
+from test_head_cpu import _fake
+
+
+def test_forward_mode_is_refused():
+    """A tangent that the kernels do not carry would come back as a derivative of zero."""
+    with forward_ad.dual_level():
+        def dual(*shape):
+            return forward_ad.make_dual(_fake(*shape), torch.ones(shape))
+        x, w8, ones = _fake(3, 8), _fake(5, 8, dtype=torch.int8), _fake(5)
+        t = _fake(3, dtype=torch.int64)
+        for call in (lambda: head.dropout(dual(3, 8), 0.5, 1), lambda: head.dropout(x, 0.5, 1, residual=dual(3, 8)), lambda: head.quantize_rows(dual(3, 8)),
+                     lambda: head.int8_linear(dual(3, 8), w8, ones), lambda: head.int8_linear(x, w8, dual(5)), lambda: head.int8_linear(x, w8, ones, dual(5)),
+                     lambda: head.int8_linear(_fake(3, 8, dtype=torch.int8), w8, ones, x_scale=dual(3)),
+                     lambda: head.linear_cross_entropy(dual(3, 8), _fake(5, 8), t), lambda: head.linear_cross_entropy(x, dual(5, 8), t),
+                     lambda: head.linear_cross_entropy(x, _fake(5, 8), t, dual(5)), lambda: head.linear_cross_entropy(x, _fake(5, 8), dual(3, 5))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="probability"):        # without a tangent the call goes on, to its next check
+            head.dropout(x, 2.0, 1)
