@@ -4,7 +4,8 @@ in 8-bit integers with a scale for each token and channel.
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the tensors' device; there is no CPU
 fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two.
-Derivatives are reverse-mode ones: a dual tensor (torch.autograd.forward_ad) is refused."""
+Derivatives are reverse-mode ones: a dual tensor (torch.autograd.forward_ad) is refused, and so is a call under torch.jit.trace or
+make_fx, whose record would lack the kernels; torch.cuda.graph captures them."""
 from __future__ import annotations
 
 import ctypes as C
@@ -13,6 +14,7 @@ import torch
 from torch import nn
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _native as N
 
@@ -25,6 +27,12 @@ def _need(ok: bool, what: str):
         raise ValueError(what)
 
 
+def _recorded() -> bool:
+    """The call is being recorded by torch.jit.trace or make_fx. They see torch operations only: the record would allocate the result and
+    return it as it is, without the kernel that fills it."""
+    return torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() > 0 and get_proxy_mode() is not None)
+
+
 def _on_gpu(name: str, x: torch.Tensor, *others):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise N.NativeError(f"alphazero_amd.head.{name} needs tensors on a GPU (no CPU fallback)")
@@ -32,6 +40,8 @@ def _on_gpu(name: str, x: torch.Tensor, *others):
     for t in others:
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
+    if _recorded():
+        raise NotImplementedError(f"{name} cannot be traced: capture it into a HIP graph (torch.cuda.graph) instead")
     # a dual tensor does not ask for a gradient: without this its tangent would be lost and the derivative read as zero
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, *others)):
         raise NotImplementedError(f"{name} has no forward-mode derivative")

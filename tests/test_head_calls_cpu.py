@@ -23,3 +23,25 @@ def test_forward_mode_is_refused():
                 call()
         with pytest.raises(ValueError, match="probability"):        # without a tangent the call goes on, to its next check
             head.dropout(x, 2.0, 1)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recording_is_refused():
+    """torch.jit.trace and make_fx record torch operations: the result's allocation, and none of the kernels."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w8, ones, t = _fake(3, 8), _fake(5, 8, dtype=torch.int8), _fake(5), _fake(3, dtype=torch.int64)
+    layer = head.Int8Linear.__new__(head.Int8Linear)
+    torch.nn.Module.__init__(layer)
+    layer.in_features, layer.out_features = 8, 5
+    for name, v in (("qweight", w8), ("weight_scale", ones), ("bias", None)):
+        layer.register_buffer(name, v)
+    calls = (lambda: head.dropout(x, 0.5, 1), lambda: head.quantize_rows(x)[1], lambda: head.int8_linear(x, w8, ones), lambda: layer(x),
+             lambda: head.linear_cross_entropy(x, _fake(5, 8), t))
+    for call in calls:
+        def one(v):
+            return v + call()
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            torch.jit.trace(one, torch.zeros(()), check_trace=False)
+    for call in calls[:3] + calls[4:]:
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            make_fx(lambda v: v + call())(torch.zeros(()))
