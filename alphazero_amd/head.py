@@ -311,5 +311,16 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        """half(), bfloat16(), to(dtype) and type() are about the bias and the inputs: the 8-bit weights and their float32 scales are moved,
+        never cast."""
+        kept = {name: getattr(self, name) for name in ("qweight", "weight_scale")}
+        super()._apply(fn, recurse)
+        for name, v in kept.items():
+            now = getattr(self, name)
+            if now.dtype != v.dtype:
+                setattr(self, name, v.to(now.device))
+        return self
+
     def forward(self, x):
         return int8_linear(x.detach(), self.qweight[:, :self.in_features], self.weight_scale, self.bias)

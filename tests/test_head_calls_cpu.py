@@ -45,3 +45,32 @@ def test_recording_is_refused():
     for call in calls[:3] + calls[4:]:
         with pytest.raises(NotImplementedError, match="cannot be traced"):
             make_fx(lambda v: v + call())(torch.zeros(()))
+
+
+def _layer(bias=True):
+    """An Int8Linear as its constructor leaves it, on the CPU."""
+    layer = head.Int8Linear.__new__(head.Int8Linear)
+    torch.nn.Module.__init__(layer)
+    layer.in_features, layer.out_features = 18, 5
+    layer.register_buffer("qweight", torch.randint(-127, 128, (5, 32)).to(torch.int8))
+    layer.register_buffer("weight_scale", torch.rand(5))
+    layer.register_buffer("bias", torch.rand(5) if bias else None)
+    return layer
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_int8_layer_keeps_its_weights_under_casts(bias):
+    for cast, kind in ((lambda m: m.half(), torch.float16), (lambda m: m.bfloat16(), torch.bfloat16), (lambda m: m.to(torch.float16), torch.float16),
+                       (lambda m: m.to("cpu", torch.bfloat16), torch.bfloat16), (lambda m: m.type(torch.float16), torch.float16),
+                       (lambda m: torch.nn.Sequential(m).half()[0], torch.float16), (lambda m: m.half().float(), torch.float32),
+                       (lambda m: m.to("cpu"), torch.float32)):
+        layer = _layer(bias)
+        q, s = layer.qweight.clone(), layer.weight_scale.clone()
+        m = cast(layer)
+        assert m is layer and m.qweight.dtype == torch.int8 and torch.equal(m.qweight, q)
+        assert m.weight_scale.dtype == torch.float32 and torch.equal(m.weight_scale, s)
+        assert set(m.state_dict()) == {"qweight", "weight_scale"} | ({"bias"} if bias else set())
+        if bias:
+            assert m.bias.dtype == kind
+    there = _layer(bias).to("meta", torch.float16)
+    assert there.qweight.is_meta and there.weight_scale.is_meta and there.weight_scale.dtype == torch.float32
