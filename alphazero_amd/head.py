@@ -298,7 +298,8 @@ def _int8_refuse(x, qweight, weight_scale, bias, x_scale, out_dtype):
 
 class Int8Linear(nn.Module):
     """A linear layer whose weights are held in 8 bits with a scale per output channel and whose input is quantised per row: the
-    serving form of a trained nn.Linear (on a GPU). Rows are laid out at multiples of 16 bytes once, here."""
+    serving form of a trained nn.Linear (on a GPU). Rows are laid out at multiples of 16 bytes once, here. As with int8_linear there is
+    no gradient: an input that asks for one is refused."""
 
     def __init__(self, linear: nn.Linear):
         super().__init__()
@@ -323,4 +324,4 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x):
-        return int8_linear(x.detach(), self.qweight[:, :self.in_features], self.weight_scale, self.bias)
+        return int8_linear(x, self.qweight[:, :self.in_features], self.weight_scale, self.bias)

@@ -74,3 +74,13 @@ def test_int8_layer_keeps_its_weights_under_casts(bias):
             assert m.bias.dtype == kind
     there = _layer(bias).to("meta", torch.float16)
     assert there.qweight.is_meta and there.weight_scale.is_meta and there.weight_scale.dtype == torch.float32
+
+
+def test_int8_layer_has_no_gradient_and_says_so():
+    layer = _layer()
+    for name in ("qweight", "weight_scale", "bias"):
+        setattr(layer, name, getattr(layer, name).as_subclass(_fake(1).__class__))
+    with pytest.raises(ValueError, match="no gradient"):
+        layer(_fake(3, 18).requires_grad_(True))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        layer(forward_ad.make_dual(_fake(3, 18), torch.ones(3, 18)))
