@@ -42,6 +42,7 @@ struct MmOperand {
     int64_t pitch;       // bytes between rows, a multiple of 16, at most MM_MAX_PITCH
     int64_t plane;       // bytes between the planes of a split float32 operand
     int32_t rows;
+    int32_t short_by;    // bytes that the last row lacks of kbytes (fewer than 16): they are not read and count as zero
 };
 constexpr int64_t MM_MAX_PITCH = (int64_t(1) << 31) / 256 - 16;   // 256 rows of a tile stay below 2^31 bytes
 
@@ -95,7 +96,7 @@ __device__ __forceinline__ void mm_tile(const MmOperand& P, const MmOperand& Q, 
     const char* const pbase = P.base + p0 * P.pitch;
     const char* const qbase = Q.base + q0 * Q.pitch;
     // bytes from the tile's first row to the end of the matrix' last row; below zero (an empty tile) reads nothing
-    const int64_t pext = ((int64_t)P.rows - p0 - 1) * P.pitch + kbytes, qext = ((int64_t)Q.rows - q0 - 1) * Q.pitch + kbytes;
+    const int64_t pext = ((int64_t)P.rows - p0 - 1) * P.pitch + kbytes - P.short_by, qext = ((int64_t)Q.rows - q0 - 1) * Q.pitch + kbytes - Q.short_by;
     int ks = segments > 1 ? k_first / ksteps : 0;      // segment and step within it of the next stage to fetch
     int kk = k_first - ks * ksteps;
     int left = k_last - k_first;                // stages still to fetch

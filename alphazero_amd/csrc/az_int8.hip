@@ -478,17 +478,22 @@ struct Plan {
 Plan plan_of(const az_int8_args& a) {
     Plan p;
     p.kpitch = round_up(a.features, 16);
-    auto crooked = [&](const void* q, int64_t pitch) { return (((uintptr_t)q | (uintptr_t)pitch) & 15) != 0 || (a.features & 15) != 0 || pitch > MM_MAX_PITCH; };
+    auto crooked = [&](const void* q, int64_t pitch) { return (((uintptr_t)q | (uintptr_t)pitch) & 15) != 0 || pitch > MM_MAX_PITCH; };
     const bool copy = crooked(a.weight, a.weight_pitch);
     // Where the kernel for few tokens takes the place of the tiles. From 16384 channels on the tiles fill the chip in one walk (one int8 token,
     // 1024 -> 32000: 8.3 us against 13.6; 4096 -> 32000: 23.6 against 27). Below, they join pieces of k in a second launch (16 x 4096 ->
     // 4096: 11.4 against 9.2, 16 x 4096 -> 8000 13.1 against 9.6, 48 x 1024 -> 4096 8.7 against 7.5), which pays with more tokens and with
     // longer walks (32 x 4096 -> 1024 8.7 against 10.7, 16 x 8192 -> 1024 10 against 14, 64 x 4096 -> 32000 24.8 against 76). A weight that the
-    // tiles have to copy: 4 x 4095 -> 4096 22 against 24, 32 x 4095 -> 4096 23 against 36. One or two floating tokens are quantised in
+    // tiles have to copy: 4 x 4095 -> 4096 22 against 24, 32 x 4095 -> 4096 23 against 36. A weight that they read in place, its rows ending
+    // inside 16 bytes, meets this kernel's byte-by-byte end of a row: tiles (floating tokens, few against tiles: 3 x 162 -> 82 7.5 and 6.2, 16 x
+    // 722 -> 362 14.3 and 8.1, 48 x 2047 -> 4096 14.9 and 13.0), but for up to 4 int8 tokens, which the tiles would have to copy (4 x 162 -> 82
+    // 4.6 and 5.8, 4 x 4095 -> 4096 12.4 and 12.5, though 4 x 722 -> 362 9.2 and 7.0). One or two floating tokens are quantised in
     // the same launch, also for more channels where a row is long (1 x 14336 -> 4096 bfloat16: 17 us against 23, 1 x 4096 -> 16384 14.3 against
     // 16.3, 1 x 1024 -> 32000 16.7 against 11.7; four tokens 14336 -> 4096 29 against 25).
     const bool small = a.channels < 16384;
-    p.few = small && a.features <= 4096 && a.tokens <= (copy ? 4 : a.features <= 2048 ? FEW_TOKENS : 16);
+    const bool ragged = (a.features & 15) != 0;
+    const int most = copy || (ragged && a.x_dtype == AZ_DT_I8) ? 4 : ragged ? 0 : a.features <= 2048 ? FEW_TOKENS : 16;
+    p.few = small && a.features <= 4096 && a.tokens <= most;
     p.fused = (small || a.channels <= 4 * a.features) && a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
     if (p.fused) return p;
     if (a.x_dtype != AZ_DT_I8) {
@@ -497,7 +502,9 @@ Plan plan_of(const az_int8_args& a) {
     }
     if (p.few) return p;
     p.align_w = copy;
-    p.align_x = a.x_dtype == AZ_DT_I8 && crooked(a.x, a.x_pitch);
+    // A weight's row may end inside its last 16 bytes: what lies behind it meets the zeros behind a token's last feature, which quantising or
+    // copying the token puts there. So one of the two is copied where features are not a multiple of 16, and that is the tokens.
+    p.align_x = a.x_dtype == AZ_DT_I8 && (crooked(a.x, a.x_pitch) || ragged);
     if (p.align_w) p.w = p.take(a.channels * p.kpitch);
     if (p.align_x) p.x = p.take(a.tokens * p.kpitch);
     auto tiles = [&](int64_t e) { return ((a.channels + e - 1) / e) * ((a.tokens + e - 1) / e); };
@@ -639,7 +646,8 @@ int product(const az_int8_args& a, const Plan& p, const int8_t* x, int64_t x_pit
         x_pitch = p.kpitch;
     }
     TileArgs t{};
-    t.w = MmOperand{(const char*)w, w_pitch, 0, (int)a.channels};
+    // the last row is read up to the 4 bytes that hold its last feature
+    t.w = MmOperand{(const char*)w, w_pitch, 0, (int)a.channels, p.align_w ? 0 : (int)(p.kpitch - a.features) & ~3};
     t.s = s;
     t.kbytes = (int)p.kpitch;
     t.tiles_p = (int)((a.channels + p.edge - 1) / p.edge);

@@ -30,3 +30,32 @@ def test_int8_layer_cast_with_its_module(dtype, tokens):
     with torch.no_grad():
         y = cast(x)
     assert y.dtype == dtype and torch.equal(y, want)
+
+
+# ragged and whole pieces of 16 bytes; few tokens, tiles of each size, walks in pieces
+PADDED = [(40, 162, 82), (70, 722, 362), (256, 722, 362), (100, 17, 33), (64, 4095, 300), (300, 129, 517), (2304, 250, 5632), (20, 8201, 70), (65, 3, 65), (49, 15, 1), (1, 162, 82),
+          (2, 2047, 600), (3, 722, 362), (4, 162, 82), (5, 4095, 300), (16, 2047, 600), (4, 4095, 16500)]
+
+
+@pytest.mark.parametrize("size", PADDED, ids=ids)
+def test_int8_rows_that_end_inside_16_bytes(size):
+    """Rows at multiples of 16 bytes with anything between them, the last one at the end of its memory, against a dense weight."""
+    head = _head()
+    m, k, n = size
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x = torch.randn((m, k), generator=g, device="cuda")
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda").to(torch.int8)
+    ws = torch.rand(n, generator=g, device="cuda") / 127
+    q, s = head.quantize_rows(x)
+    want = ((q.double() @ w.double().t()).float() * s[:, None]) * ws      # the sum is exact, then two roundings
+    pitch = (k + 15) // 16 * 16
+    for fill in (77, -128):
+        for extra in (0, 16, 48):
+            store = torch.full(((n - 1) * (pitch + extra) + k,), fill, dtype=torch.int8, device="cuda")
+            rows = store.as_strided((n, k), (pitch + extra, 1))
+            rows.copy_(w)
+            assert torch.equal(head.int8_linear(x, rows, ws), want)
+            q8 = torch.full((m, pitch + extra), fill, dtype=torch.int8, device="cuda")
+            q8[:, :k] = q
+            assert torch.equal(head.int8_linear(q8[:, :k], rows, ws, x_scale=s), want)
+            assert torch.equal(head.int8_linear(q8[:, :k], w, ws, x_scale=s), want)

@@ -1,8 +1,11 @@
 """Calls of alphazero_amd.head that have to be refused rather than answered wrongly, on stand-ins for GPU tensors."""
+import ctypes as C
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from alphazero_amd import _native as N
 from alphazero_amd import head
 from test_head_cpu import _fake
 
@@ -84,3 +87,19 @@ def test_int8_layer_has_no_gradient_and_says_so():
         layer(_fake(3, 18).requires_grad_(True))
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         layer(forward_ad.make_dual(_fake(3, 18), torch.ones(3, 18)))
+
+
+def test_padded_int8_weights_are_read_in_place():
+    """The layout of Int8Linear, rows at multiples of 16 bytes: no scratch memory for a copy, whatever the number of features."""
+    L = N.lib()
+    for tokens, features, channels in ((256, 722, 362), (60, 162, 82), (32, 4095, 4096), (300, 17, 5000)):
+        pitch = (features + 15) // 16 * 16
+
+        def size(**change):
+            good = dict(x=256, weight=512, x_scale=None, weight_scale=768, bias=None, y=1024, tokens=tokens, features=features, channels=channels, x_pitch=pitch,
+                        weight_pitch=pitch, x_dtype=N.AZ_DT_F32, bias_dtype=0, y_dtype=N.AZ_DT_F32)
+            return L.az_int8_workspace(C.byref(N.AzInt8Args(**(good | change))))
+        assert size() == size(features=pitch)
+        assert size(weight=513) >= size() + channels * pitch and size(weight_pitch=pitch + 1) >= size() + channels * pitch
+        eight = dict(x_dtype=N.AZ_DT_I8, x_scale=256)      # 8-bit tokens: they are copied instead, with zeros behind their last feature
+        assert size(**eight) >= size(features=pitch, **eight) + tokens * pitch
