@@ -487,14 +487,17 @@ Plan plan_of(const az_int8_args& a) {
     // tiles have to copy: 4 x 4095 -> 4096 22 against 24, 32 x 4095 -> 4096 23 against 36. A weight that they read in place, its rows ending
     // inside 16 bytes, meets this kernel's byte-by-byte end of a row: tiles (floating tokens, few against tiles: 3 x 162 -> 82 7.5 and 6.2, 16 x
     // 722 -> 362 14.3 and 8.1, 48 x 2047 -> 4096 14.9 and 13.0), but for up to 4 int8 tokens, which the tiles would have to copy (4 x 162 -> 82
-    // 4.6 and 5.8, 4 x 4095 -> 4096 12.4 and 12.5, though 4 x 722 -> 362 9.2 and 7.0). One or two floating tokens are quantised in
-    // the same launch, also for more channels where a row is long (1 x 14336 -> 4096 bfloat16: 17 us against 23, 1 x 4096 -> 16384 14.3 against
-    // 16.3, 1 x 1024 -> 32000 16.7 against 11.7; four tokens 14336 -> 4096 29 against 25).
+    // 4.6 and 5.8, 4 x 4095 -> 4096 12.4 and 12.5, though 4 x 722 -> 362 9.2 and 7.0).
+    // One or two floating tokens are quantised in the same launch wherever they fit its LDS, against quantising and tiles (us, weights that lie
+    // in the last-level cache): 1 x 4096 -> 4096 8.4 and 12.7, 1 x 1024 -> 16000 8.5 and 8.1, 1 x 4096 -> 16384 14.5 and 16.6, 2 x 4096 ->
+    // 24576 22.6 and 23.2, 1 x 1024 -> 131072 27.4 and 30.7, 1 x 8192 -> 65536 122 and 135, 1 x 14336 -> 4096 16 and 20.5; of 32 shapes up to
+    // 128 times as wide as long the tiles won at three by more than 5 % (1 x 722 -> 362 10.8 and 9.8, 2 x 1024 -> 16384 9.4 and 8.4, 2 x
+    // 3584 -> 18944 21 and 19.1). Four tokens 14336 -> 4096: 29 against 25.
     const bool small = a.channels < 16384;
     const bool ragged = (a.features & 15) != 0;
     const int most = copy || (ragged && a.x_dtype == AZ_DT_I8) ? 4 : ragged ? 0 : a.features <= 2048 ? FEW_TOKENS : 16;
     p.few = small && a.features <= 4096 && a.tokens <= most;
-    p.fused = (small || a.channels <= 4 * a.features) && a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
+    p.fused = a.x_dtype != AZ_DT_I8 && a.tokens <= FUSED_TOKENS && a.tokens * round_up(a.features, 64) <= FUSED_BYTES;
     if (p.fused) return p;
     if (a.x_dtype != AZ_DT_I8) {
         p.q = p.take(a.tokens * p.kpitch);
@@ -595,15 +598,17 @@ void run_tiles(const TileArgs& t, hipStream_t st) {
     hipLaunchKernelGGL((k_int8_tile<T, DT>), dim3((unsigned)(t.tiles_p * t.tiles_q * t.splits)), dim3(T::THREADS), 0, st, t);
 }
 
-// Up to FEW_TOKENS tokens. The waves of a workgroup that share 16 channels are as few as leave a workgroup per compute unit: the join is
-// then smallest.
+// Up to FEW_TOKENS tokens. The waves of a workgroup that share 16 channels are as many as leave one round of workgroups: with up to 16 tokens
+// a compute unit holds one (80 registers in 16 waves), and a second round for the last few doubles the time (1 x 4096 -> 6000 bfloat16: 8.3
+// us, with 376 workgroups of more sharing 14.3; 16 x 2048 -> 16000 int8 8.5 and 14.4). With more tokens it holds two, and one round of 256 is
+// as fast as one of 512 (48 x 2048 -> 8192 10.4 and 10.2, 48 x 512 -> 16000 7.4 and 10.4).
 template <int DT, int DX>
 int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, hipStream_t st) {
     auto run = [&](auto tokens) {
         constexpr int MT = decltype(tokens)::value, WIDE = 16 * few_fragments(DX != DT_I8, MT);
         const int64_t groups = (a.channels + WIDE - 1) / WIDE;
         int share = 16;
-        while (share > 1 && groups * share / 16 >= 512) share /= 2;
+        while (share > 1 && groups * share > 256 * 16) share /= 2;
         const FewArgs f{(const int8_t*)a.weight, x, a.weight_pitch, x_pitch, (int)a.features, share, s};
         hipLaunchKernelGGL((k_int8_few<DT, DX, MT>), dim3((unsigned)((groups * share + 15) / 16)), dim3(1024), 0, st, f);
     };

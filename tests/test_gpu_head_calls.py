@@ -59,3 +59,19 @@ def test_int8_rows_that_end_inside_16_bytes(size):
             q8[:, :k] = q
             assert torch.equal(head.int8_linear(q8[:, :k], rows, ws, x_scale=s), want)
             assert torch.equal(head.int8_linear(q8[:, :k], w, ws, x_scale=s), want)
+
+
+# around one round of workgroups, and several
+@pytest.mark.parametrize("size", [(1, 256, 4080), (2, 256, 4112), (1, 130, 6000), (1, 256, 16400), (2, 1024, 20480), (1, 64, 70001), (12, 128, 8200), (16, 256, 12000), (40, 96, 16000)],
+                         ids=ids)
+def test_int8_few_tokens_of_many_channels(size):
+    head = _head()
+    m, k, n = size
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x = torch.randn((m, k), generator=g, device="cuda")
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda").to(torch.int8)
+    ws = torch.rand(n, generator=g, device="cuda") / 127
+    q, s = head.quantize_rows(x)
+    want = ((q.double() @ w.double().t()).float() * s[:, None]) * ws
+    assert torch.equal(head.int8_linear(x, w, ws), want)
+    assert torch.equal(head.int8_linear(q, w, ws, x_scale=s), want)

@@ -103,3 +103,12 @@ def test_padded_int8_weights_are_read_in_place():
         assert size(weight=513) >= size() + channels * pitch and size(weight_pitch=pitch + 1) >= size() + channels * pitch
         eight = dict(x_dtype=N.AZ_DT_I8, x_scale=256)      # 8-bit tokens: they are copied instead, with zeros behind their last feature
         assert size(**eight) >= size(features=pitch, **eight) + tokens * pitch
+
+
+def test_one_floating_token_needs_no_scratch_memory():
+    """One or two floating tokens are quantised in the product's own launch whatever the number of channels."""
+    L = N.lib()
+    for tokens, features, channels in ((1, 162, 82), (1, 4096, 4096), (1, 1024, 32000), (2, 3584, 18944), (1, 4096, 20480), (2, 2048, 131072), (1, 32768, 64)):
+        a = N.AzInt8Args(x=256, weight=512, weight_scale=768, y=1024, tokens=tokens, features=features, channels=channels, x_pitch=features,
+                         weight_pitch=features, x_dtype=N.AZ_DT_BF16, y_dtype=N.AZ_DT_BF16)
+        assert L.az_int8_workspace(C.byref(a)) == 0, (tokens, features, channels)
