@@ -1160,12 +1160,11 @@ Layout backward_layout(const az_linear_ce_args& a) {
     }
     operand_layout(a, l);
     const int64_t np = round_up(a.rows, 64);
-    // G and its transpose of a piece stay at about 1 GB: then the sums of dx that travel between pieces cost a few per cent
+    // G and its transpose of a piece stay at about 1 GB: then the sums of dx that travel between pieces cost a few per cent. So does its part of
+    // the weight, transposed and perhaps copied (256 x 4096 -> 262144 bfloat16: one piece 3.64 ms, two 3.74, four 4.02).
     int64_t piece = (int64_t(1) << 30) / (np * 4 * l.g_planes) / 256 * 256;
-    if (l.pack_w) {
-        const int64_t w = (int64_t(1) << 29) / (l.kpitch * l.planes) / 256 * 256;
-        if (w < piece) piece = w;
-    }
+    const int64_t w = (int64_t(1) << 30) / (l.kpitch * l.planes * (l.pack_w ? 2 : 1)) / 256 * 256;
+    if (w < piece) piece = w;
     l.piece = piece < 256 ? 256 : piece;
     if (l.piece > a.classes) l.piece = a.classes;
     l.pieces = (int)((a.classes + l.piece - 1) / l.piece);

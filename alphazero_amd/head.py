@@ -153,7 +153,12 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
 
     An index outside 0..classes-1 that is not ignore_index gives a NaN loss and NaN gradients (the check is on the device, nothing
     waits for it). Everything is accumulated in float32; the gradient of the logits is rounded to the inputs' 16-bit type between the
-    products with more than 128 rows, and keeps 16 bits or more with fewer (float32 inputs: 22). Scratch memory for the backward pass stays near 1 GB whatever the number of classes."""
+    products with more than 128 rows, and keeps 16 bits or more with fewer (float32 inputs: 22).
+
+    Scratch memory of the backward pass: up to 2 GB whatever the number of classes, 6 to 8 bytes for each element of x (float32: 12), and with
+    up to 16 rows 64 bytes for each class. Of the forward pass: for float32, and for rows that are not a multiple of 16 bytes, a copy of x and up
+    to 512 MB of the weight; 16 bytes for each row and 64 to 256 classes (24 with target weights). More than a million rows or features
+    take more: the smallest piece is 256 classes."""
     _on_gpu("linear_cross_entropy", x, weight, target, bias)
     _need(reduction in _REDUCE, 'reduction is "none", "mean" or "sum"')
     _need(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1], f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")

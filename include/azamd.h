@@ -362,7 +362,10 @@ typedef struct {
     float entropy_coeff;
 } az_linear_ce_args;
 
-/* Bytes of scratch memory of a forward (backward = 0) or backward call, or a negative az_status. */
+/* Bytes of scratch memory of a forward (backward = 0) or backward call, or a negative az_status. Backward: up to 2 GB whatever the number
+ * of classes, 6 to 8 bytes for each element of x (float32: 12), with up to 16 rows 64 for each class. Forward: 16 bytes for each row and 64
+ * to 256 classes (24 with target_dense); for float32 and for rows that are not a multiple of 16 bytes a copy of x and up to 512 MB of the
+ * weight. The smallest piece is 256 classes, which alone take more beyond a million rows or features. */
 int64_t az_linear_ce_workspace(const az_linear_ce_args* args, int32_t backward);
 
 /* kept: float [4 * rows + 4], for the backward call. loss, ce, ent: the loss, its cross entropy and the softmax' entropy, one

@@ -112,3 +112,19 @@ def test_one_floating_token_needs_no_scratch_memory():
         a = N.AzInt8Args(x=256, weight=512, weight_scale=768, y=1024, tokens=tokens, features=features, channels=channels, x_pitch=features,
                          weight_pitch=features, x_dtype=N.AZ_DT_BF16, y_dtype=N.AZ_DT_BF16)
         assert L.az_int8_workspace(C.byref(a)) == 0, (tokens, features, channels)
+
+
+def test_scratch_memory_of_the_loss_is_bounded():
+    """What linear_cross_entropy says of its scratch memory, over many classes, many rows and long features."""
+    L = N.lib()
+    for dtype, size in ((N.AZ_DT_F32, 4), (N.AZ_DT_BF16, 2), (N.AZ_DT_F16, 2)):
+        for rows, features, classes in ((256, 4096, 1 << 20), (64, 4096, 1 << 20), (64, 8192, 270001), (262144, 4096, 32000), (1 << 20, 4096, 50021), (8192, 4096, 131072),
+                                        (17, 16384, 1 << 20), (129, 100000, 100000), (1, 4096, 1 << 24), (40, 8, 1 << 28), (200000, 8, 4000), (1 << 20, 64, 1000), (500, 1 << 20, 900)):
+            for pitch in (features, features + 1):        # a weight that is read in place, and one that is copied
+                a = N.AzLinearCeArgs(x=256, weight=512, target=768, rows=rows, features=features, classes=classes, x_pitch=pitch, weight_pitch=pitch,
+                                     ignore_index=-100, dtype=dtype, reduction=N.AZ_REDUCE_MEAN)
+                back, ahead = (L.az_linear_ce_workspace(C.byref(a), b) for b in (1, 0))
+                x = rows * features * size
+                weight = max(2 ** 29, 256 * features * size)        # of a piece of the classes, which has 256 at least
+                assert 0 < back <= 1.25 * 2 ** 30 + 2 * weight + 4 * x + 70 * classes, (dtype, rows, features, classes, pitch, back / 2 ** 30)
+                assert 0 < ahead <= 2 ** 25 + weight + 1.01 * x + 16 * (rows * classes / 32 + rows + classes), (dtype, rows, features, classes, pitch, ahead / 2 ** 30)
