@@ -212,6 +212,11 @@ __device__ __forceinline__ float reference_minus(float a, float b) {
     return fabsf(a) < 131072.0f && fabsf(b) < 131072.0f ? 2.0f * (a - b) : (reference_size(a) - reference_size(b)) * LOG2E;
 }
 
+// The backward pass makes the logits again, by other kernels than the forward pass where these are faster, and so with other roundings: in
+// logits of millions they leave more than the distance to the sum. No p is above one all the same: t goes up to this, from 1 / sum 2^t.
+// (A logit that is no number is lost here, but in 1 / sum it is not.)
+__device__ __forceinline__ float most_of(float inv) { return -__builtin_amdgcn_logf(inv); }
+
 // Sums of a part of a row: its reference (-inf: no class that can be), sum 2^t, sum 2^t t, sum pi t, sum pi.
 struct Part {
     float ref, l, s, dot, pi;
@@ -727,6 +732,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_ce_grad(GradArgs a) {
             if (!DENSE && (target < 0 || target >= a.t.classes)) f = NAN;
         }
         const Reference at(ref);
+        const float most = most_of(inv);
         f32x4 pi[T::FP];
         if constexpr (DENSE) target_weights<T>(a.t, n, a.v0 + ml, left, p0 + T::BP <= a.t.classes - a.v0, pi);
         const float scale = (DENSE ? total * inv : inv) * f, c = a.t.entropy * LN2 * inv * f;
@@ -734,7 +740,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void k_ce_grad(GradArgs a) {
         for (int i = 0; i < T::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float t = at.t(acc[i][j][r]);
+                const float t = fminf(at.t(acc[i][j][r]), most);
                 const float e = __builtin_amdgcn_exp2f(t);
                 float g = e * scale;
                 if constexpr (DENSE) g -= pi[i][r] * f;

@@ -205,10 +205,10 @@ __global__ __launch_bounds__(1024) void k_ce_few(FewArgs a) {
                         else if (target < 0 || target >= a.t.classes) f = NAN;
                     }
                     const Reference at(row ? a.ref[n] : 0.0f);
-                    const float inv = row ? a.inv[n] : 0.0f, mean = row ? a.mean[n] : 0.0f;
+                    const float inv = row ? a.inv[n] : 0.0f, mean = row ? a.mean[n] : 0.0f, most = most_of(inv);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float q = at.t(z[r]), e = __builtin_amdgcn_exp2f(q);
+                        const float q = fminf(at.t(z[r]), most), e = __builtin_amdgcn_exp2f(q);
                         float g = e * (inv * total) - pi[r];
                         if (target == m + r) g -= 1.0f;
                         if (entropy && e != 0.0f) g += a.t.entropy * LN2 * inv * e * (q - mean);

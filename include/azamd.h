@@ -347,7 +347,9 @@ typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2 } az_re
  * ignore_index cost nothing, get zero gradients and stay out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
  * -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax and gives NaN. The gradient of the logits is
  * held in 16 bits between the products (two planes for float32 and for up to 128 rows), relative to the largest sum of target weights of a row: with float16,
- * rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give NaN with float32. */
+ * rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give NaN with float32. The backward pass makes
+ * the logits again, where that is faster by another kernel than the forward pass: their rounding (2^-22 of a logit and more) is in its
+ * softmax, so rows with logits beyond some 10^5 get gradients of a few bits; never a p above one. */
 typedef struct {
     const void* x;            /* [rows, features] of dtype */
     const void* weight;       /* [classes, features] of dtype */

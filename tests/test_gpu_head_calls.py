@@ -75,3 +75,29 @@ def test_int8_few_tokens_of_many_channels(size):
     want = ((q.double() @ w.double().t()).float() * s[:, None]) * ws
     assert torch.equal(head.int8_linear(x, w, ws), want)
     assert torch.equal(head.int8_linear(q, w, ws, x_scale=s), want)
+
+
+def _loss_inputs(rows, feats, classes, dtype, dense, bias, seed=0):
+    from test_gpu_head import _inputs
+    return _inputs(rows, feats, classes, dtype, dense, bias, seed)
+
+
+def _loss_run(x, w, b, t, grad=None, **kw):
+    from test_gpu_head import _run
+    return _run(x, w, b, t, grad, **kw)
+
+
+@pytest.mark.parametrize("size", [(20, 64, 300), (10, 64, 300), (9, 1032, 33000), (30, 300, 2000), (200, 64, 300), (100, 5000, 60)], ids=ids)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+@pytest.mark.parametrize("factor", [1e6, 1e9, 1e12, 1e16])
+def test_a_row_of_huge_logits_has_a_finite_gradient(size, dtype, factor):
+    """The passes may make the logits by different kernels; what their roundings differ by must not become a p of infinity."""
+    x, w, b, t = _loss_inputs(*size, dtype, False, True)
+    x[3] *= factor
+    t[3] = 5
+    loss, ce, ent, gx, gw, gb = _loss_run(x, w, b, t, reduction="sum", entropy_coeff=0.01)
+    for v in (loss, ce, ent, gx, gw, gb):
+        assert torch.isfinite(v).all()
+    # |G| of a row sums to twice its weights' sum and the entropy's part at most, with every p at most one; roundings beside it
+    most = (2 + 0.01 * (0.4 + math.log(size[2]))) * 1.02
+    assert float(gx[3].abs().max()) <= most * float(w.abs().max())
