@@ -19,7 +19,8 @@
 //
 // float32 operands come as two float16 planes, v = h + m / 2048 (split2), scaled by powers of two beforehand. k is walked three times,
 // first with the plane pairs (h, m) and (m, h), whose sum is then divided by 2048, then with (h, h); (m, m) / 2^22 is below
-// 2^-24 of the result and left out. Each product keeps 22 bits or more, the sum is float32's: 2.5 PFLOP/s / 3 against the 0.16
+// 2^-24 of the result and left out. Each product keeps 22 bits or more, of values down to 2^-27 of the largest with the same scale; the sum is
+// float32's: 2.5 PFLOP/s / 3 against the 0.16
 // PFLOP/s of the float32 matrix instructions.
 #pragma once
 #include <hip/hip_runtime.h>

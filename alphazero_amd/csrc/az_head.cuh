@@ -41,8 +41,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float larger(float top, float v) { return v > top || v != v ? v : top; }      // a NaN stays
 
 // Copies a [rows, cols] matrix (any row stride, any alignment) into rows of `pitch` bytes, zeros behind the last column. float32 is
-// scaled by a power of two and split into two planes: in the forward pass each row by its own (its reciprocal goes to `own`), in the
-// backward pass all rows by the one of the largest (`all`), since there a sum also runs over the rows. Rows that do not count become
+// scaled by a power of two, each row by its own (its reciprocal goes to `own`), and split into two planes. Rows that do not count become
 // zeros. Bound by memory; only operands that the tile loop cannot read in place come here (float32, rows that do not start at
 // multiples of 16 bytes).
 struct PackJob {
@@ -51,8 +50,7 @@ struct PackJob {
     int32_t rows, cols;
     char* dst;
     int64_t pitch, plane;   // bytes
-    float* own;
-    const float* all;
+    float* own;             // float32
     const int64_t* target;  // null: every row counts
     int64_t ignore;
     // Lanes of a row that is scaled by itself: as many as it has pieces, up to a wave, or a workgroup from 4096 columns on (forward pass of
@@ -95,7 +93,7 @@ __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block, floa
 #pragma unroll
         for (int p = 0; p < NP; ++p) *(uint4*)(j.dst + p * j.plane + r * j.pitch + piece * 16) = *(const uint4*)h[p];
     };
-    if (DT == DT_F32 && j.own) {
+    if constexpr (DT == DT_F32) {
         const int lanes = j.lanes(), lane = threadIdx.x & (lanes - 1);
         const int64_t r = block * (256 / lanes) + threadIdx.x / lanes;
         if (r >= j.rows) return;
@@ -129,12 +127,13 @@ __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block, floa
         for (int i = lane + lanes; i < pieces; i += lanes) put(r, i, scale);
     } else {
         const int64_t at = block * 256 + threadIdx.x;
-        if (at < (int64_t)j.rows * pieces) put(at / pieces, (int)(at % pieces), DT == DT_F32 ? 1.0f / *j.all : 1.0f);
+        if (at < (int64_t)j.rows * pieces) put(at / pieces, (int)(at % pieces), 1.0f);
     }
 }
 
-// The same, transposed: dst row c = column c of the source, rows behind the last one (up to the pitch, a multiple of 128 bytes) zero;
-// rows that do not count become zeros, so that whatever a padded row holds - NaN included - stays out of dW. 64 x 64 elements per
+// The same, transposed: dst row c = column c of the source, rows behind the last one (up to the pitch, a multiple of 128 bytes) zero. The
+// products' sums run over the source's rows here, so all of float32 is divided by what the largest row is (`all`): every value keeps 22
+// bits down to 2^-27 of the largest, and what is left above 2^-49 of it below that. Rows that do not count become zeros, so that whatever a padded row holds - NaN included - stays out of dW. 64 x 64 elements per
 // workgroup through LDS.
 struct TurnJob {
     const void* src;
@@ -256,8 +255,7 @@ struct StatArgs {
     Rows t;
     const void* bias;
     int32_t kbytes;
-    const float *un_w, *un_x;   // float32: what the operands were divided by, per class of the piece and per row (un_step 1) or for all (0)
-    int32_t un_step;
+    const float *un_w, *un_x;   // float32: what the operands were divided by, per class of the piece and per row
     int32_t v0;             // first class of the piece that w starts at
     int32_t tile0, tiles;   // first tile of the piece, tiles of all classes
     f32x4* part;            // [rows][tiles] ref, l, s, dot
@@ -315,13 +313,12 @@ __device__ __forceinline__ void logits(const A& a, int64_t p0, int64_t q0, char*
 #pragma unroll
         for (int j = 0; j < T::FQ; ++j) {
             const int64_t n = q0 + wq * T::TQ + j * 16 + (lane & 15);
-            un[j] = a.un_x[(n < a.x.rows ? n : a.x.rows - 1) * a.un_step];
+            un[j] = a.un_x[n < a.x.rows ? n : a.x.rows - 1];
         }
-        const AxisView un_w(a.un_w + p0 * a.un_step, a.un_step ? here : 0);
+        const AxisView un_w(a.un_w + p0, here);
 #pragma unroll
         for (int i = 0; i < T::FP; ++i) {
-            f32x4 u = un_w.four(ml + i * 16);
-            if (!a.un_step) u = f32x4{1.0f, 1.0f, 1.0f, 1.0f} * *a.un_w;
+            const f32x4 u = un_w.four(ml + i * 16);
 #pragma unroll
             for (int j = 0; j < T::FQ; ++j)
 #pragma unroll
@@ -556,7 +553,7 @@ __device__ __forceinline__ void reduce_rows(const JoinArgs& a) {
         h += a.ent[n];
         if (a.t.dense && a.tabs[n] < INFINITY) top = fmaxf(top, a.tabs[n]);     // a row of infinite weights spoils itself only
     }
-    float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides all rows by it
+    float ux = 0.0f, uw = 0.0f;        // the largest: the backward pass divides its transposed copies by it
     if (a.un_x) {
         for (int n = threadIdx.x; n < a.count_x; n += 1024) ux = fmaxf(ux, a.un_x[n]);
 #pragma unroll 4
@@ -685,7 +682,7 @@ struct GradArgs {
     const void* bias;
     int32_t kbytes;
     const float *un_w, *un_x;
-    int32_t un_step, v0;
+    int32_t v0;
     int32_t tiles_p, tiles_q;
     Walk walk;
     const float *ref, *inv, *mean, *tsum;
@@ -1177,6 +1174,10 @@ Layout backward_layout(const az_linear_ce_args& a) {
     const int64_t vp = round_up(l.piece, 64);
     if (l.pack_x) l.xp = l.take(a.rows * l.kpitch * l.planes);
     if (l.pack_w) l.wp = l.take(l.piece * l.kpitch * l.planes);
+    if (l.split) {
+        l.ux = l.take(a.rows * 4);
+        l.uw = l.take(l.piece * 4);
+    }
     l.xt = l.take(a.features * np * 2 * l.planes);
     l.wt = l.take(a.features * vp * 2 * l.planes);
     l.g = l.take(a.rows * vp * 2 * l.g_planes);
@@ -1281,17 +1282,16 @@ FewArgs few_args(const az_linear_ce_args& a) {
 
 // The operands of a piece's logits, in place or as copies that `p` is to make (x with the first piece).
 template <int DT, class S>
-void operands(const az_linear_ce_args& a, const Layout& l, int piece, int64_t nv, const char* w, char* ws, float* own_w, float* own_x,
-              const float* all_w, const float* all_x, PackArgs& p, S& s) {
+void operands(const az_linear_ce_args& a, const Layout& l, int piece, int64_t nv, const char* w, char* ws, PackArgs& p, S& s) {
     s.w = MmOperand{w, a.weight_pitch * 2, 0, (int)nv};
     s.x = MmOperand{(const char*)a.x, a.x_pitch * 2, 0, (int)a.rows};
     if (l.pack_w) {
-        p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch, own_w, all_w, nullptr, 0};
+        p.w = PackJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wp, l.kpitch, l.piece * l.kpitch, (float*)s.un_w, nullptr, 0};
         s.w = MmOperand{ws + l.wp, l.kpitch, l.piece * l.kpitch, (int)nv};
     }
     if (l.pack_x) {
         if (piece == 0)
-            p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch, own_x, all_x, s.t.index, a.ignore_index};
+            p.x = PackJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xp, l.kpitch, a.rows * l.kpitch, (float*)s.un_x, s.t.index, a.ignore_index};
         s.x = MmOperand{ws + l.xp, l.kpitch, a.rows * l.kpitch, (int)a.rows};
     }
 }
@@ -1346,7 +1346,6 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
     }
     s.bias = a.bias;
     s.un_x = l.split ? (float*)(ws + l.ux) : nullptr;
-    s.un_step = 1;
     s.part = (f32x4*)(ws + l.part);
     s.tpart = a.target_dense ? (float*)(ws + l.tpart) : nullptr;
     s.zt = a.target_dense ? nullptr : (float*)(ws + l.zt);
@@ -1358,7 +1357,7 @@ int forward(const az_linear_ce_args& a, float* kept, float* loss, float* ce, flo
         const char* w = (const char*)a.weight + v0 * a.weight_pitch * (l.split ? 4 : 2);
         PackArgs p{};
         s.un_w = l.split ? (float*)(ws + l.uw) + v0 : nullptr;
-        operands<DT>(a, l, i, nv, w, ws, (float*)s.un_w, (float*)s.un_x, nullptr, nullptr, p, s);
+        operands<DT>(a, l, i, nv, w, ws, p, s);
         pack<DT>(p, st);
         s.v0 = (int)v0;
         s.tile0 = (int)(v0 / edge);
@@ -1410,9 +1409,8 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     GradArgs s{};
     s.t = rows_of(a);
     s.bias = a.bias;
-    s.un_x = un_x;
-    s.un_w = un_w;
-    s.un_step = 0;
+    s.un_x = l.split ? (float*)(ws + l.ux) : nullptr;      // the logits are those of the forward pass again, to the bit of their scales
+    s.un_w = l.split ? (float*)(ws + l.uw) : nullptr;
     s.kbytes = (int)l.kpitch;     // of an operand read in place too: its rows are whole 16 bytes
     s.ref = kept.ref;
     s.inv = kept.inv;
@@ -1432,7 +1430,7 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         const char* w = (const char*)a.weight + v0 * a.weight_pitch * esize;
         const int64_t vpi = round_up(nv, 64);    // k of dx in this piece
         PackArgs p{};
-        operands<DT>(a, l, i, nv, w, ws, nullptr, nullptr, un_w, un_x, p, s);
+        operands<DT>(a, l, i, nv, w, ws, p, s);
         if (gx) p.wt = TurnJob{w, a.weight_pitch, (int)nv, (int)a.features, ws + l.wt, vpi * 2, a.features * vpi * 2, un_w, nullptr, 0};
         if (gw && i == 0) p.xt = TurnJob{a.x, a.x_pitch, (int)a.rows, (int)a.features, ws + l.xt, np * 2, a.features * np * 2, un_x, s.t.index, a.ignore_index};
         pack<DT>(p, st);

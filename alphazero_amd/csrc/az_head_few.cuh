@@ -21,7 +21,7 @@ struct FewArgs {
     Rows t;
     f32x4* part;                  // [rows][workgroups]
     float *tpart, *zt;
-    float *un_w, *un_x;           // float32, [workgroups]: unscale_of the largest values, which the backward pass of more rows divides by
+    float *un_w, *un_x;           // float32, [workgroups]: unscale_of the largest values, which a backward pass with tiles divides transposed copies by
     const float *ref, *inv, *mean, *tsum, *grad, *scalars;   // gradient
     int32_t each, mean_of;
     float* g;                     // [classes][16 * MT]

@@ -155,6 +155,9 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     waits for it). Everything is accumulated in float32; the gradient of the logits is rounded to the inputs' 16-bit type between the
     products with more than 128 rows, and keeps 16 bits or more with fewer (float32 inputs: 22).
 
+    float32 gradients: with more than 16 rows the sums over the classes (for x) and over the rows (for the weight) hold weight and x to
+    22 bits each, and to 2^-49 of that matrix' largest value: values below 2^-27 of the largest lose bits.
+
     Scratch memory of the backward pass: up to 2 GB whatever the number of classes, 6 to 8 bytes for each element of x (float32: 12), and with
     up to 16 rows 64 bytes for each class. Of the forward pass: for float32, and for rows that are not a multiple of 16 bytes, a copy of x and up
     to 512 MB of the weight; 16 bytes for each row and 64 to 256 classes (24 with target weights). More than a million rows or features

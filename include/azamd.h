@@ -349,7 +349,9 @@ typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2 } az_re
  * held in 16 bits between the products (two planes for float32 and for up to 128 rows), relative to the largest sum of target weights of a row: with float16,
  * rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give NaN with float32. The backward pass makes
  * the logits again, where that is faster by another kernel than the forward pass: their rounding (2^-22 of a logit and more) is in its
- * softmax, so rows with logits beyond some 10^5 get gradients of a few bits; never a p above one. */
+ * softmax, so rows with logits beyond some 10^5 get gradients of a few bits; never a p above one. float32 gradients hold weight (in
+ * grad_x's sums over the classes) and x (in grad_weight's over the rows) to 22 bits and to 2^-49 of that matrix' largest value, so values
+ * below 2^-27 of the largest lose bits there; the loss and the softmax scale every row by itself. */
 typedef struct {
     const void* x;            /* [rows, features] of dtype */
     const void* weight;       /* [classes, features] of dtype */

@@ -101,3 +101,33 @@ def test_a_row_of_huge_logits_has_a_finite_gradient(size, dtype, factor):
     # |G| of a row sums to twice its weights' sum and the entropy's part at most, with every p at most one; roundings beside it
     most = (2 + 0.01 * (0.4 + math.log(size[2]))) * 1.02
     assert float(gx[3].abs().max()) <= most * float(w.abs().max())
+
+
+@pytest.mark.parametrize("rows", [10, 20, 50, 200, 300])
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("factor", [1e6, 1e12, 1e16])
+def test_float32_rows_of_very_different_size(rows, dense, reduction, factor):
+    """One counted row of x, then one class of the weight, far larger than the others: every row has its own softmax and gradient. The sums of
+    the gradients hold their operand to 2^-49 of its largest value (2^-35 in planes whose largest is 2^13 or more, rounded)."""
+    for large in ("row", "class"):
+        x, w, b, t = _loss_inputs(rows, 64, 300, F32, dense, True)
+        if large == "row":
+            x[3] *= factor
+            if not dense:
+                t[3] = 5
+        else:
+            w[7] *= factor
+        grad = torch.ones((rows,) if reduction == "none" else (), device="cuda")
+        got = _loss_run(x, w, b, t, grad, reduction=reduction)
+        ref = R.loss_reference(x, w, t, b, reduction=reduction, grad=grad)
+        ref = {k: (v.clone(), tol.clone()) for k, (v, tol) in ref.items()}
+        counts = torch.ones(rows, dtype=torch.bool, device="cuda") if dense else t != -100
+        each = 1.0 if reduction == "none" else 1.0 / float(counts.sum())
+        total = t.double().sum(1) if dense else counts.double()
+        # each row of G sums to twice its weights' sum at most, each column to that over the rows
+        ref["gx"][1].add_((2.0 ** -49 * float(w.abs().max()) * 2 * each * total)[:, None])
+        ref["gw"][1].add_(2.0 ** -49 * float(x[counts].abs().max()) * 2 * each * float(total.sum()))
+        for name, v in zip(("loss", "ce", "ent", "gx", "gw", "gb"), got):
+            R.close(name, v[counts] if name in ("loss", "ce", "ent") and v.dim() else v, ref[name] if name in ("gx", "gw", "gb") or not v.dim() else
+                    (ref[name][0][counts], ref[name][1][counts]))
