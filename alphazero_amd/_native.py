@@ -13,7 +13,7 @@ AZ_OK, AZ_ERR_ARG, AZ_ERR_HIP, AZ_ERR_STATE, AZ_ERR_ILLEGAL, AZ_ERR_NOCHILD, AZ_
 AZ_FEAT_F32_NCHW, AZ_FEAT_BF16_NHWC = 0, 1
 AZ_NET_BF16, AZ_NET_F32 = 0, 1
 AZ_DT_F32, AZ_DT_BF16, AZ_DT_F16, AZ_DT_I8 = 0, 1, 2, 3
-AZ_REDUCE_NONE, AZ_REDUCE_MEAN, AZ_REDUCE_SUM = 0, 1, 2
+AZ_REDUCE_NONE, AZ_REDUCE_MEAN, AZ_REDUCE_SUM, AZ_PRECISE_GRADIENT = 0, 1, 2, 4
 
 
 class AzConfig(C.Structure):

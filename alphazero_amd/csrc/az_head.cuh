@@ -979,10 +979,14 @@ bool in_place(const void* p, int64_t pitch, int64_t cols) { return ((uintptr_t)p
 void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.split = a.dtype == AZ_DT_F32;
     l.planes = l.split ? 2 : 1;
-    // With few rows a handful of values (the targets) are most of G, and the rounding of each to 16 bits shows in the gradients: 1.6 times
-    // the error of their own type's rounding with up to 40 rows, 1.45 with 100, 1.4 and steady beyond. There G takes two planes: 1.0,
-    // for 8 to 20 % of the two passes' time (64 x 4096 -> 4096 bfloat16: 77 us, now 91; 64 x 722 -> 362 34, now 39).
-    const bool two = !l.split && a.rows <= 128;
+    // Where a handful of values is most of G, the rounding of each to 16 bits shows in the gradients. Their error against what the rounding of
+    // the gradients themselves makes: 1.6 with up to 40 rows, 1.45 with 100; 1.4 with 362 classes and target weights whatever the
+    // rows, 1.2 with 512 and class indices, 1.18 with 2048 to 4096, 1.06 to 1.13 with 32000. With two planes of G it is 1.0 everywhere.
+    // They cost, in both passes together, 8 to 20 % with up to 128 rows (64 x 4096 -> 4096 bfloat16 77 and 91 us, 64 x 722 -> 362 34 and
+    // 39), 7 to 17 % with up to 512 classes (256 x 162 -> 82 float16 36.8 and 39.4, 4096 x 722 -> 362 80 and 89, 16384 x 722 -> 362 176
+    // and 201, 16384 x 256 -> 512 115 and 131), and from 13 % to twice the time beyond (4096 x 256 -> 2048 87 and 103, 1024 x 1024 -> 4096 99
+    // and 127, 1024 x 2048 -> 32000 687 and 1403), where it is the caller's choice.
+    const bool two = !l.split && (a.rows <= 128 || a.classes <= 512 || (a.reduction & AZ_PRECISE_GRADIENT));
     l.g_planes = l.split || two ? 2 : 1;
     if (two) l.edge_most = 128;
     l.pack_w = l.split || !in_place(a.weight, a.weight_pitch, a.features);
@@ -1209,7 +1213,7 @@ int check_args(const az_linear_ce_args* a) {
     if (!a->x || !a->weight || !a->target) return fail(AZ_ERR_ARG, "null argument");
     if (a->x_pitch < a->features || a->weight_pitch < a->features || (a->target_dense && a->target_pitch < a->classes))
         return fail(AZ_ERR_ARG, "a row stride is smaller than the row");
-    if (a->reduction < AZ_REDUCE_NONE || a->reduction > AZ_REDUCE_SUM) return fail(AZ_ERR_ARG, "reduction is none, mean or sum");
+    if ((a->reduction & ~AZ_PRECISE_GRADIENT) < AZ_REDUCE_NONE || (a->reduction & ~AZ_PRECISE_GRADIENT) > AZ_REDUCE_SUM) return fail(AZ_ERR_ARG, "reduction is none, mean or sum");
     return AZ_OK;
 }
 
@@ -1217,6 +1221,8 @@ int launched(const char* what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AZ_OK : fail(AZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
+
+int reduction_of(const az_linear_ce_args& a) { return a.reduction & ~AZ_PRECISE_GRADIENT; }
 
 Rows rows_of(const az_linear_ce_args& a) {
     Rows t;
@@ -1304,7 +1310,7 @@ struct Kept {      // what the forward pass leaves for the backward one
 template <int DT>
 int join(const az_linear_ce_args& a, const Layout& l, const StatArgs& s, float* kept, float* loss, float* ce, float* ent, char* ws, hipStream_t st) {
     const Kept k(kept, a.rows);
-    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, a.reduction, k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
+    const JoinArgs j{s.t, s.part, s.tpart, s.zt, s.tiles, reduction_of(a), k.ref, k.inv, k.mean, k.tsum, k.scalars, (float*)(ws + l.ce), (float*)(ws + l.ce) + a.rows,
                      a.target_dense ? (float*)(ws + l.tabs) : nullptr, loss, ce, ent,
                      l.ux >= 0 ? (float*)(ws + l.ux) : nullptr, l.uw >= 0 ? (float*)(ws + l.uw) : nullptr,
                      l.few ? l.grid : (int)a.rows, l.few ? l.grid : (int)a.classes};
@@ -1383,8 +1389,8 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         f.tsum = kept.tsum;
         f.grad = grad;
         f.scalars = kept.scalars;
-        f.each = a.reduction == AZ_REDUCE_NONE;
-        f.mean_of = a.reduction == AZ_REDUCE_MEAN;
+        f.each = reduction_of(a) == AZ_REDUCE_NONE;
+        f.mean_of = reduction_of(a) == AZ_REDUCE_MEAN;
         f.g = (float*)(ws + l.fg);
         hipLaunchKernelGGL((k_ce_few<DT, 1, true>), dim3((unsigned)l.grid), dim3(1024), 0, st, f);
         if (const int rc = launched("k_ce_few")) return rc;
@@ -1400,10 +1406,10 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
         return launched("k_ce_few_out");
     }
     const int esize = l.split ? 4 : 2;
-    const int64_t np = round_up(a.rows, 64), vp = round_up(l.piece, 64);
-    const bool each = a.reduction == AZ_REDUCE_NONE;
+    const int64_t np = round_up(a.rows, 64);
+    const bool each = reduction_of(a) == AZ_REDUCE_NONE;
     const float *un_x = l.split ? kept.scalars + 2 : nullptr, *un_w = l.split ? kept.scalars + 3 : nullptr;
-    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, a.reduction == AZ_REDUCE_MEAN, DT != DT_BF16, nullptr, a.target_dense ? nullptr : (const int64_t*)a.target,
+    const Factor f{grad, kept.scalars, each ? (const float*)(ws + l.largest) : nullptr, reduction_of(a) == AZ_REDUCE_MEAN, DT != DT_BF16, nullptr, a.target_dense ? nullptr : (const int64_t*)a.target,
                    a.ignore_index};
     if (each) hipLaunchKernelGGL(k_ce_largest, dim3(1), dim3(1024), 0, st, grad, rows_of(a), (float*)(ws + l.largest));
     GradArgs s{};
@@ -1419,8 +1425,6 @@ int backward(const az_linear_ce_args& a, const Kept& kept, const float* grad, vo
     s.f = f;
     s.two = !l.split && l.g_planes == 2;
     s.g = gx ? ws + l.g : nullptr;
-    s.g_pitch = vp * 2;
-    s.g_plane = a.rows * vp * 2;
     s.gt = gw ? ws + l.gt : nullptr;
     s.gt_pitch = np * 2;
     s.gt_plane = l.piece * np * 2;

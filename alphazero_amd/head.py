@@ -86,16 +86,16 @@ def _scratch(size: int, device) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------------------------------------ loss of a linear layer
-def _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff):
+def _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff, precise):
     dense = target.dim() == 2
     return N.AzLinearCeArgs(x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr(), x.shape[0], x.shape[1], weight.shape[0], _pitch(x),
-                            _pitch(weight), _pitch(target) if dense else 0, ignore_index, _DTYPES[x.dtype], dense, _REDUCE[reduction], entropy_coeff)
+                            _pitch(weight), _pitch(target) if dense else 0, ignore_index, _DTYPES[x.dtype], dense, _REDUCE[reduction] | (N.AZ_PRECISE_GRADIENT if precise else 0), entropy_coeff)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, reduction, entropy_coeff, parts):
-        a = _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff)
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction, entropy_coeff, precise, parts):
+        a = _ce_args(x, weight, bias, target, ignore_index, reduction, entropy_coeff, precise)
         rows, dev = x.shape[0], x.device
         shape = (rows,) if reduction == "none" else ()
         out = tuple(torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3 if parts else 1))
@@ -110,7 +110,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             for o in out:
                 o.fill_(float("nan") if reduction == "mean" else 0.0)
         ctx.save_for_backward(x, weight, bias, target, kept)
-        ctx.args = (ignore_index, reduction, entropy_coeff)
+        ctx.args = (ignore_index, reduction, entropy_coeff, precise)
         if parts:
             ctx.mark_non_differentiable(out[1], out[2])
         ctx.set_materialize_grads(False)
@@ -120,7 +120,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, *_parts):
         if grad is None:
-            return (None,) * 8
+            return (None,) * 9
         x, weight, bias, target, kept = ctx.saved_tensors
         a = _ce_args(x, weight, bias, target, *ctx.args)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -133,16 +133,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
             for g in (gw, gb):
                 if g is not None:
                     g.zero_()
-            return gx, gw, gb, None, None, None, None, None
+            return gx, gw, gb, None, None, None, None, None, None
         r = C.byref(a)
         size = N.check(N.lib().az_linear_ce_workspace(r, 1), "az_linear_ce_workspace")
         ws = _scratch(size, dev)
         _native(dev, "az_linear_ce_backward", r, kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), size, _stream(dev))
-        return gx, gw, gb, None, None, None, None, None
+        return gx, gw, gb, None, None, None, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100, reduction: str = "mean", entropy_coeff: float = 0.0,
-                         parts: bool = False):
+                         parts: bool = False, precise_gradient: bool = False):
     """Cross entropy of softmax(x weight^T + bias) minus entropy_coeff times that softmax' entropy, without ever holding the logits.
 
     x [..., features], weight [classes, features], bias [classes] or None: one dtype (float32, bfloat16, float16; under autocast they
@@ -152,8 +152,10 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     "none". Returns the float32 loss; with parts=True (loss, cross entropy, entropy), the last two without gradient.
 
     An index outside 0..classes-1 that is not ignore_index gives a NaN loss and NaN gradients (the check is on the device, nothing
-    waits for it). Everything is accumulated in float32; the gradient of the logits is rounded to the inputs' 16-bit type between the
-    products with more than 128 rows, and keeps 16 bits or more with fewer (float32 inputs: 22).
+    waits for it). Everything is accumulated in float32; between the products of the backward pass the gradient of the logits keeps
+    22 bits for float32 inputs. For 16-bit ones it keeps 16 bits or more with up to 128 rows or 512 classes and is rounded to the
+    inputs' type beyond, which adds 6 to 20 % to the error that rounding the results makes; precise_gradient=True keeps 16 bits or more
+    there too, in up to twice the time.
 
     float32 gradients: with more than 16 rows the sums over the classes (for x) and over the rows (for the weight) hold weight and x to
     22 bits each, and to 2^-49 of that matrix' largest value: values below 2^-27 of the largest lose bits.
@@ -183,7 +185,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
         target = target.reshape(-1).contiguous()
     x2 = _rows(x)
     out = _LinearCrossEntropy.apply(x2, _rows(weight), bias if bias is None else bias.contiguous(), target, int(ignore_index), reduction,
-                                    float(entropy_coeff), bool(parts))
+                                    float(entropy_coeff), bool(precise_gradient), bool(parts))
     if reduction == "none" and len(lead) != 1:
         out = tuple(t.reshape(lead) for t in out)
     return out if parts else out[0]

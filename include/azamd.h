@@ -340,13 +340,14 @@ int az_pack_planes(const float* planes, int32_t count, int32_t board_size, int32
  * further apart than they are long (pitches in elements); every call enqueues on `stream` and allocates nothing: scratch memory is
  * the caller's `workspace` (256-byte aligned, contents undefined before and after, not shared by calls that may overlap). */
 typedef enum { AZ_DT_F32 = 0, AZ_DT_BF16 = 1, AZ_DT_F16 = 2, AZ_DT_I8 = 3 } az_dtype;
-typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2 } az_reduce;
+typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2, AZ_PRECISE_GRADIENT = 4 } az_reduce;
 
 /* Cross entropy of softmax(x weight^T + bias) against class indices or against rows of target weights, minus entropy_coeff times
  * the softmax' entropy; the logits are never stored (up to 8 MB of partial sums of few of them are). Rows whose index is
  * ignore_index cost nothing, get zero gradients and stay out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
  * -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax and gives NaN. The gradient of the logits is
- * held in 16 bits between the products (two planes for float32 and for up to 128 rows), relative to the largest sum of target weights of a row: with float16,
+ * held in 16 bits between the products (in two planes, 16 bits or more, for float32, for up to 128 rows or 512 classes, and for any size
+ * with AZ_PRECISE_GRADIENT or-ed into the reduction, which can double the backward pass' time), relative to the largest sum of target weights of a row: with float16,
  * rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give NaN with float32. The backward pass makes
  * the logits again, where that is faster by another kernel than the forward pass: their rounding (2^-22 of a logit and more) is in its
  * softmax, so rows with logits beyond some 10^5 get gradients of a few bits; never a p above one. float32 gradients hold weight (in
@@ -362,7 +363,7 @@ typedef struct {
     int64_t ignore_index;
     int32_t dtype;            /* AZ_DT_F32 / BF16 / F16 */
     int32_t target_dense;
-    int32_t reduction;        /* az_reduce; NONE: one gradient per row is handed to the backward call */
+    int32_t reduction;        /* az_reduce, perhaps with AZ_PRECISE_GRADIENT; NONE: one gradient per row is handed to the backward call */
     float entropy_coeff;
 } az_linear_ce_args;
 

@@ -131,3 +131,53 @@ def test_float32_rows_of_very_different_size(rows, dense, reduction, factor):
         for name, v in zip(("loss", "ce", "ent", "gx", "gw", "gb"), got):
             R.close(name, v[counts] if name in ("loss", "ce", "ent") and v.dim() else v, ref[name] if name in ("gx", "gw", "gb") or not v.dim() else
                     (ref[name][0][counts], ref[name][1][counts]))
+
+
+def _loss_gradients(x, w, b, t, f):
+    """gx and gw in 64 bits, for the factor f of each row."""
+    z = x.double() @ w.double().t() + (0 if b is None else b.double())
+    if t.is_floating_point():
+        pi = t.double()
+    else:
+        pi = torch.zeros_like(z)
+        live = t != -100
+        pi[live, t[live]] = 1.0
+    g = f[:, None] * (pi.sum(1, keepdim=True) * torch.softmax(z, 1) - pi)
+    return g @ w.double(), g.t() @ x.double()
+
+
+# (rows, features, classes, the caller asks for it)
+KEPT = [(129, 722, 362, False), (256, 162, 82, False), (1030, 722, 362, False), (4096, 722, 362, False), (2000, 100, 512, False), (40, 256, 3000, False),
+        (200, 100, 513, True), (1024, 512, 4096, True), (700, 65, 20000, True), (9000, 64, 33000, True), (300, 64, 40, True)]
+
+
+@pytest.mark.parametrize("size", KEPT, ids=ids)
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=ids)
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_gradients_as_near_as_their_type(size, dtype, dense, reduction):
+    """With G in 16 bits or more, the error of a gradient is what rounding it to its own type makes. G's rounding (2^-17 of a value against
+    2^-9 in bfloat16) and float32's sums add less than 3 % to its size; G in the type's own bits adds 6 to 60 %."""
+    rows, feats, classes, asked = size
+    if dense and rows * classes > 1 << 25:
+        pytest.skip("64-bit target weights of this size")
+    x, w, b, t = _loss_inputs(rows, feats, classes, dtype, dense, True)
+    f = torch.full((rows,), 64.0, device="cuda")
+    if reduction == "none":
+        f *= 0.5 + torch.rand(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    got = _loss_run(x, w, b, t, f if reduction == "none" else f[0], reduction=reduction, precise_gradient=asked)
+    for name, v, want in zip(("gx", "gw"), got[3:5], _loss_gradients(x, w, b, t, f)):
+        fine = want.abs() >= 2.0 ** -14 if dtype == F16 else torch.ones_like(want, dtype=torch.bool)     # below, float16 has fewer bits
+        own = float((want.to(dtype).double() - want)[fine].norm())
+        assert float((v.double() - want)[fine].norm()) <= 1.03 * own, (name, float((v.double() - want)[fine].norm()) / own)
+
+
+def test_precise_gradient_changes_nothing_else():
+    for dtype in DTYPES:
+        x, w, b, t = _loss_inputs(300, 96, 2000, dtype, False, True)
+        one, two = (_loss_run(x, w, b, t, entropy_coeff=0.01, precise_gradient=p) for p in (False, True))
+        for k in (0, 1, 2) if dtype != F32 else range(6):
+            assert torch.equal(one[k], two[k])
+        ref = R.loss_reference(x, w, t, b, c=0.01, grad=torch.ones((), device="cuda"))
+        for name, v in zip(("gx", "gw", "gb"), two[3:]):
+            R.close(name, v, ref[name])

@@ -128,3 +128,16 @@ def test_scratch_memory_of_the_loss_is_bounded():
                 weight = max(2 ** 29, 256 * features * size)        # of a piece of the classes, which has 256 at least
                 assert 0 < back <= 1.25 * 2 ** 30 + 2 * weight + 4 * x + 70 * classes, (dtype, rows, features, classes, pitch, back / 2 ** 30)
                 assert 0 < ahead <= 2 ** 25 + weight + 1.01 * x + 16 * (rows * classes / 32 + rows + classes), (dtype, rows, features, classes, pitch, ahead / 2 ** 30)
+
+
+def test_precise_gradient_of_the_c_entry_points():
+    """The flag goes with every reduction, and with nothing else; it takes the memory of a second plane."""
+    L = N.lib()
+    good = dict(x=256, weight=512, target=768, rows=4000, features=64, classes=3000, x_pitch=64, weight_pitch=64, ignore_index=-100, dtype=N.AZ_DT_BF16)
+    for reduction in (N.AZ_REDUCE_NONE, N.AZ_REDUCE_MEAN, N.AZ_REDUCE_SUM):
+        plain, precise = (N.AzLinearCeArgs(reduction=reduction | flag, **good) for flag in (0, N.AZ_PRECISE_GRADIENT))
+        assert L.az_linear_ce_workspace(C.byref(plain), 0) == L.az_linear_ce_workspace(C.byref(precise), 0) > 0
+        more = L.az_linear_ce_workspace(C.byref(precise), 1) - L.az_linear_ce_workspace(C.byref(plain), 1)
+        assert more >= 4 * 4000 * 3000 * 0.99       # G and its transpose
+    for reduction in (3, 3 | N.AZ_PRECISE_GRADIENT, 8, -1, 8 | N.AZ_PRECISE_GRADIENT):
+        assert L.az_linear_ce_workspace(C.byref(N.AzLinearCeArgs(reduction=reduction, **good)), 0) == N.AZ_ERR_ARG
