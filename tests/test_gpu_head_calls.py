@@ -181,3 +181,68 @@ def test_precise_gradient_changes_nothing_else():
         ref = R.loss_reference(x, w, t, b, c=0.01, grad=torch.ones((), device="cuda"))
         for name, v in zip(("gx", "gw", "gb"), two[3:]):
             R.close(name, v, ref[name])
+
+
+# ------------------------------------------------------------------------------------------------ several pieces of the classes
+def _scratch(rows, feats, classes, dtype, dense, reduction, precise=False):
+    """Bytes of scratch memory of the forward and of the backward pass."""
+    import ctypes as C
+    from alphazero_amd import _native as N
+    code = {"none": N.AZ_REDUCE_NONE, "mean": N.AZ_REDUCE_MEAN, "sum": N.AZ_REDUCE_SUM}[reduction] | (N.AZ_PRECISE_GRADIENT if precise else 0)
+    a = N.AzLinearCeArgs(x=256, weight=512, target=768, rows=rows, features=feats, classes=classes, x_pitch=feats, weight_pitch=feats, target_pitch=classes,
+                         ignore_index=-100, dtype={F32: N.AZ_DT_F32, BF16: N.AZ_DT_BF16, F16: N.AZ_DT_F16}[dtype], target_dense=dense, reduction=code)
+    return [N.lib().az_linear_ce_workspace(C.byref(a), k) for k in (0, 1)]
+
+
+def _pieces(rows, feats, classes, dtype, dense, reduction, precise=False):
+    """(forward, backward): at least so many pieces of the classes, from the scratch memory, which would hold the copies of the weight (forward) or
+    G and its transpose (backward) of all classes were there one piece."""
+    ahead, back = _scratch(rows, feats, classes, dtype, dense, reduction, precise)
+    planes = 2 if dtype == F32 else 1
+    copied = classes * feats * 2 * planes if dtype == F32 or feats % 8 else 0
+    g = classes * rows * 4 * (2 if dtype == F32 or rows <= 128 or precise else 1)
+    return math.ceil(copied / ahead), math.ceil((g + classes * feats * 2 * planes + copied) / back)
+
+
+# G's bytes make the pieces, with one and two planes; the weight's copies do, in both passes, with few and many rows
+PIECES = [(2800, 16, 100003, F32, False, "mean", False, 1, 3), (2800, 24, 60001, F32, True, "none", False, 1, 2), (8200, 16, 70001, BF16, False, "none", False, 0, 3),
+          (8200, 16, 40001, F16, False, "sum", False, 0, 2), (4200, 40, 70000, BF16, False, "mean", True, 0, 3), (9000, 33, 33001, F16, True, "none", False, 1, 2),
+          (50, 8192, 33001, F32, False, "none", False, 3, 2), (50, 8192, 20001, F32, True, "mean", False, 2, 2), (200, 4100, 40001, F32, False, "mean", False, 2, 2),
+          (70, 8191, 40001, BF16, False, "mean", False, 2, 2), (300, 8191, 40001, F16, True, "none", False, 2, 2), (100, 4095, 70001, BF16, True, "none", False, 2, 2),
+          (60, 4096, 140001, F16, False, "none", False, 0, 2), (300, 4096, 140001, BF16, False, "none", False, 0, 2)]
+
+
+@pytest.mark.parametrize("case", PIECES, ids=ids)
+def test_several_pieces_of_the_classes(case):
+    """Against the 64-bit form: packed weights and in-place ones, per-row gradients, target weights with entropy and bias, split sums that go on
+    from the piece before."""
+    rows, feats, classes, dtype, dense, reduction, precise, ahead, back = case
+    got = _pieces(rows, feats, classes, dtype, dense, reduction, precise)
+    assert got[0] >= ahead and got[1] >= back, got
+    _check_pieces(rows, feats, classes, dtype, dense, reduction, precise)
+
+
+# a weight that is read in place, one that is copied, and planes of float32: pieces of 131072, 65536 and 16384 classes
+@pytest.mark.parametrize("case", [(300, 4096, 131072, F16, False, "mean"), (100, 4095, 65536, BF16, True, "none"), (50, 8192, 16384, F32, False, "none")], ids=ids)
+@pytest.mark.parametrize("more", [0, 1])
+def test_one_class_more_than_a_piece(case, more):
+    rows, feats, classes, *rest = case
+    sums = rows * feats * 4        # of dx, which go from piece to piece: that is what one class more has to bring
+    assert _scratch(rows, feats, classes + 1, *rest)[1] - _scratch(rows, feats, classes, *rest)[1] >= sums
+    assert _scratch(rows, feats, classes, *rest)[1] - _scratch(rows, feats, classes - 1, *rest)[1] < sums
+    _check_pieces(rows, feats, classes + more, *rest)
+
+
+def _check_pieces(rows, feats, classes, dtype, dense, reduction, precise=False):
+    x, w, b, t = _loss_inputs(rows, feats, classes, dtype, dense, True)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    grad = (0.5 + torch.rand(rows, generator=g, device="cuda")) * 64 if reduction == "none" else torch.tensor(64.0, device="cuda")
+    c = 0.01 if dense else 0.0
+    out = _loss_run(x, w, b, t, grad, reduction=reduction, entropy_coeff=c, precise_gradient=precise)
+    ref = R.loss_reference(x, w, t, b, c=c, reduction=reduction, grad=grad)
+    counts = torch.ones(rows, dtype=torch.bool, device="cuda") if dense else t != -100
+    for name, v in zip(("loss", "ce", "ent", "gx", "gw", "gb"), out):
+        if name in ("loss", "ce", "ent") and v.dim():
+            R.close(name, v[counts], (ref[name][0][counts], ref[name][1][counts]))
+        else:
+            R.close(name, v, ref[name])
