@@ -4,8 +4,8 @@ in 8-bit integers with a scale for each token and channel.
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the tensors' device; there is no CPU
 fallback. Upstream computes the loss from stored logits (go_zero/train.py:537-541) and has no counterpart of the other two.
-Derivatives are reverse-mode ones: a dual tensor (torch.autograd.forward_ad) is refused, and so is a call under torch.jit.trace or
-make_fx, whose record would lack the kernels; torch.cuda.graph captures them."""
+Derivatives are first ones in reverse mode: a dual tensor (torch.autograd.forward_ad) is refused, and a second derivative raises. So does
+a call under torch.jit.trace or make_fx, whose record would lack the kernels; torch.cuda.graph captures them."""
 from __future__ import annotations
 
 import ctypes as C
@@ -117,28 +117,47 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, *_parts):
         if grad is None:
             return (None,) * 9
         x, weight, bias, target, kept = ctx.saved_tensors
-        a = _ce_args(x, weight, bias, target, *ctx.args)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = x.device
-        grad = grad.to(torch.float32).contiguous()
-        gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
-        gb = torch.empty(bias.shape, dtype=x.dtype, device=dev) if bias is not None and need_b else None
-        if not x.shape[0]:
-            for g in (gw, gb):
-                if g is not None:
-                    g.zero_()
-            return gx, gw, gb, None, None, None, None, None, None
-        r = C.byref(a)
-        size = N.check(N.lib().az_linear_ce_workspace(r, 1), "az_linear_ce_workspace")
-        ws = _scratch(size, dev)
-        _native(dev, "az_linear_ce_backward", r, kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), size, _stream(dev))
-        return gx, gw, gb, None, None, None, None, None, None
+        with torch.no_grad():
+            found = _ce_backward(x, weight, bias, target, kept, grad, ctx.args, ctx.needs_input_grad[:3])
+        if torch.is_grad_enabled():        # create_graph: the gradients depend on all of these
+            found = tuple(None if g is None else _NoSecondDerivative.apply(g, grad, x, weight, bias) for g in found)
+        return (*found, None, None, None, None, None, None)
+
+
+def _ce_backward(x, weight, bias, target, kept, grad, args, need):
+    a = _ce_args(x, weight, bias, target, *args)
+    need_x, need_w, need_b = need
+    dev = x.device
+    grad = grad.to(torch.float32).contiguous()
+    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
+    gb = torch.empty(bias.shape, dtype=x.dtype, device=dev) if bias is not None and need_b else None
+    if not x.shape[0]:
+        for g in (gw, gb):
+            if g is not None:
+                g.zero_()
+        return gx, gw, gb
+    r = C.byref(a)
+    size = N.check(N.lib().az_linear_ce_workspace(r, 1), "az_linear_ce_workspace")
+    ws = _scratch(size, dev)
+    _native(dev, "az_linear_ce_backward", r, kept.data_ptr(), grad.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), size, _stream(dev))
+    return gx, gw, gb
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """A gradient that says so when it is differentiated, instead of being taken for a constant."""
+
+    @staticmethod
+    def forward(ctx, g, *depends):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        raise NotImplementedError("linear_cross_entropy has no second derivative")
 
 
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100, reduction: str = "mean", entropy_coeff: float = 0.0,

@@ -246,3 +246,30 @@ def _check_pieces(rows, feats, classes, dtype, dense, reduction, precise=False):
             R.close(name, v[counts], (ref[name][0][counts], ref[name][1][counts]))
         else:
             R.close(name, v, ref[name])
+
+
+# ------------------------------------------------------------------------------------------------ derivatives of derivatives
+@pytest.mark.parametrize("dense", [False, True], ids=["index", "dense"])
+def test_a_second_derivative_is_refused(dense):
+    """create_graph gives the first derivatives; what is differentiated again raises, where it would be taken for a constant."""
+    head = _head()
+    x, w, b, t = _loss_inputs(40, 64, 90, F32, dense, True)
+    want = _loss_run(x, w, b, t)[3:]
+    for k in range(3):
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        loss = head.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        for g, v in zip(grads, want):
+            assert torch.equal(g, v)
+        with pytest.raises(NotImplementedError, match="second derivative"):
+            (loss + grads[k].square().sum()).backward()
+        other = (leaves[0] ** 3).sum()              # a second derivative of something else in the same graph
+        loss = head.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        g, = torch.autograd.grad(other + loss, leaves[1 - k % 2], create_graph=True)
+        assert g.requires_grad
+    xs = x.clone().requires_grad_(True)
+    factor = torch.ones((), device="cuda", requires_grad=True)
+    y = head.dropout(xs, 0.25, 3)
+    g, = torch.autograd.grad(y.sum() * factor, xs, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
