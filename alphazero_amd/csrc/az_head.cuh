@@ -9,8 +9,8 @@
 // Forward: one product whose tiles end in a few sums per row (Part), joined per row by a second kernel. Backward: the classes in pieces;
 // per piece the logits are made again, turned into G (16 bits, in both orientations), and two products take it to dx and dW. Bound
 // by the matrix instructions: 2 N V D forward, 6 N V D backward. 8192 rows, 4096 features, 131072 classes, bfloat16: logits and their
-// sums 6.5 ms (1.35 PFLOP/s), G 7.4 ms (of which 0.9 ms are its 4.3 GB), dx and dW 13.1 ms (1.35 PFLOP/s), copies of W^T 0.4 ms
-// (5.3 TB/s), joining 0.03 ms.
+// sums 6.5 to 6.9 ms by box (1.35 PFLOP/s), G 7.4 to 7.7 ms (of which 0.9 ms are its 4.3 GB), dx and dW 13.1 to 13.3 ms (1.35 PFLOP/s),
+// copies of W^T 0.4 ms (5.3 TB/s), joining 0.03 ms.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -980,8 +980,9 @@ void operand_layout(const az_linear_ce_args& a, Layout& l) {
     l.split = a.dtype == AZ_DT_F32;
     l.planes = l.split ? 2 : 1;
     // Where a handful of values is most of G, the rounding of each to 16 bits shows in the gradients. Their error against what the rounding of
-    // the gradients themselves makes: 1.6 with up to 40 rows, 1.45 with 100; 1.4 with 362 classes and target weights whatever the
-    // rows, 1.2 with 512 and class indices, 1.18 with 2048 to 4096, 1.06 to 1.13 with 32000. With two planes of G it is 1.0 everywhere.
+    // the gradients themselves makes: 1.6 with up to 40 rows, 1.45 with 100; beyond, with target weights 1.4 at 362
+    // classes, 1.36 at 600, 1.25 at 2000, 1.05 to 1.15 at 20000, with class indices 1.2 at 512, 1.1 to 1.18 at 4000, 1.01 to 1.13 at
+    // 20000 to 32000 (less in bfloat16). With two planes of G it is 1.0 everywhere.
     // They cost, in both passes together, 8 to 20 % with up to 128 rows (64 x 4096 -> 4096 bfloat16 77 and 91 us, 64 x 722 -> 362 34 and
     // 39), 7 to 17 % with up to 512 classes (256 x 162 -> 82 float16 36.8 and 39.4, 4096 x 722 -> 362 80 and 89, 16384 x 722 -> 362 176
     // and 201, 16384 x 256 -> 512 115 and 131), and from 13 % to twice the time beyond (4096 x 256 -> 2048 87 and 103, 1024 x 1024 -> 4096 99

@@ -4,7 +4,7 @@
 //   y_mn = s_m w_n sum_k q_mk Q_nk + b_n        (the sum in 32-bit integers: exact, whatever its order)
 //
 // Many tokens: the tile loop of az_gemm.cuh, bound by the matrix instructions and LDS (8192^3 in 430 to 520 us by box, 2.1 to 2.5 POP/s,
-// quantising 50 us). Few tokens (up to 64): bound by the bytes of Q, which stream from memory to registers once.
+// quantising 42 to 50 us). Few tokens (up to 48): bound by the bytes of Q, which stream from memory to registers once.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -90,7 +90,7 @@ __device__ __forceinline__ void quantize_chunk(const float (&v)[NV], const Range
 }
 
 // LANES threads per row (up to 64, or a workgroup), HELD chunks per thread stay in registers between the maximum and the quotients; a longer row is read again (from
-// L2). Up to 64 lanes the maximum needs no barrier. Bound by memory: 8192 x 8192 bfloat16 in 40 us (5.0 TB/s).
+// L2). Up to 64 lanes the maximum needs no barrier. Bound by memory: 8192 x 8192 bfloat16 in 42 us (4.8 TB/s).
 template <int DT, int LANES, int HELD>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_quantize(QuantArgs a) {
     static_assert(LANES <= 64 || LANES >= 256, "the waves of a row are a workgroup");
@@ -600,7 +600,7 @@ void run_tiles(const TileArgs& t, hipStream_t st) {
 
 // Up to FEW_TOKENS tokens. The waves of a workgroup that share 16 channels are as many as leave one round of workgroups: with up to 16 tokens
 // a compute unit holds one (80 registers in 16 waves), and a second round for the last few doubles the time (1 x 4096 -> 6000 bfloat16: 8.3
-// us, with 376 workgroups of more sharing 14.3; 16 x 2048 -> 16000 int8 8.5 and 14.4). With more tokens it holds two, and one round of 256 is
+// us, with 375 workgroups of more sharing 14.3; 16 x 2048 -> 16000 int8 8.5 and 14.4). With more tokens it holds two, and one round of 256 is
 // as fast as one of 512 (48 x 2048 -> 8192 10.4 and 10.2, 48 x 512 -> 16000 7.4 and 10.4).
 template <int DT, int DX>
 int few(const az_int8_args& a, const void* x, int64_t x_pitch, const Scales& s, hipStream_t st) {

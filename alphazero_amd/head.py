@@ -173,8 +173,8 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     An index outside 0..classes-1 that is not ignore_index gives a NaN loss and NaN gradients (the check is on the device, nothing
     waits for it). Everything is accumulated in float32; between the products of the backward pass the gradient of the logits keeps
     22 bits for float32 inputs. For 16-bit ones it keeps 16 bits or more with up to 128 rows or 512 classes and is rounded to the
-    inputs' type beyond, which adds 6 to 20 % to the error that rounding the results makes; precise_gradient=True keeps 16 bits or more
-    there too, in up to twice the time.
+    inputs' type beyond, which adds up to 20 % to the error that rounding the results makes, with target weights up to 35 %;
+    precise_gradient=True keeps 16 bits or more there too, in up to twice the time.
 
     float32 gradients: with more than 16 rows the sums over the classes (for x) and over the rows (for the weight) hold weight and x to
     22 bits each, and to 2^-49 of that matrix' largest value: values below 2^-27 of the largest lose bits.
@@ -266,7 +266,8 @@ def dropout(x, p: float, seed, offset: int = 0, *, residual=None):
 # ------------------------------------------------------------------------------------------------ 8-bit integers
 def quantize_rows(x):
     """(q int8 [..., n], scale float32 [...]) with x ~ q * scale: scale = max|row| / 127, q = the nearest whole number of
-    127 x / max|row| (ties to even). A row of zeros has scale 0; a row with an infinity or NaN has q = 0 and scale NaN."""
+    127 x / max|row| (ties to even). A row of zeros has scale 0; a row with an infinity or NaN has q = 0 and scale NaN. Neither
+    has a gradient."""
     _on_gpu("quantize_rows", x)
     _need(x.dtype in _DTYPES, f"x is float32, bfloat16 or float16, not {x.dtype}")
     _need(x.dim() >= 1 and x.shape[-1] >= 1, "a row has at least one element")

@@ -36,7 +36,7 @@ def loss_reference(x, w, target, bias, ignore=-100, c=0.0, reduction="mean", gra
     ent = -plogp.sum(1)
     row = torch.where(counts, ce - c * ent, 0.0)
     n = counts.sum().double()
-    # a logit's error: the sum's, float32's three planes cover 2^-22 of each product, the bias is added in float32
+    # a logit's error: the sum's, float32's two planes cover 2^-22 of each product, the bias is added in float32
     mag = xd.abs() @ wd.abs().t()
     fine = torch.where(torch.isfinite(bd), bd.abs(), 0.0)
     ez = ((feats + 8) * F32 + (2.0 ** -22 if dt == torch.float32 else 0.0)) * mag + 2 * F32 * (mag + fine)
@@ -55,7 +55,7 @@ def loss_reference(x, w, target, bias, ignore=-100, c=0.0, reduction="mean", gra
     f = torch.where(counts, (grad.double() if reduction == "none" else grad.double().expand(rows)) / d, 0.0)
     inner = c * (plogp + p * ent[:, None])
     g = torch.where(counts[:, None], (total[:, None] * p - pi + inner) * f[:, None], 0.0)
-    # of G: its terms in float32, then its rounding (three planes for float32)
+    # of G: its terms in float32, then its rounding (two planes for float32)
     terms = total[:, None].abs() * p + pi.abs() + abs(c) * (plogp.abs() + p * ent[:, None].abs())
     ep = p * (2 * eo[:, None] + 2.0 ** -22 * (2 + torch.where(torch.isfinite(logp), logp.abs(), 0.0)))
     lp = torch.where(torch.isfinite(logp), logp.abs(), 0.0)

@@ -157,7 +157,7 @@ KEPT = [(129, 722, 362, False), (256, 162, 82, False), (1030, 722, 362, False), 
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 def test_gradients_as_near_as_their_type(size, dtype, dense, reduction):
     """With G in 16 bits or more, the error of a gradient is what rounding it to its own type makes. G's rounding (2^-17 of a value against
-    2^-9 in bfloat16) and float32's sums add less than 3 % to its size; G in the type's own bits adds 6 to 60 %."""
+    2^-9 in bfloat16) and float32's sums add less than 3 % to its size; G in the type's own bits adds up to 60 %."""
     rows, feats, classes, asked = size
     if dense and rows * classes > 1 << 25:
         pytest.skip("64-bit target weights of this size")
