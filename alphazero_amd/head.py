@@ -153,7 +153,8 @@ class _NoSecondDerivative(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, g, *depends):
-        return g.view_as(g)
+        ctx.mark_dirty(g)        # the same tensor, with this node behind it: a view could not be changed in place
+        return g
 
     @staticmethod
     def backward(ctx, *_grads):

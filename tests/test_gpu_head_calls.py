@@ -263,10 +263,14 @@ def test_a_second_derivative_is_refused(dense):
             assert torch.equal(g, v)
         with pytest.raises(NotImplementedError, match="second derivative"):
             (loss + grads[k].square().sum()).backward()
+        with torch.no_grad():                       # clipping, say
+            assert torch.equal(grads[k].mul_(0.5), 0.5 * want[k])
+        assert torch.equal((grads[k] * 2).detach(), want[k])
         other = (leaves[0] ** 3).sum()              # a second derivative of something else in the same graph
         loss = head.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
         g, = torch.autograd.grad(other + loss, leaves[1 - k % 2], create_graph=True)
         assert g.requires_grad
+        g.mul_(2.0)
     xs = x.clone().requires_grad_(True)
     factor = torch.ones((), device="cuda", requires_grad=True)
     y = head.dropout(xs, 0.25, 3)
