@@ -19,9 +19,8 @@
 //
 // float32 operands come as two float16 planes, v = h + m / 2048 (split2), scaled by powers of two beforehand. k is walked three times,
 // first with the plane pairs (h, m) and (m, h), whose sum is then divided by 2048, then with (h, h); (m, m) / 2^22 is below
-// 2^-24 of the result and left out. Each product keeps 22 bits or more, of values down to 2^-27 of the largest with the same scale; the sum is
-// float32's: 2.5 PFLOP/s / 3 against the 0.16
-// PFLOP/s of the float32 matrix instructions.
+// 2^-24 of the result and left out. Each product keeps 22 bits or more, of values down to 2^-27 of the largest with the same scale; the
+// sum is float32's: 2.5 PFLOP/s / 3 against the 0.16 PFLOP/s of the float32 matrix instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -43,7 +42,7 @@ struct MmOperand {
     int64_t pitch;       // bytes between rows, a multiple of 16, at most MM_MAX_PITCH
     int64_t plane;       // bytes between the planes of a split float32 operand
     int32_t rows;
-    int32_t short_by;    // bytes that the last row lacks of kbytes (fewer than 16): they are not read and count as zero
+    int32_t short_by;    // bytes that the last row lacks of kbytes (whole 4 bytes, fewer than 16): they are not read and count as zero
 };
 constexpr int64_t MM_MAX_PITCH = (int64_t(1) << 31) / 256 - 16;   // 256 rows of a tile stay below 2^31 bytes
 

@@ -133,7 +133,8 @@ __device__ __forceinline__ void pack_block(const PackJob& j, int64_t block, floa
 
 // The same, transposed: dst row c = column c of the source, rows behind the last one (up to the pitch, a multiple of 128 bytes) zero. The
 // products' sums run over the source's rows here, so all of float32 is divided by what the largest row is (`all`): every value keeps 22
-// bits down to 2^-27 of the largest, and what is left above 2^-49 of it below that. Rows that do not count become zeros, so that whatever a padded row holds - NaN included - stays out of dW. 64 x 64 elements per
+// bits down to 2^-27 of the largest, and what is left above 2^-49 of it below that. Rows that do not count become zeros, so that
+// whatever a padded row holds - NaN included - stays out of dW. 64 x 64 elements per
 // workgroup through LDS.
 struct TurnJob {
     const void* src;

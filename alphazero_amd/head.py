@@ -177,8 +177,8 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     inputs' type beyond, which adds up to 20 % to the error that rounding the results makes, with target weights up to 35 %;
     precise_gradient=True keeps 16 bits or more there too, in up to twice the time.
 
-    float32 gradients: with more than 16 rows the sums over the classes (for x) and over the rows (for the weight) hold weight and x to
-    22 bits each, and to 2^-49 of that matrix' largest value: values below 2^-27 of the largest lose bits.
+    float32 gradients, but for up to 16 rows of a large weight: the sums over the classes (for x) and over the rows (for the weight) hold
+    weight and x to 22 bits each, and to 2^-49 of that matrix' largest value, so values below 2^-27 of the largest lose bits.
 
     Scratch memory of the backward pass: up to 2 GB whatever the number of classes, 6 to 8 bytes for each element of x (float32: 12), and with
     up to 16 rows 64 bytes for each class. Of the forward pass: for float32, and for rows that are not a multiple of 16 bytes, a copy of x and up
