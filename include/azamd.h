@@ -344,15 +344,16 @@ typedef enum { AZ_REDUCE_NONE = 0, AZ_REDUCE_MEAN = 1, AZ_REDUCE_SUM = 2, AZ_PRE
 
 /* Cross entropy of softmax(x weight^T + bias) against class indices or against rows of target weights, minus entropy_coeff times
  * the softmax' entropy; the logits are never stored (up to 8 MB of partial sums of few of them are). Rows whose index is
- * ignore_index cost nothing, get zero gradients and stay out of the mean; an index outside 0..classes-1 that is not ignore_index makes its row's loss and every gradient NaN. A logit of
- * -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax and gives NaN. The gradient of the logits is
- * held in 16 bits between the products (in two planes, 16 bits or more, for float32, for up to 128 rows or 512 classes, and for any size
- * with AZ_PRECISE_GRADIENT or-ed into the reduction, which can double the backward pass' time), relative to the largest sum of target
- * weights of a row: with float16, rows whose weights sum to less than 2^-16 of the largest lose bits. Infinite features or weights give
- * NaN with float32. The backward pass makes the logits again, where that is faster by another kernel than the forward pass: their rounding (2^-22 of a logit and more) is in its
- * softmax, so rows with logits beyond some 10^5 get gradients of a few bits; never a p above one. float32 gradients hold weight (in
- * grad_x's sums over the classes) and x (in grad_weight's over the rows) to 22 bits and to 2^-49 of that matrix' largest value, so values
- * below 2^-27 of the largest lose bits there; the loss and the softmax scale every row by itself. */
+ * ignore_index cost nothing, get zero gradients and stay out of the mean; an index outside 0..classes-1 that is not ignore_index makes
+ * its row's loss and every gradient NaN. A logit of -inf (from the bias) is a class that cannot be; a row of nothing else has no softmax
+ * and gives NaN. The gradient of the logits is held in 16 bits between the products (in two planes, 16 bits or more, for float32, for up
+ * to 128 rows or 512 classes, and for any size with AZ_PRECISE_GRADIENT or-ed into the reduction, which can double the backward pass'
+ * time), relative to the largest sum of target weights of a row: with float16, rows whose weights sum to less than 2^-16 of the largest
+ * lose bits. Infinite features or weights give NaN with float32. The backward pass makes the logits again, where that is faster by another
+ * kernel than the forward pass: their rounding (2^-22 of a logit and more) is in its softmax, so rows with logits beyond some 10^5 get
+ * gradients of a few bits; never a p above one. float32 gradients hold weight (in grad_x's sums over the classes) and x (in grad_weight's
+ * over the rows) to 22 bits and to 2^-49 of that matrix' largest value, so values below 2^-27 of the largest lose bits there; the loss
+ * and the softmax scale every row by itself. */
 typedef struct {
     const void* x;            /* [rows, features] of dtype */
     const void* weight;       /* [classes, features] of dtype */
