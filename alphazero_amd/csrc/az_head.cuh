@@ -9,7 +9,7 @@
 // Forward: one product whose tiles end in a few sums per row (Part), joined per row by a second kernel. Backward: the classes in pieces;
 // per piece the logits are made again, turned into G (16 bits, in both orientations), and two products take it to dx and dW. Bound
 // by the matrix instructions: 2 N V D forward, 6 N V D backward. 8192 rows, 4096 features, 131072 classes, bfloat16: logits and their
-// sums 6.5 to 6.9 ms by box (1.35 PFLOP/s), G 7.4 to 7.7 ms (of which 0.9 ms are its 4.3 GB), dx and dW 13.1 to 13.3 ms (1.35 PFLOP/s),
+// sums 6.5 to 6.9 ms by card (1.35 PFLOP/s), G 7.4 to 7.7 ms (of which 0.9 ms are its 4.3 GB), dx and dW 13.1 to 13.3 ms (1.35 PFLOP/s),
 // copies of W^T 0.4 ms (5.3 TB/s), joining 0.03 ms.
 #pragma once
 #include <hip/hip_runtime.h>

@@ -3,7 +3,7 @@
 //
 // Forward: the weight streams once, from memory to the matrix instructions' registers, with no copy and no LDS in between; rows may
 // start anywhere. float32 uses the float32 matrix instruction (0.16 PFLOP/s, which is more than the memory feeds with 16 rows).
-// 1 x 4096 -> 131072 bfloat16: 187 us (5.7 TB/s); 5 x 3765 -> 52111 float32: 219 to 233 us by box (3.4 to 3.6 TB/s).
+// 1 x 4096 -> 131072 bfloat16: 187 us (5.7 TB/s); 5 x 3765 -> 52111 float32: 219 to 233 us by card (3.4 to 3.6 TB/s).
 // Backward: the logits are made again the same way and become G [classes][16] in float32; then one pass reads the weight, adds G W
 // to dx in registers and writes dW = G^T x. That is three reads of the weight in all and one write of its gradient.
 // Included by az_head.cuh.

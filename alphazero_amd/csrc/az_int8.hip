@@ -3,7 +3,7 @@
 //   q_mk = rint(127 x_mk / max_k |x_mk|) (ties to even), s_m = max_k |x_mk| / 127
 //   y_mn = s_m w_n sum_k q_mk Q_nk + b_n        (the sum in 32-bit integers: exact, whatever its order)
 //
-// Many tokens: the tile loop of az_gemm.cuh, bound by the matrix instructions and LDS (8192^3 in 430 to 520 us by box, 2.1 to 2.5 POP/s,
+// Many tokens: the tile loop of az_gemm.cuh, bound by the matrix instructions and LDS (8192^3 in 430 to 520 us by card, 2.1 to 2.5 POP/s,
 // quantising 42 to 50 us). Few tokens (up to 48): bound by the bytes of Q, which stream from memory to registers once.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
