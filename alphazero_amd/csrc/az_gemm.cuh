@@ -9,7 +9,7 @@
 // a matrix are turned into zeros by the buffer descriptor's range check, so ragged sizes need no other code.
 //
 // Measured with the 256 x 256 tile of 8 waves: 8192 x 8192 results over 4096 bfloat16 1.43 PFLOP/s, over 8192 int8 2.2 to 2.6 POP/s by
-// box (power). A step takes 2912 cycles at the 2.05 GHz that the power limit leaves, 2048 of them the matrix instruction's; without the
+// card (power). A step takes 2912 cycles at the 2.05 GHz that the power limit leaves, 2048 of them the matrix instruction's; without the
 // fetches the loop reaches 1.83, without the fragment reads 1.6 PFLOP/s. 64-byte steps in 3 to 5 stages: 1.36. Four waves of 128 x 128,
 // which read a third less from LDS, have nobody to hide their waits: 1.25. Left to the compiler's order of reads and products: 1.41.
 //
